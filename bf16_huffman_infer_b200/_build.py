@@ -30,6 +30,14 @@ NVCC_FLAGS = [
 ]
 
 
+# files whose 32-bit arithmetic keeps subnormal values and takes the fast functions only where it names them
+EXACT_UNITS = ("bhi_mxfp4",)
+
+
+def _unit_flags(unit: str):
+    return [f for f in NVCC_FLAGS if f != "--use_fast_math" or not os.path.basename(unit).startswith(EXACT_UNITS)]
+
+
 def _newer(target: str, sources) -> bool:
     if not os.path.exists(target):
         return False
@@ -62,7 +70,7 @@ def build_library(force: bool = False) -> str:
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(units)) as pool:      # the files take minutes each
         objects = [os.path.join(tmp, os.path.basename(u)[:-3] + ".o") for u in units]
         logs = [os.path.basename(u)[:-3] + ".log" for u in units]
-        list(pool.map(lambda u, o, log: _run([_nvcc(), *NVCC_FLAGS, "-c", "-o", o, u], log), units, objects, logs))
+        list(pool.map(lambda u, o, log: _run([_nvcc(), *_unit_flags(u), "-c", "-o", o, u], log), units, objects, logs))
         _run([_nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB_PATH, *objects], "build_lib.log")
     return LIB_PATH
 

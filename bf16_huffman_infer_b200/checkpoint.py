@@ -21,7 +21,8 @@ from safetensors import safe_open
 from safetensors.torch import save_file
 from torch import nn
 
-from .functional import (ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight, _FusedSlice)
+from .functional import (ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight, _FusedSlice, _is_gated_mlp)
+from .mxfp4 import GatedMLP, GatedMXFP4, MXFP4Weight
 
 __all__ = ["save_compressed", "load_compressed", "compressed_manifest"]
 
@@ -29,6 +30,8 @@ _FORMAT = "bf16_huffman_infer_b200/1"
 
 
 def _weight_meta(w: HuffmanWeight) -> Dict:
+    if isinstance(w, MXFP4Weight):
+        return {"algo": w.algo, "shape": list(w.shape)}
     meta = {"algo": w.algo, "rem": list(w.rem.shape), "exp": int(w.exp.numel()), "offsets": list(w.offsets.shape)}
     if w.algo == "ans":
         meta["lut"] = int(w.LUT.numel())        # 2^precision table words
@@ -44,6 +47,9 @@ def compressed_manifest(model: nn.Module) -> Dict:
         elif isinstance(mod, FusedCompressedLinear):
             entries[name] = {"kind": "fused", "bias": mod.bias is not None, "splits": [list(s) for s in mod.splits],
                              **_weight_meta(mod.weight)}
+        elif isinstance(mod, GatedMLP):
+            entries[name] = {"kind": "gated", "bias": mod.gate_up.bias is not None, "activation": mod.gate_up.activation,
+                             **_weight_meta(mod.gate_up.weight)}
     slices = {}
     for name, mod in model.named_modules():
         if isinstance(mod, _FusedSlice):
@@ -68,6 +74,10 @@ def _validate(model: nn.Module, manifest: Dict) -> None:
     """The manifest must describe THIS model: every named module exists and is a linear layer of the shape the
     compressed buffers encode (``rem`` is ``[S, out_features, in_features / S]``)."""
     def check_shape(name: str, meta: Dict, out_features: int, in_features: int) -> None:
+        if meta.get("algo") == MXFP4Weight.algo:
+            if meta.get("shape") != [out_features, in_features]:
+                raise ValueError(f"checkpoint entry {name!r} does not fit a linear layer {in_features} -> {out_features}: {meta}")
+            return
         rem = meta.get("rem")
         if (meta.get("algo") not in ("huffman", "ans") or not isinstance(rem, list) or len(rem) != 3
                 or rem[1] != out_features or rem[0] * rem[2] != in_features
@@ -94,11 +104,21 @@ def _validate(model: nn.Module, manifest: Dict) -> None:
                                                for i in range(len(olds))] or len({o.in_features for o in olds}) != 1:
                 raise ValueError(f"stacked entry {name!r} does not match the layers it replaces")
             check_shape(name, meta, splits[-1][1], olds[0].in_features)
+        elif meta.get("kind") == "gated":
+            old = names.get(name)
+            act = None if old is None else _is_gated_mlp(old)
+            if act is None or act != meta.get("activation") or meta.get("algo") != MXFP4Weight.algo:
+                raise ValueError(f"checkpoint names {name!r}, which is not a feed-forward block with the activation {meta.get('activation')!r}")
+            check_shape(name, meta, 2 * old.gate_proj.out_features, old.gate_proj.in_features)
         else:
             raise ValueError(f"unknown entry kind in checkpoint: {meta.get('kind')!r}")
 
 
 def _empty_weight(meta: Dict) -> HuffmanWeight:
+    if meta["algo"] == MXFP4Weight.algo:
+        M, K = meta["shape"]
+        tiles, groups = (M + 15) // 16, (K + 127) // 128
+        return MXFP4Weight(torch.empty(tiles, groups, 16, 64, dtype=torch.uint8), torch.empty(tiles, groups, 16, 4, dtype=torch.uint8), M, K)
     rem = torch.empty(meta["rem"], dtype=torch.uint8)
     exp = torch.empty(meta["exp"], dtype=torch.int32)
     offsets = torch.empty(meta["offsets"], dtype=torch.int32)
@@ -121,7 +141,13 @@ def load_compressed(model: nn.Module, path: str, strict: bool = True) -> nn.Modu
         state = {k: f.get_tensor(k) for k in f.keys()}
     _validate(model, manifest)
     owners = {}
+    for name, meta in manifest["modules"].items():             # blocks before the projections inside them
+        if meta["kind"] == "gated":
+            bias = nn.Parameter(torch.empty(meta["shape"][0], dtype=state[name + ".gate_up.bias"].dtype), requires_grad=False) if meta["bias"] else None
+            model.set_submodule(name, GatedMLP(GatedMXFP4(_empty_weight(meta), bias, meta["activation"]), model.get_submodule(name).down_proj))
     for name, meta in manifest["modules"].items():
+        if meta["kind"] == "gated":
+            continue
         weight = _empty_weight(meta)
         if meta["kind"] == "linear":
             old = model.get_submodule(name)

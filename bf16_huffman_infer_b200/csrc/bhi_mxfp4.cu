@@ -1,0 +1,300 @@
+// 4-bit microscaled weights: quantisation, the dense matrix, products.
+#include "bhi_mxfp4.cuh"
+
+namespace bhi {
+
+// ---- quantisation ----------------------------------------------------------------------------------------------------
+// Per block of 32: e = floor(log2 max|v|) - 2 (the largest code is 6 = 1.5 * 2^2), not below -127; codes are v / 2^e rounded to the
+// nearest, ties to the even code, saturated at 6.  A power of two divides exactly, subnormal values included, and the
+// hardware's conversion rounds and saturates so: every code is the format's own.  A block with an infinity or a NaN is NaN.
+//
+// A thread makes one word (8 values), the four threads of a block share its maximum; a warp reads 256 values of a row in one
+// piece and writes two 64-byte pieces.  Bound by memory: read once, written once.
+template <class T>
+__device__ __forceinline__ void mx_load8(const T *p, uint32_t (&bits)[8]);
+template <>
+__device__ __forceinline__ void mx_load8<__nv_bfloat16>(const __nv_bfloat16 *p, uint32_t (&bits)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        bits[2 * i] = w[i] << 16;
+        bits[2 * i + 1] = w[i] & 0xFFFF0000u;
+    }
+}
+template <>
+__device__ __forceinline__ void mx_load8<__half>(const __half *p, uint32_t (&bits)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        bits[2 * i] = __float_as_uint(f16lo_to_f32(w[i]));
+        bits[2 * i + 1] = __float_as_uint(f16hi_to_f32(w[i]));
+    }
+}
+template <>
+__device__ __forceinline__ void mx_load8<float>(const float *p, uint32_t (&bits)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) bits[i] = w[i];
+}
+
+constexpr int kMxQuantThreads = 256;
+
+template <class T>
+__global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W, int M, int K, int groups, int64_t words, uint8_t *codes, uint8_t *scales) {
+    const int per_row = groups * 16;                                      // words of a row
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kMxQuantThreads + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * kMxQuantThreads) {
+        const int m = static_cast<int>(i / per_row), at = static_cast<int>(i % per_row);      // words is a multiple of 64: whole warps
+        uint32_t v[8] = {};
+        if (m < M && at * 8 < K) mx_load8(W + static_cast<int64_t>(m) * K + at * 8, v);
+        uint32_t top = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, v[j] & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const uint32_t field = top >> 23;                                 // floor(log2 top) + 127 of a normal value
+        const bool nan = field == 255u;
+        const uint32_t byte = nan ? 255u : field > 2u ? field - 2u : 0u;
+        const float inv = __uint_as_float((254u - byte) << 23);           // 2^(127 - byte); not used for a NaN
+        uint32_t word = 0u;
+        if (!nan) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = __uint_as_float(v[j]) * inv;
+            // bytes: (e0, e2) (e4, e6) (e1, e3) (e5, e7), the first in the low half
+            asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b0, %3, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %7, %5;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b2, %4, %2;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %6;\n\t"
+                "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+                : "=r"(word) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+        }
+        const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
+        const int64_t row = mx_code_row(m, groups);
+        *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4) = word;
+        if (t == 0) scales[mx_scale_row(m, groups) + g * kMxTileScales + j] = static_cast<uint8_t>(byte);
+    }
+}
+
+// ---- the dense matrix ------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, int64_t words, uint16_t *Y) {
+    const int per_row = W.K / 8;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kMxQuantThreads + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * kMxQuantThreads) {
+        const int m = static_cast<int>(i / per_row), at = static_cast<int>(i % per_row);
+        const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t *>(W.codes + mx_code_row(m, W.groups) + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4));
+        const float scale = mx_scale(__ldg(W.scales + mx_scale_row(m, W.groups) + g * kMxTileScales + j));
+        float v[8];
+        mx_word_to_f32(word, scale, v);
+        *reinterpret_cast<uint4 *>(Y + static_cast<int64_t>(m) * W.K + at * 8) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+}
+
+// ---- products: one value after another ---------------------------------------------------------------------------------
+__device__ __forceinline__ float mx_value(const MxWeight &W, int m, int k) {
+    const int g = k >> 7, j = (k >> 5) & 3, t = (k >> 3) & 3, e = k & 7;
+    const int nibble = (e >> 1) + (e & 1) * 4;
+    const uint32_t byte = W.codes[mx_code_row(m, W.groups) + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4 + (nibble >> 1)];
+    const uint32_t code = (byte >> ((nibble & 1) * 4)) & 15u;
+    uint32_t h[4];
+    mx_word_to_f16(code, h);
+    return f16lo_to_f32(h[0]) * mx_scale(W.scales[mx_scale_row(m, W.groups) + g * kMxTileScales + j]);
+}
+
+constexpr int kMxTile = 32;          // 32 x 32 outputs a block, 32 terms at a time
+
+// out[r][c] of a tile: sum over i of A(r, i) B(c, i), A rows of activations, B the weight (kGrad: B(c, i) = W[i][c])
+template <bool kGrad>
+__device__ __forceinline__ void mx_tile_sum(const MxWeight &W, const uint16_t *A, int64_t rows, int lda, int64_t r0, int c0, int cols, int terms, int w0,
+                                            float (&sa)[kMxTile][kMxTile + 1], float (&sb)[kMxTile][kMxTile + 1], float (&acc)[4]) {
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    for (int i0 = 0; i0 < terms; i0 += kMxTile) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int r = ty + 8 * q;
+            sa[r][tx] = (r0 + r < rows && i0 + tx < terms) ? __uint_as_float(static_cast<uint32_t>(A[(r0 + r) * lda + i0 + tx]) << 16) : 0.f;
+            if constexpr (kGrad) sb[r][tx] = (i0 + r < terms && c0 + tx < cols) ? mx_value(W, i0 + r, c0 + tx) : 0.f;
+            else sb[r][tx] = (c0 + r < cols && i0 + tx < terms) ? mx_value(W, w0 + c0 + r, i0 + tx) : 0.f;
+        }
+        __syncthreads();
+        for (int i = 0; i < kMxTile; i++) {
+            const float b = kGrad ? sb[i][tx] : sb[tx][i];
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc[q] = fmaf(sa[ty + 8 * q][i], b, acc[q]);
+        }
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ float bf16_at(const uint16_t *p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
+
+__global__ void __launch_bounds__(256) mx_linear_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, int64_t rows, int tiles_c) {
+    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
+    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
+    float acc[4] = {};
+    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, W.M, W.K, 0, sa, sb, acc);
+    for (int q = 0; q < 4; q++) {
+        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
+        if (r < rows && c < W.M) Y[r * W.M + c] = f32_to_bf16_rn(acc[q] + (bias ? bf16_at(bias, c) : 0.f));
+    }
+}
+
+__global__ void __launch_bounds__(256) mx_linear_grad_kernel(MxWeight W, const uint16_t *dY, int ldy, uint16_t *dX, int64_t rows, int tiles_c) {
+    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
+    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
+    float acc[4] = {};
+    mx_tile_sum<true>(W, dY, rows, ldy, r0, c0, W.K, W.M, 0, sa, sb, acc);
+    for (int q = 0; q < 4; q++) {
+        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
+        if (r < rows && c < W.K) dX[r * W.K + c] = f32_to_bf16_rn(acc[q]);
+    }
+}
+
+template <int kAct>
+__global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, uint16_t *H, float *pre, int64_t rows, int tiles_c) {
+    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
+    const int inter = W.M / 2;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
+    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
+    float g[4] = {}, u[4] = {};
+    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, inter, W.K, 0, sa, sb, g);
+    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, inter, W.K, inter, sa, sb, u);
+    for (int q = 0; q < 4; q++) {
+        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
+        if (r >= rows || c >= inter) continue;
+        if (bias) {
+            g[q] += bf16_at(bias, c);
+            u[q] += bf16_at(bias, inter + c);
+        }
+        H[r * inter + c] = f32_to_bf16_rn(mx_act<kAct>(g[q]) * u[q]);
+        if (pre) {
+            pre[r * W.M + c] = g[q];
+            pre[r * W.M + inter + c] = u[q];
+        }
+    }
+}
+
+// ---- the gated pair's gradient: dg = dh u act'(g), du = dh act(g) --------------------------------------------------------
+template <int kAct>
+__global__ void __launch_bounds__(256) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, uint16_t *dpre, int inter, int ldp, int64_t n) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / inter, c = i % inter;
+        const float g = pre[r * 2 * inter + c], u = pre[r * 2 * inter + inter + c], dh = bf16_at(dH, i);
+        float a, da;
+        mx_act_grad<kAct>(g, a, da);
+        dpre[r * ldp + c] = f32_to_bf16_rn(dh * u * da);
+        dpre[r * ldp + inter + c] = f32_to_bf16_rn(dh * a);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+static int mx_check(const void *codes, const void *scales, int M, int K) {
+    BHI_REQUIRE(codes && scales, "null weight buffer");
+    BHI_REQUIRE(M >= 1, "empty weight");
+    BHI_REQUIRE(K >= 32 && K % 32 == 0, "columns must be a multiple of 32");
+    BHI_REQUIRE(M <= BHI_MXFP4_MAX_DIM && K <= BHI_MXFP4_MAX_DIM, "weight dimension beyond the limit");
+    BHI_REQUIRE(aligned(codes, 16) && aligned(scales, 16), "weight buffers must be 16-byte aligned");
+    return BHI_OK;
+}
+static MxWeight mx_weight(const uint8_t *codes, const uint8_t *scales, int M, int K) { return {codes, scales, M, K, (K + kMxGroup - 1) / kMxGroup}; }
+
+static int mx_launched(const char *what) {
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? BHI_OK : cuda_fail(e, what);
+}
+static int mx_stream_grid(int64_t items, int threads) {
+    const int64_t blocks = (items + threads - 1) / threads, most = static_cast<int64_t>(sm_count()) * 16;
+    return static_cast<int>(blocks < most ? blocks : most);
+}
+
+}  // namespace bhi
+
+using namespace bhi;
+
+extern "C" {
+
+int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream) {
+    if (int rc = mx_check(codes, scales, M, K)) return rc;
+    BHI_REQUIRE(W && aligned(W, 16), "the matrix must be 16-byte aligned");
+    BHI_REQUIRE(dtype >= BHI_DTYPE_BF16 && dtype <= BHI_DTYPE_FP32, "unknown type");
+    const int groups = (K + kMxGroup - 1) / kMxGroup;
+    const int64_t words = static_cast<int64_t>((M + 15) / 16 * 16) * groups * 16;
+    const int grid = mx_stream_grid(words, kMxQuantThreads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+    case BHI_DTYPE_BF16: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const __nv_bfloat16 *>(W), M, K, groups, words, codes, scales); break;
+    case BHI_DTYPE_FP16: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const __half *>(W), M, K, groups, words, codes, scales); break;
+    default: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const float *>(W), M, K, groups, words, codes, scales); break;
+    }
+    return mx_launched("quantisation launch");
+}
+
+int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, uint16_t *Y, void *stream) {
+    if (int rc = mx_check(codes, scales, M, K)) return rc;
+    BHI_REQUIRE(Y && aligned(Y, 16), "the output must be 16-byte aligned");
+    const int64_t words = static_cast<int64_t>(M) * (K / 8);
+    mx_dense_kernel<<<mx_stream_grid(words, kMxQuantThreads), kMxQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), words, Y);
+    return mx_launched("dense launch");
+}
+
+int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *X, const uint16_t *bias, uint16_t *Y, int rows,
+                     void *stream) {
+    if (int rc = mx_check(codes, scales, M, K)) return rc;
+    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(X && Y && aligned(X, 16) && aligned(Y, 2) && aligned(bias, 2), "X must be 16-byte aligned");
+    const int tiles_c = (M + kMxTile - 1) / kMxTile;
+    const int64_t blocks = static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c;
+    mx_linear_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), X, bias, Y, rows, tiles_c);
+    return mx_launched("product launch");
+}
+
+int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *dY, int ldy, uint16_t *dX, int rows, void *stream) {
+    if (int rc = mx_check(codes, scales, M, K)) return rc;
+    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(ldy >= M && ldy % 8 == 0, "rows of dY must be a multiple of 8 values apart");
+    BHI_REQUIRE(dY && dX && aligned(dY, 16) && aligned(dX, 16), "dY and dX must be 16-byte aligned");
+    const int tiles_c = (K + kMxTile - 1) / kMxTile;
+    const int64_t blocks = static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c;
+    mx_linear_grad_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), dY, ldy, dX, rows, tiles_c);
+    return mx_launched("gradient launch");
+}
+
+int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int K, const uint16_t *X, const uint16_t *bias, int activation, uint16_t *H,
+                    float *pre, int rows, void *stream) {
+    BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2, "bad number of gated outputs");
+    if (int rc = mx_check(codes, scales, 2 * inter, K)) return rc;
+    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
+    BHI_REQUIRE(X && H && aligned(X, 16) && aligned(H, 2) && aligned(bias, 2) && aligned(pre, 16), "X must be 16-byte aligned");
+    const MxWeight W = mx_weight(codes, scales, 2 * inter, K);
+    const int tiles_c = (inter + kMxTile - 1) / kMxTile;
+    const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (activation) {
+    case BHI_ACT_SILU: mx_gated_kernel<BHI_ACT_SILU><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
+    case BHI_ACT_GELU: mx_gated_kernel<BHI_ACT_GELU><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
+    default: mx_gated_kernel<BHI_ACT_GELU_TANH><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
+    }
+    return mx_launched("gated product launch");
+}
+
+int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows, void *stream) {
+    BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2 && rows >= 1, "empty gradient");
+    BHI_REQUIRE(pre && dH && dpre && aligned(pre, 16) && aligned(dH, 2) && aligned(dpre, 16) && ldp >= 2 * inter, "bad gradient buffers");
+    BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
+    const int64_t n = static_cast<int64_t>(rows) * inter;
+    const int grid = mx_stream_grid(n, 256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (activation) {
+    case BHI_ACT_SILU: mx_gated_grad_kernel<BHI_ACT_SILU><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
+    case BHI_ACT_GELU: mx_gated_grad_kernel<BHI_ACT_GELU><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
+    default: mx_gated_grad_kernel<BHI_ACT_GELU_TANH><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
+    }
+    return mx_launched("gated gradient launch");
+}
+
+}  // extern "C"

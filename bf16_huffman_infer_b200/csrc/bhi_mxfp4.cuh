@@ -1,0 +1,113 @@
+// 4-bit microscaled weights (OCP MXFP4): the layout in memory and what every kernel on them shares.
+//
+// Blocks of 32 values along a row share a scale byte s (E8M0, 2^(s - 127); 255 is NaN); a value is a 4-bit code (E2M1: sign,
+// two exponent bits, one mantissa bit; 0, 0.5, 1, 1.5, 2, 3, 4, 6).
+//
+// The rows are cut into tiles of 16 and the columns into groups of 128; both are padded with zeros.  One (tile, group) pair is
+// 1 KB of codes and 64 bytes of scales, so whatever walks along K reads whole lines, and a lane of an m16n8k16 product finds
+// the four words it needs of a row in one 16-byte load:
+//
+//   codes  [ceil(M / 16)][ceil(K / 128)][16 rows][4 quarters t][4 blocks j][4 bytes]   word (t, j): elements 8 t .. 8 t + 7 of block j
+//   scales [ceil(M / 16)][ceil(K / 128)][16 rows][4 blocks j]
+//
+// Inside a word, nibble i is element 2 i and nibble 4 + i element 2 i + 1 (i = 0..3): a mask leaves the pair (2 i, 2 i + 1) in
+// the two halves of a register.  Blocks whose scale is NaN hold zero codes, so that a product with an infinite scale yields NaN.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "bhi_staged.cuh"
+
+namespace bhi {
+
+constexpr int kMxRows = 16;                     // rows of a tile
+constexpr int kMxGroup = 128;                   // columns of a group
+constexpr int kMxTileCodes = 1024;              // bytes of a (tile, group) pair
+constexpr int kMxTileScales = 64;
+
+struct MxWeight {
+    const uint8_t *codes, *scales;
+    int M, K, groups;                           // groups = ceil(K / 128)
+};
+
+// byte offsets of row m, group 0
+__host__ __device__ __forceinline__ int64_t mx_code_row(int m, int groups) {
+    return static_cast<int64_t>(m >> 4) * groups * kMxTileCodes + (m & 15) * 64;
+}
+__host__ __device__ __forceinline__ int64_t mx_scale_row(int m, int groups) {
+    return static_cast<int64_t>(m >> 4) * groups * kMxTileScales + (m & 15) * 4;
+}
+
+// Byte b of a code word as two FP16 values: nibble 2 b in the low half, 2 b + 1 in the high half.
+__device__ __forceinline__ void mx_word_to_f16(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+
+__device__ __forceinline__ float f16lo_to_f32(uint32_t pair) {
+    float f;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(pair));
+    return f;
+}
+__device__ __forceinline__ float f16hi_to_f32(uint32_t pair) {
+    float f;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(f) : "r"(pair));
+    return f;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// 2^(s - 127); 255 gives infinity here (its codes are zero, so that their product is NaN)
+__device__ __forceinline__ float mx_scale(uint32_t s) { return __uint_as_float(s == 0u ? 0x00400000u : s << 23); }
+
+// The eight values of a word in element order, exact in 32 bits.
+__device__ __forceinline__ void mx_word_to_f32(uint32_t w, float scale, float (&v)[8]) {
+    uint32_t h[4];
+    mx_word_to_f16(w, h);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        // halves of h[i] are nibbles 2 i and 2 i + 1, and nibble n is element 2 n (n < 4) or 2 (n - 4) + 1
+        const int n = 2 * i;
+        v[n < 4 ? 2 * n : 2 * (n - 4) + 1] = f16lo_to_f32(h[i]) * scale;
+        v[n + 1 < 4 ? 2 * (n + 1) : 2 * (n - 3) + 1] = f16hi_to_f32(h[i]) * scale;
+    }
+}
+
+// ---- activations of the gated pair ---------------------------------------------------------------------------------
+// act(g) = g s(g) and act'(g), in 32 bits.  s is a logistic function (silu: of g; gelu's tanh form: of 2 z, since
+// (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)), which does not cancel for negative z) or half of erfc(-g / sqrt 2).  The fast exponential
+// and division are off by a few units of 2^-23 here: far below the one rounding to BF16 that follows.
+__device__ __forceinline__ float mx_logistic(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+template <int kAct>
+__device__ __forceinline__ void mx_act_grad(float g, float &a, float &da) {
+    if constexpr (kAct == BHI_ACT_SILU) {
+        const float s = mx_logistic(g);
+        a = g * s;
+        da = s + a * (1.f - s);
+    } else if constexpr (kAct == BHI_ACT_GELU) {
+        const float c = 0.5f * erfcf(g * -0.70710678118654752f);
+        a = g * c;
+        da = c + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    } else {
+        const float g2 = g * g;
+        const float s = mx_logistic(1.59576912160573071f * (g + 0.044715f * g2 * g));
+        a = g * s;
+        da = s + a * (1.f - s) * 1.59576912160573071f * (1.f + 0.134145f * g2);
+    }
+}
+template <int kAct>
+__device__ __forceinline__ float mx_act(float g) {
+    float a, da;
+    mx_act_grad<kAct>(g, a, da);
+    return a;
+}
+
+}  // namespace bhi

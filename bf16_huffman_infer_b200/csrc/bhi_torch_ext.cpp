@@ -14,6 +14,7 @@
 
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/bf16_huffman_b200.h"
@@ -671,6 +672,137 @@ void boxed_ans_emit_pass(StableIValue *stack, uint64_t, uint64_t) {
                             stream_of(W)));
 }
 
+// ---- 4-bit microscaled weights -------------------------------------------------------------------
+struct MxView {
+    const uint8_t *codes, *scales;
+    int M, K;
+};
+
+int int_of(int64_t v, const char *name) {
+    STD_TORCH_CHECK(v >= 1 && v <= INT32_MAX, name, " must be in [1, 2^31)");
+    return static_cast<int>(v);
+}
+
+MxView mx_of(const Tensor &codes, const Tensor &scales, int64_t M, int64_t K) {
+    want(codes, ScalarType::Byte, "codes", 4);
+    want(scales, ScalarType::Byte, "scales", 4);
+    same_device(codes, scales, "scales");
+    STD_TORCH_CHECK(M >= 1 && K >= 32 && K % 32 == 0 && M <= BHI_MXFP4_MAX_DIM && K <= BHI_MXFP4_MAX_DIM, "a weight has rows and a multiple of 32 columns");
+    const int64_t tiles = (M + 15) / 16, groups = (K + 127) / 128;
+    for (const auto &[t, last] : {std::pair<const Tensor &, int64_t>(codes, 64), std::pair<const Tensor &, int64_t>(scales, 4)})
+        STD_TORCH_CHECK(t.dim() == 4 && t.size(0) == tiles && t.size(1) == groups && t.size(2) == 16 && t.size(3) == last,
+                        "codes must be [ceil(M/16), ceil(K/128), 16, 64], scales [ceil(M/16), ceil(K/128), 16, 4]");
+    return {ptr<const uint8_t>(codes), ptr<const uint8_t>(scales), static_cast<int>(M), static_cast<int>(K)};
+}
+
+const uint16_t *mx_bias(const std::optional<Tensor> &bias, const Tensor &like, int64_t n) {
+    if (!bias.has_value()) return nullptr;
+    want(*bias, ScalarType::BFloat16, "bias");
+    same_device(like, *bias, "bias");
+    STD_TORCH_CHECK(bias->dim() == 1 && bias->numel() == n, "bias must hold a value for each row of the weight");
+    return ptr<const uint16_t>(*bias);
+}
+
+// mxfp4_quantize(W, codes(a!), scales(b!)) -> ()
+void boxed_mxfp4_quantize(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor W = arg(stack, 0), codes = arg(stack, 1), scales = arg(stack, 2);
+    const ScalarType st = W.scalar_type();
+    const int dtype = st == ScalarType::BFloat16 ? BHI_DTYPE_BF16 : st == ScalarType::Half ? BHI_DTYPE_FP16 : BHI_DTYPE_FP32;
+    want(W, dtype == BHI_DTYPE_FP32 ? ScalarType::Float : st, "W");
+    STD_TORCH_CHECK(W.dim() == 2, "W must be a matrix");
+    same_device(W, codes, "codes");
+    const MxView v = mx_of(codes, scales, W.size(0), W.size(1));
+    OnDevice on(W);
+    check(bhi_mxfp4_quantize(W.data_ptr(), dtype, v.M, v.K, ptr<uint8_t>(codes), ptr<uint8_t>(scales), stream_of(W)));
+}
+
+// dense_mxfp4(codes, scales, M, K) -> W
+void boxed_dense_mxfp4(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor codes = arg(stack, 0), scales = arg(stack, 1);
+    const MxView v = mx_of(codes, scales, iarg(stack, 2), iarg(stack, 3));
+    OnDevice on(codes);
+    const int64_t sizes[2] = {v.M, v.K}, strides[2] = {v.K, 1};
+    Tensor Y = empty_bf16(codes, 2, sizes, strides);
+    check(bhi_mxfp4_dense(v.codes, v.scales, v.M, v.K, ptr<uint16_t>(Y), stream_of(codes)));
+    stack[0] = torch::stable::detail::from(Y);
+}
+
+// forward_mxfp4(X, codes, scales, M, bias?) -> Y   (any leading dimensions)
+void boxed_forward_mxfp4(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor X = arg(stack, 0), codes = arg(stack, 1), scales = arg(stack, 2);
+    want(X, ScalarType::BFloat16, "X");
+    same_device(X, codes, "codes");
+    const MxView v = mx_of(codes, scales, iarg(stack, 3), X.size(-1));
+    std::optional<Tensor> bias = torch::stable::detail::to<std::optional<Tensor>>(stack[4]);
+    const uint16_t *b = mx_bias(bias, X, v.M);
+    OnDevice on(X);
+    Tensor Y = output_like(X, v.M);
+    if (X.numel() > 0)
+        check(bhi_mxfp4_linear(v.codes, v.scales, v.M, v.K, ptr<const uint16_t>(X), b, ptr<uint16_t>(Y), int_of(X.numel() / v.K, "rows"), stream_of(X)));
+    stack[0] = torch::stable::detail::from(Y);
+}
+
+// mxfp4_linear_grad(dY, codes, scales, M, K) -> dX; dY [rows, >= M]
+void boxed_mxfp4_linear_grad(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor dY = arg(stack, 0), codes = arg(stack, 1), scales = arg(stack, 2);
+    want(dY, ScalarType::BFloat16, "dY");
+    same_device(dY, codes, "codes");
+    const MxView v = mx_of(codes, scales, iarg(stack, 3), iarg(stack, 4));
+    STD_TORCH_CHECK(dY.dim() == 2 && dY.size(1) >= v.M, "dY must be [rows, at least M]");
+    OnDevice on(dY);
+    const int64_t sizes[2] = {dY.size(0), v.K}, strides[2] = {v.K, 1};
+    Tensor dX = empty_bf16(dY, 2, sizes, strides);
+    if (sizes[0] > 0)
+        check(bhi_mxfp4_linear_grad(v.codes, v.scales, v.M, v.K, ptr<const uint16_t>(dY), int_of(dY.size(1), "columns of dY"), ptr<uint16_t>(dX),
+                                    int_of(sizes[0], "rows"), stream_of(dY)));
+    stack[0] = torch::stable::detail::from(dX);
+}
+
+// gated_mxfp4(X, codes, scales, M, bias?, activation, pre(a!)?) -> H
+void boxed_gated_mxfp4(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor X = arg(stack, 0), codes = arg(stack, 1), scales = arg(stack, 2);
+    want(X, ScalarType::BFloat16, "X");
+    same_device(X, codes, "codes");
+    const MxView v = mx_of(codes, scales, iarg(stack, 3), X.size(-1));
+    STD_TORCH_CHECK(v.M % 2 == 0, "a stacked weight has an even number of rows");
+    std::optional<Tensor> bias = torch::stable::detail::to<std::optional<Tensor>>(stack[4]);
+    const uint16_t *b = mx_bias(bias, X, v.M);
+    const int64_t rows = X.numel() / v.K;
+    std::optional<Tensor> pre = torch::stable::detail::to<std::optional<Tensor>>(stack[6]);
+    float *p = nullptr;
+    if (pre.has_value()) {
+        want(*pre, ScalarType::Float, "pre");
+        same_device(X, *pre, "pre");
+        STD_TORCH_CHECK(pre->numel() == rows * v.M, "pre must hold a value for each row of X and of the weight");
+        p = ptr<float>(*pre);
+    }
+    const int64_t act = iarg(stack, 5);
+    OnDevice on(X);
+    Tensor H = output_like(X, v.M / 2);
+    if (rows > 0)
+        check(bhi_mxfp4_gated(v.codes, v.scales, v.M / 2, v.K, ptr<const uint16_t>(X), b, static_cast<int>(act), ptr<uint16_t>(H), p, int_of(rows, "rows"),
+                              stream_of(X)));
+    stack[0] = torch::stable::detail::from(H);
+}
+
+// mxfp4_gated_grad(pre, dH, activation) -> dpre [rows, 2 * inter rounded up to a multiple of 8]
+void boxed_mxfp4_gated_grad(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor pre = arg(stack, 0), dH = arg(stack, 1);
+    want(pre, ScalarType::Float, "pre");
+    want(dH, ScalarType::BFloat16, "dH");
+    same_device(pre, dH, "dH");
+    const int64_t inter = dH.size(-1), act = iarg(stack, 2);
+    STD_TORCH_CHECK(inter >= 1 && pre.numel() == 2 * dH.numel() && pre.size(-1) == 2 * inter, "pre must hold two values for each of dH");
+    OnDevice on(pre);
+    const int64_t rows = dH.numel() / inter, ld = (2 * inter + 7) / 8 * 8;
+    const int64_t sizes[2] = {rows, ld}, strides[2] = {ld, 1};
+    Tensor dpre = empty_bf16(pre, 2, sizes, strides);
+    if (rows > 0)
+        check(bhi_mxfp4_gated_grad(ptr<const float>(pre), ptr<const uint16_t>(dH), int_of(inter, "gated outputs"), static_cast<int>(act), ptr<uint16_t>(dpre),
+                                   int_of(ld, "columns"), int_of(rows, "rows"), stream_of(pre)));
+    stack[0] = torch::stable::detail::from(dpre);
+}
+
 }  // namespace
 
 STABLE_TORCH_LIBRARY(BHI_TORCH_NAMESPACE, m) {
@@ -704,6 +836,13 @@ STABLE_TORCH_LIBRARY(BHI_TORCH_NAMESPACE, m) {
     m.def("huffman_emit_pass(Tensor W, int split_k, Tensor code_lengths, Tensor code_values, Tensor offsets, Tensor(a!) rem, Tensor(b!) exp) -> ()");
     m.def("ans_size_pass(Tensor W, int split_k, Tensor freq, Tensor cum, Tensor(a!) words_per_row, Tensor(b!) stream_words) -> ()");
     m.def("ans_emit_pass(Tensor W, int split_k, Tensor freq, Tensor cum, Tensor offsets, Tensor stream_words, Tensor(a!) rem, Tensor(b!) exp) -> ()");
+    // 4-bit microscaled weights
+    m.def("mxfp4_quantize(Tensor W, Tensor(a!) codes, Tensor(b!) scales) -> ()");
+    m.def("dense_mxfp4(Tensor codes, Tensor scales, int M, int K) -> Tensor");
+    m.def("forward_mxfp4(Tensor X, Tensor codes, Tensor scales, int M, Tensor? bias) -> Tensor");
+    m.def("mxfp4_linear_grad(Tensor dY, Tensor codes, Tensor scales, int M, int K) -> Tensor");
+    m.def("gated_mxfp4(Tensor X, Tensor codes, Tensor scales, int M, Tensor? bias, int activation, Tensor(a!)? pre) -> Tensor");
+    m.def("mxfp4_gated_grad(Tensor pre, Tensor dH, int activation) -> Tensor");
 }
 
 STABLE_TORCH_LIBRARY_IMPL(BHI_TORCH_NAMESPACE, CompositeExplicitAutograd, m) {
@@ -737,4 +876,10 @@ STABLE_TORCH_LIBRARY_IMPL(BHI_TORCH_NAMESPACE, CUDA, m) {
     m.impl("huffman_emit_pass", &boxed_huffman_emit_pass);
     m.impl("ans_size_pass", &boxed_ans_size_pass);
     m.impl("ans_emit_pass", &boxed_ans_emit_pass);
+    m.impl("mxfp4_quantize", &boxed_mxfp4_quantize);
+    m.impl("dense_mxfp4", &boxed_dense_mxfp4);
+    m.impl("forward_mxfp4", &boxed_forward_mxfp4);
+    m.impl("mxfp4_linear_grad", &boxed_mxfp4_linear_grad);
+    m.impl("gated_mxfp4", &boxed_gated_mxfp4);
+    m.impl("mxfp4_gated_grad", &boxed_mxfp4_gated_grad);
 }

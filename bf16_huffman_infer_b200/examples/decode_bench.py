@@ -1,6 +1,7 @@
 """Whole-model decode speed, the way the reference's README measures it: a Hugging Face causal LM with a
 ``StaticCache``, the one-token step CUDA-graphed, greedy decoding; first as plain BF16, then with
-every linear layer compressed in place by ``convert_all_linear``.
+every linear layer compressed in place by ``convert_all_linear``: losslessly, or with ``--algo mxfp4`` rounded to 4-bit floats
+(the feed-forward blocks' first half is one kernel then).
 
     python -m bf16_huffman_infer_b200.examples.decode_bench                      # Qwen3-8B architecture
     python -m bf16_huffman_infer_b200.examples.decode_bench --layers 4 --tokens 32
@@ -87,7 +88,7 @@ def main():
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--prompt", type=int, default=8)
     ap.add_argument("--tokens", type=int, default=256)
-    ap.add_argument("--algo", default="huffman", choices=["huffman", "ans", "smallest"])
+    ap.add_argument("--algo", default="huffman", choices=["huffman", "ans", "smallest", "mxfp4"])
     ap.add_argument("--tables", default="limit6", choices=["limit6", "limit8", "escape", "reference"])
     ap.add_argument("--min-out-features", type=int, default=0)
     ap.add_argument("--no-fuse", action="store_true", help="keep q/k/v and gate/up as separate layers")
@@ -117,7 +118,7 @@ def main():
         "one_token_steps": stats,
         "model_bytes_bf16": size_raw, "model_bytes_compressed": size_comp, "ratio": round(size_comp / size_raw, 4),
         "convert_seconds": round(convert_s, 1),
-        # lossless weights, but the fused kernel sums in another order than cuBLAS: greedy tokens of a random-weight
+        # lossless weights (all but mxfp4), but the fused kernel sums in another order than cuBLAS: greedy tokens of a random-weight
         # model (near-uniform logits) may part ways after some steps
         "same_greedy_tokens_as_dense": bool(same), "first_differing_position": first_diff,
     }))

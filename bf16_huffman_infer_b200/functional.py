@@ -27,6 +27,7 @@ from tqdm import tqdm
 from . import ops, transfer
 from .ans import RANSEncoder
 from .huffman import LUTHuffmanEncoder
+from .mxfp4 import ACTIVATIONS, GatedMLP, GatedMXFP4, MXFP4Weight, linear_mxfp4
 from .utils import get_block_size_n, split_bf16
 
 OP_PER_LANE = 1
@@ -81,6 +82,7 @@ __all__ = [
     "convert_all_linear",
     "convert",
     "fuse_sibling_linears",
+    "fuse_gated_mlps",
     "set_huffman_tables",
     "set_ans_precision",
 ]
@@ -613,7 +615,8 @@ class ANSWeight(HuffmanWeight):
 
 
 class CompressedLinear(nn.Module):
-    """``nn.Linear`` replacement whose weight is a :class:`HuffmanWeight` / :class:`ANSWeight` (reference ``functional.py:313-320``)."""
+    """``nn.Linear`` replacement whose weight is a :class:`HuffmanWeight` / :class:`ANSWeight` (reference ``functional.py:313-320``),
+    or an :class:`MXFP4Weight`."""
 
     def __init__(self, weight: HuffmanWeight, bias: Optional[Tensor]) -> None:
         super().__init__()
@@ -638,6 +641,8 @@ class CompressedLinear(nn.Module):
             bias = self.bias
         if type(input) is Tensor and type(weight) in (HuffmanWeight, ANSWeight) and not torch._C._is_torch_function_mode_enabled():
             return _linear_compressed(input, weight, bias)
+        if type(input) is Tensor and type(weight) is MXFP4Weight and not torch._C._is_torch_function_mode_enabled():
+            return linear_mxfp4(input, weight, bias)
         return F.linear(input, weight, bias)
 
 
@@ -723,6 +728,9 @@ _CODERS = {"huffman": (HuffmanWeight,), "ans": (ANSWeight,), "smallest": (Huffma
 
 def _compress_for(a: Tensor, algo: str) -> HuffmanWeight:
     """``a`` compressed as ``algo`` says, on the device it is on."""
+    if algo == MXFP4Weight.algo:
+        assert a.dtype == torch.bfloat16, a.dtype          # its products take activations of this type
+        return MXFP4Weight.compress(a, to_cpu=not a.is_cuda)
     assert algo in _CODERS
     return _compress(a, get_block_size_n(a)[0], _CODERS[algo], to_cpu=not a.is_cuda)
 
@@ -731,7 +739,8 @@ def convert(linear: nn.Linear, name, disable_precision_check: bool = True, algo:
     """Compress one ``nn.Linear``; returns a :class:`CompressedLinear`, or ``linear`` itself when
     compression does not pay (ratio >= 1) or, if checking is enabled, when the fused output is off
     by 2 % or more on a random input (reference ``functional.py:323-375``).  The module comes back
-    on the device ``linear`` was on."""
+    on the device ``linear`` was on.  ``algo="mxfp4"`` rounds the weights to 4 bits; its output is
+    checked against the rounded weights."""
     home = linear.weight.device
     module = CompressedLinear(weight=_compress_for(linear.weight, algo), bias=linear.bias)
 
@@ -745,7 +754,7 @@ def convert(linear: nn.Linear, name, disable_precision_check: bool = True, algo:
         module.to(work)
         x = torch.randn(1, linear.in_features, dtype=torch.bfloat16, device=work)
         with torch.no_grad():
-            y1 = linear(x)
+            y1 = linear(x) if algo != MXFP4Weight.algo else F.linear(x, module.weight.get_weight(), module.bias)
             y2 = module(x)
         max_rtol = ((y2 - y1).abs() / y1.abs().clamp(min=1e-4)).max().item()
         linear.to(home)
@@ -862,15 +871,76 @@ def fuse_sibling_linears(model: nn.Module, groups=SIBLING_GROUPS, algo: str = "h
     return len(todo)
 
 
+def _activation_of(act_fn: nn.Module) -> Optional[str]:
+    """The name of the activation that ``act_fn`` computes, by what it does."""
+    v = torch.linspace(-6, 6, 97, device="cpu")
+    try:
+        with torch.no_grad():
+            y = act_fn(v)
+    except Exception:                            # an activation with parameters elsewhere, or of another signature
+        return None
+    known = {"silu": F.silu(v), "gelu": F.gelu(v), "gelu_tanh": F.gelu(v, approximate="tanh")}
+    assert known.keys() == ACTIVATIONS.keys()
+    for name, want in known.items():
+        if torch.is_tensor(y) and y.shape == v.shape and torch.allclose(y, want, rtol=0, atol=1e-6):      # the two gelus are 5e-4 apart
+            return name
+    return None
+
+
+def _is_gated_mlp(parent: nn.Module) -> Optional[str]:
+    """The activation of a block that computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` and nothing else, found by its
+    parts and by running it on one row; None for any other module."""
+    parts = dict(parent.named_children())
+    if parts.keys() != {"gate_proj", "up_proj", "down_proj", "act_fn"} or any(True for _ in parent.parameters(recurse=False)):
+        return None
+    gate, up, down = (parts[n] for n in ("gate_proj", "up_proj", "down_proj"))
+    if not all(type(m) is nn.Linear for m in (gate, up, down)) or gate.weight.shape != up.weight.shape or gate.in_features % 32:
+        return None
+    if (gate.bias is None) != (up.bias is None) or gate.weight.dtype != torch.bfloat16 or gate.weight.device != up.weight.device:
+        return None
+    if any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in parent.modules()):
+        return None
+    name = _activation_of(parts["act_fn"])
+    if name is None:
+        return None
+    x = torch.linspace(-2, 2, gate.in_features, device=gate.weight.device).to(torch.bfloat16)[None]
+    try:
+        with torch.no_grad():
+            # by their bits: a model that is still to be loaded may hold NaNs
+            same = torch.equal(parent(x).view(torch.int16), down(parts["act_fn"](gate(x)) * up(x)).view(torch.int16))
+    except Exception:                            # takes or returns something else
+        return None
+    return name if same else None
+
+
+def fuse_gated_mlps(model: nn.Module, algo: str = "mxfp4", progress: bool = False) -> int:
+    """Replace, in place, every block that computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` with a :class:`GatedMLP`: gate and up
+    projection are stacked, rounded to 4 bits and computed with the activation and the product in one kernel.  The down
+    projection is left as it is (:func:`convert_all_linear` converts it).  Returns the number of blocks."""
+    if algo != MXFP4Weight.algo:
+        raise ValueError(f"gated blocks are fused for algo={MXFP4Weight.algo!r}, not {algo!r}")
+    todo = [(name, parent, act) for name, parent in model.named_modules() if name and (act := _is_gated_mlp(parent)) is not None]
+    for name, parent, act in tqdm(todo, disable=not progress):
+        gate, up = parent.gate_proj, parent.up_proj
+        weight = _compress_for(torch.cat([gate.weight.detach(), up.weight.detach()]), algo)
+        bias = None if gate.bias is None else nn.Parameter(torch.cat([gate.bias.detach(), up.bias.detach()]), requires_grad=False)
+        block = GatedMLP(GatedMXFP4(weight, bias, act), parent.down_proj)
+        model.set_submodule(name, block.train(parent.training))
+    return len(todo)
+
+
 def convert_all_linear(model: nn.Module, min_out_features: int = 4096, progress: bool = True,
                        algo: str = "huffman", fuse_siblings: bool = False, huffman_tables: Optional[str] = None) -> None:
     """Replace, in place, every ``nn.Linear`` with at least ``min_out_features`` outputs
     (reference ``functional.py:378-387``).  Not in the reference: ``fuse_siblings=True`` first stacks
     q/k/v and gate/up projections into single compressed weights (:class:`FusedCompressedLinear`);
-    ``huffman_tables`` picks the table builder for this call (:func:`set_huffman_tables`)."""
+    ``huffman_tables`` picks the table builder for this call (:func:`set_huffman_tables`); ``algo="mxfp4"`` rounds the weights
+    to 4-bit floats (:class:`MXFP4Weight`), with ``fuse_siblings=True`` also turning feed-forward blocks into :class:`GatedMLP`."""
     previous = set_huffman_tables(huffman_tables) if huffman_tables is not None else None
     try:
         if fuse_siblings:
+            if algo == MXFP4Weight.algo:
+                fuse_gated_mlps(model, algo=algo, progress=progress)
             fuse_sibling_linears(model, algo=algo, progress=progress)
         targets = [name for name, mod in model.named_modules()
                    if isinstance(mod, nn.Linear) and mod.out_features >= min_out_features]

@@ -1,0 +1,330 @@
+"""4-bit microscaled weights (OCP MXFP4) beside the lossless coders: ``convert_all_linear(model, algo="mxfp4")``.
+
+A quarter of BF16's bytes (4.25 bits a value) for a rounding of every weight: blocks of 32 values along a row share a power of
+two, each value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives.  :class:`MXFP4Weight` stands where a
+:class:`HuffmanWeight` does: as the weight of ``F.linear`` or of a :class:`CompressedLinear`.  Products take BF16 activations as
+they are (nothing but the weight is quantised), sum in 32 bits and round once; the gradient with respect to the input flows
+through the frozen weight.  :func:`gated_mxfp4` is the first half of a gated feed-forward block in one kernel.
+
+The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from typing import Callable, Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor, nn
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from . import ops, transfer
+
+__all__ = ["MXFP4Weight", "linear_mxfp4", "gated_mxfp4", "GatedMXFP4", "GatedMLP"]
+
+BLOCK = 32
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+class MXFP4Weight(nn.Module):
+    """A ``[M, K]`` weight of 4-bit floats with a scale byte for every 32 (``K`` a multiple of 32).
+
+    Buffers, padded with zeros to tiles of 16 rows and groups of 128 columns: ``codes`` u8 ``[ceil(M/16), ceil(K/128), 16, 64]`` and
+    ``scales`` u8 ``[ceil(M/16), ceil(K/128), 16, 4]``, in the order that the kernels read (``include/bf16_huffman_b200.h``);
+    :meth:`from_packed` and :meth:`packed` translate from and to the plain order that checkpoints have.
+    """
+
+    algo = "mxfp4"
+
+    def __init__(self, codes: Tensor, scales: Tensor, out_features: int, in_features: int):
+        super().__init__()
+        tiles, groups = _padded(out_features, in_features)
+        for name, t, last in (("codes", codes, 64), ("scales", scales, 4)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (tiles, groups, 16, last):
+                raise ValueError(f"{name} of a {out_features} x {in_features} weight must be u8 {(tiles, groups, 16, last)}, "
+                                 f"not {t.dtype} {tuple(t.shape)}")
+        self.codes = nn.Buffer(codes)
+        self.scales = nn.Buffer(scales)
+        self.out_features, self.in_features = int(out_features), int(in_features)
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.out_features, self.in_features)
+
+    def nbytes(self) -> int:
+        return sum(b.nelement() * b.element_size() for b in self.buffers())
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        if func is not F.linear:
+            return NotImplemented
+        return linear_mxfp4(*args, **(kwargs or {}))
+
+    def rows(self, lo: int, hi: int) -> "MXFP4Weight":
+        """Rows ``lo`` to ``hi`` as a weight of their own."""
+        codes, scales = self.packed()
+        return type(self).from_packed(codes[lo:hi], scales[lo:hi])
+
+    def get_weight(self) -> Tensor:
+        """Dense BF16 ``[M, K]``: exactly the values that the products use."""
+        b = self.__dict__["_buffers"]
+        assert b["codes"].is_cuda
+        return ops.dense_mxfp4(b["codes"], b["scales"], self.out_features, self.in_features)
+
+    # -- making one ---------------------------------------------------------------------------
+    @classmethod
+    def compress(cls, a: Tensor, to_cpu: bool = True) -> "MXFP4Weight":
+        """``a`` (BF16, FP16 or FP32) rounded to the format: the scale of a block is ``2^(floor(log2 max|v|) - 2)``, values go to
+        the nearest code (ties to even) and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
+        assert a.dim() == 2 and a.dtype in _TYPES, (a.shape, a.dtype)
+        a = a.detach()
+        if not a.is_cuda and not torch.cuda.is_available():
+            raise RuntimeError("bf16_huffman_infer_b200 needs a CUDA device: there is no CPU implementation")
+        home = a.device
+        a = a.to(home if a.is_cuda else torch.device("cuda", torch.cuda.current_device())).contiguous()
+        if a.data_ptr() % 16:
+            a = a.clone()
+        tiles, groups = _padded(*a.shape)
+        codes = torch.empty(tiles, groups, 16, 64, dtype=torch.uint8, device=a.device)
+        scales = torch.empty(tiles, groups, 16, 4, dtype=torch.uint8, device=a.device)
+        ops.mxfp4_quantize(a, codes, scales)
+        if to_cpu:
+            codes, scales = transfer.download(codes), transfer.download(scales)
+        else:
+            # the buffers must be complete in memory before a kernel with launch overlap reads them
+            torch.cuda.current_stream(a.device).synchronize()
+        return cls(codes, scales, *a.shape)
+
+    @classmethod
+    def from_packed(cls, codes: Tensor, scales: Tensor) -> "MXFP4Weight":
+        """From the plain order: ``codes`` u8 ``[M, K/2]`` (the even element in the low half of a byte) and ``scales`` u8 ``[M, K/32]``
+        (E8M0; also as ``torch.float8_e8m0fnu``), on their device."""
+        if scales.dtype == torch.float8_e8m0fnu:
+            scales = scales.view(torch.uint8)
+        if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.size(1) % 16 \
+                or tuple(scales.shape) != (codes.size(0), codes.size(1) // 16):
+            raise ValueError(f"want codes u8 [M, K/2] and scales u8 [M, K/32], got {codes.dtype} {tuple(codes.shape)}, "
+                             f"{scales.dtype} {tuple(scales.shape)}")
+        M, K = codes.size(0), 2 * codes.size(1)
+        tiles, groups = _padded(M, K)
+        s = F.pad(scales, (0, groups * 4 - K // 32, 0, tiles * 16 - M))
+        # a NaN block holds zero codes
+        c = codes.view(M, -1, 16).masked_fill((scales == 255)[..., None], 0).view(M, -1)
+        c = F.pad(c, (0, groups * 64 - K // 2, 0, tiles * 16 - M)).view(tiles, 16, groups, 4, 4, 4)     # tile, row, group, block, quarter, byte
+        low, high = c & 15, c >> 4
+        byte = [low[..., 0] | low[..., 1] << 4, low[..., 2] | low[..., 3] << 4, high[..., 0] | high[..., 1] << 4, high[..., 2] | high[..., 3] << 4]
+        c = torch.stack(byte, -1).permute(0, 2, 1, 4, 3, 5).reshape(tiles, groups, 16, 64)
+        s = s.view(tiles, 16, groups, 4).transpose(1, 2).contiguous()
+        if c.is_cuda:
+            torch.cuda.current_stream(c.device).synchronize()          # complete in memory, as after compress
+        return cls(c, s, M, K)
+
+    def packed(self) -> Tuple[Tensor, Tensor]:
+        """``(codes u8 [M, K/2], scales u8 [M, K/32])`` in the plain order; the inverse of :meth:`from_packed`."""
+        M, K = self.shape
+        tiles, groups = self.codes.shape[:2]
+        c = self.codes.view(tiles, groups, 16, 4, 4, 4).permute(0, 2, 1, 4, 3, 5).reshape(tiles * 16, groups * 16, 4)
+        low, high = c & 15, c >> 4
+        byte = [low[..., 0] | low[..., 2] << 4, high[..., 0] | high[..., 2] << 4, low[..., 1] | low[..., 3] << 4, high[..., 1] | high[..., 3] << 4]
+        c = torch.stack(byte, -1).view(tiles * 16, groups * 64)[:M, :K // 2].contiguous()
+        return c, self.scales.transpose(1, 2).reshape(tiles * 16, groups * 4)[:M, :K // 32].contiguous()
+
+
+def _padded(M: int, K: int) -> Tuple[int, int]:
+    """Tiles of rows and groups of columns of a weight."""
+    if M < 1 or K < BLOCK or K % BLOCK:
+        raise ValueError(f"an MXFP4 weight needs at least one row and a multiple of {BLOCK} columns, not {M} x {K}")
+    return (M + 15) // 16, (K + 127) // 128
+
+
+def _differentiable(*tensors: Optional[Tensor]) -> bool:
+    """Whether a derivative or a transformation of torch.func may be asked of a call on these tensors."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+
+
+def _plain(x: Tensor) -> Tensor:
+    """``x`` as the kernels read it: rows one after another from a 16-byte boundary."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def _check(input: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor], outputs: int) -> None:
+    assert input.is_cuda and input.dtype == torch.bfloat16, (input.device, input.dtype)
+    if input.dim() < 1 or input.size(-1) != weight.in_features:
+        raise RuntimeError(f"input of shape {tuple(input.shape)} does not fit a weight of {weight.in_features} columns")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (outputs,) or bias.device != input.device):
+        raise RuntimeError(f"bias must be a BF16 vector of {outputs} values on {input.device}")
+
+
+def _product(x: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor]) -> Tensor:
+    b = weight.__dict__["_buffers"]
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return ops.forward_mxfp4(_plain(x), b["codes"], b["scales"], weight.out_features, bias)
+
+
+def _rows_of_eight(dy: Tensor) -> Tensor:
+    """Rows of a gradient as the kernels read them: a multiple of 8 values apart."""
+    dy = dy.flatten(0, -2) if dy.dim() > 1 else dy[None]
+    if dy.size(1) % 8 == 0:
+        return _plain(dy)
+    out = dy.new_empty(dy.size(0), (dy.size(1) + 7) // 8 * 8)
+    out[:, :dy.size(1)] = dy
+    return out
+
+
+class _Held:
+    """Hands a weight through an autograd function, which would otherwise ask its ``__torch_function__`` about the call."""
+
+    __slots__ = ("weight",)
+
+    def __init__(self, weight: "MXFP4Weight"):
+        self.weight = weight
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(x, held, bias):
+        return _product(x, held.weight, bias)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.held, ctx.shape = inputs[1], output.shape
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = _LinearGradient.apply(dy, ctx.held) if ctx.needs_input_grad[0] else None
+        db = dy.flatten(0, -2).sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[2] else None
+        return dx, None, db
+
+    @staticmethod
+    def jvp(ctx, dx, _, db):
+        if dx is None:
+            return db.expand(ctx.shape)
+        return linear_mxfp4(dx, ctx.held.weight, db)
+
+    @staticmethod
+    def vmap(info, in_dims, x, held, bias):
+        return _batched(info, in_dims, x, bias, lambda x, bias: linear_mxfp4(x, held.weight, bias))
+
+
+class _LinearGradient(torch.autograd.Function):
+    """dx = dy W, itself linear in dy."""
+
+    @staticmethod
+    def forward(dy, held):
+        w = held.weight
+        b = w.__dict__["_buffers"]
+        return ops.mxfp4_linear_grad(_rows_of_eight(dy), b["codes"], b["scales"], w.out_features, w.in_features).view(*dy.shape[:-1], w.in_features)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.held = inputs[1]
+
+    @staticmethod
+    def backward(ctx, ddx):
+        return linear_mxfp4(ddx, ctx.held.weight), None
+
+    @staticmethod
+    def jvp(ctx, ddy, _):
+        return _LinearGradient.apply(ddy, ctx.held)
+
+    @staticmethod
+    def vmap(info, in_dims, dy, held):
+        return _LinearGradient.apply(dy.movedim(in_dims[0], 0), held), 0
+
+
+def _batched(info, in_dims, x: Tensor, bias: Optional[Tensor], call: Callable) -> Tuple[Tensor, int]:
+    """``call`` over a batch dimension of ``x``; a bias with one of its own is handed on item by item."""
+    if in_dims[2] is None:
+        return call(x.movedim(in_dims[0], 0), bias), 0
+    bias = bias.movedim(in_dims[2], 0)
+    x = x.expand(info.batch_size, *x.shape) if in_dims[0] is None else x.movedim(in_dims[0], 0)
+    return torch.stack([call(a, b) for a, b in zip(x.unbind(0), bias.unbind(0))]), 0
+
+
+def linear_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = None) -> Tensor:
+    """``F.linear`` on a 4-bit weight: ``input`` BF16 ``[..., K]``, any number of rows; the bias (BF16, a value for each output) is part
+    of the 32-bit sum.  Differentiable with respect to the input and the bias."""
+    _check(input, weight, bias, weight.out_features)
+    if _differentiable(input, bias):
+        return _Linear.apply(input, _Held(weight), bias)
+    return _product(input, weight, bias)
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, held, bias, activation):
+        weight = held.weight
+        ctx.held, ctx.activation = held, activation
+        inter = weight.out_features // 2
+        pre = torch.empty(*x.shape[:-1], 2 * inter, dtype=torch.float32, device=x.device)
+        h = _gated(x, weight, bias, activation, pre)
+        ctx.save_for_backward(pre)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        pre, = ctx.saved_tensors
+        w = ctx.held.weight
+        b = w.__dict__["_buffers"]
+        dpre = ops.mxfp4_gated_grad(pre, dh.contiguous(), ctx.activation)
+        dx = db = None
+        if ctx.needs_input_grad[0]:
+            dx = ops.mxfp4_linear_grad(dpre, b["codes"], b["scales"], w.out_features, w.in_features).view(*dh.shape[:-1], w.in_features)
+        if ctx.needs_input_grad[2]:
+            db = dpre[:, :w.out_features].sum(0, dtype=torch.float32).to(dh.dtype)
+        return dx, None, db, None
+
+
+def _gated(x: Tensor, weight: MXFP4Weight, bias: Optional[Tensor], activation: int, pre: Optional[Tensor]) -> Tensor:
+    b = weight.__dict__["_buffers"]
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return ops.gated_mxfp4(_plain(x), b["codes"], b["scales"], weight.out_features, bias, activation, pre)
+
+
+def gated_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = None, activation: str = "silu") -> Tensor:
+    """``act(x G^T + b_g) * (x U^T + b_u)`` for the stacked weight ``[G; U]`` (gate rows first) and bias ``[b_g; b_u]``: BF16 ``[..., M/2]``
+    from BF16 ``[..., K]`` in one kernel, the projections kept in 32 bits.  ``activation``: ``"silu"``, ``"gelu"`` or
+    ``"gelu_tanh"``.  Differentiable once with respect to the input and the bias; a call that may be differentiated keeps
+    the projections (8 bytes a gated value) for the backward pass."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+    if weight.out_features % 2:
+        raise RuntimeError(f"a stacked weight has an even number of rows, not {weight.out_features}")
+    _check(input, weight, bias, weight.out_features)
+    if _differentiable(input, bias):
+        return _Gated.apply(input, _Held(weight), bias, ACTIVATIONS[activation])
+    return _gated(input, weight, bias, ACTIVATIONS[activation], None)
+
+
+class GatedMXFP4(nn.Module):
+    """The gate and up projection of a feed-forward block with the activation and the product: :func:`gated_mxfp4` on its weight."""
+
+    def __init__(self, weight: MXFP4Weight, bias: Optional[Tensor], activation: str):
+        super().__init__()
+        if activation not in ACTIVATIONS or weight.out_features % 2:
+            raise ValueError(f"no gated pair: {weight.shape}, {activation!r}")
+        self.weight = weight
+        self.bias = bias
+        self.activation = activation
+
+    def forward(self, input: Tensor) -> Tensor:
+        return gated_mxfp4(input, self.weight, self.bias, self.activation)
+
+
+class GatedMLP(nn.Module):
+    """``down_proj(act(gate_proj(x)) * up_proj(x))`` with the two first projections stacked."""
+
+    def __init__(self, gate_up: GatedMXFP4, down_proj: nn.Module):
+        super().__init__()
+        self.gate_up = gate_up
+        self.down_proj = down_proj
+
+    def forward(self, x: Tensor) -> Tensor:
+        return self.down_proj(self.gate_up(x))

@@ -154,3 +154,18 @@ def ans_size_pass(W: Tensor, split_k: int, freq: Tensor, cum: Tensor, words_per_
 def ans_emit_pass(W: Tensor, split_k: int, freq: Tensor, cum: Tensor, offsets: Tensor, stream_words: Tensor,
                   rem: Tensor, exp: Tensor) -> None:
     _ops.ans_emit_pass.default(W, split_k, freq, cum, offsets, stream_words, rem, exp)
+
+
+# ---- 4-bit microscaled weights ----------------------------------------------------------------------
+# (W, codes, scales) -> (): W BF16, FP16 or FP32; codes and scales as in MXFP4Weight
+mxfp4_quantize = _ops.mxfp4_quantize.default
+# (codes, scales, M, K) -> W BF16
+dense_mxfp4 = _ops.dense_mxfp4.default
+# (X, codes, scales, M, bias or None) -> Y: any number of rows of X, any leading dimensions
+forward_mxfp4 = _ops.forward_mxfp4.default
+# (dY [rows, at least M], codes, scales, M, K) -> dX
+mxfp4_linear_grad = _ops.mxfp4_linear_grad.default
+# (X, codes, scales, M = 2 * gated outputs, bias or None, activation, pre f32 or None) -> H, and the projections to pre
+gated_mxfp4 = _ops.gated_mxfp4.default
+# (pre, dH, activation) -> dpre [rows, M rounded up to 8]
+mxfp4_gated_grad = _ops.mxfp4_gated_grad.default

@@ -22,6 +22,7 @@ from torch import Tensor, nn
 
 from . import ops
 from .functional import FUSED_MAX_ROWS, ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight
+from .mxfp4 import MXFP4Weight
 
 __all__ = ["row_range", "shard_rows", "RowShardedLinear", "shard_model_linears", "PeerArena", "PeerRowShardedLinear"]
 
@@ -37,8 +38,12 @@ def shard_rows(weight: HuffmanWeight, rank: int, world: int) -> HuffmanWeight:
     Works on any device; no re-encoding.  Each chunk's records of the row range form one
     contiguous span of ``exp`` (records are stored chunk-major, rows ascending); the spans are
     concatenated, each followed by the 64 padding words a decoder may look at, and the offsets
-    are re-based onto the new buffer.
+    are re-based onto the new buffer.  A 4-bit weight's rows are cut out of its tiles.
     """
+    if isinstance(weight, MXFP4Weight):
+        lo, hi = row_range(weight.shape[0], rank, world)
+        assert hi > lo, "a rank would own no rows"
+        return weight.rows(lo, hi)
     rem, exp, offsets = weight.rem, weight.exp, weight.offsets
     if rem.dim() == 2:
         rem = rem[None]
@@ -199,6 +204,8 @@ class PeerRowShardedLinear(nn.Module):
 
     @classmethod
     def from_full(cls, full: CompressedLinear, arena: PeerArena, group=None) -> "PeerRowShardedLinear":
+        if isinstance(full.weight, MXFP4Weight):
+            raise TypeError("4-bit weights have no exchange kernel: use RowShardedLinear")
         M = full.out_features
         assert M % arena.world == 0, "out_features must divide evenly across ranks"
         lo, hi = row_range(M, arena.rank, arena.world)
@@ -228,17 +235,18 @@ class PeerRowShardedLinear(nn.Module):
 
 def shard_model_linears(model: nn.Module, rank: int, world: int, group=None, arena: Optional[PeerArena] = None) -> None:
     """Replace every :class:`CompressedLinear` whose row count divides by ``world`` with its row shard
-    (an all-gather layer, or an exchange layer when a :class:`PeerArena` is given; commit the arena afterwards)."""
+    (an all-gather layer, or an exchange layer when a :class:`PeerArena` is given; commit the arena afterwards).  4-bit
+    weights have no exchange kernel: theirs are all-gather layers, and gated pairs stay whole."""
     for name, mod in list(model.named_modules()):
         if isinstance(mod, CompressedLinear) and mod.out_features % world == 0:
-            if arena is not None:
+            if arena is not None and not isinstance(mod.weight, MXFP4Weight):
                 model.set_submodule(name, PeerRowShardedLinear.from_full(mod, arena, group))
             else:
                 model.set_submodule(name, RowShardedLinear.from_full(mod, rank, world, group))
         elif isinstance(mod, FusedCompressedLinear) and mod.sharded is None and mod.weight.shape[0] % world == 0:
             # stacked siblings: shard the stacked rows; the slices the siblings return stay views of the full output
             full = CompressedLinear(mod.weight, mod.bias)
-            if arena is not None:
+            if arena is not None and not isinstance(mod.weight, MXFP4Weight):
                 mod.sharded = PeerRowShardedLinear.from_full(full, arena, group)
             else:
                 mod.sharded = RowShardedLinear.from_full(full, rank, world, group)

@@ -277,6 +277,48 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
                       const uint32_t *cum, const int32_t *offsets, const uint8_t *stream_words,
                       uint8_t *A_rem, uint32_t *A_exp, void *stream);
 
+/* ---- 4-bit microscaled weights (OCP MXFP4) ------------------------------------------------------
+ * No counterpart in the reference.  Blocks of 32 values along a row share a power of two (E8M0 byte), values are 4-bit
+ * floats (E2M1).  M outputs, K columns (a multiple of 32), both up to BHI_MXFP4_MAX_DIM, padded to T = ceil(M / 16) tiles of
+ * rows and G = ceil(K / 128) groups of columns:
+ *
+ *   codes   u8 [T, G, 16, 64]   rows of a tile; a row's 64 bytes are [4 quarters t][4 blocks j][4 bytes]: elements 8 t .. 8 t + 7
+ *                               of block j, nibble i (from the lowest) element 2 i, nibble 4 + i element 2 i + 1
+ *   scales  u8 [T, G, 16, 4]    byte s of each block: 2^(s - 127); 255 is NaN (its codes must be zero)
+ *
+ * Padding must be zeros; bhi_mxfp4_quantize writes it.  Sums are 32-bit floats, each output is rounded to BF16 once. */
+#define BHI_MXFP4_MAX_DIM (1 << 24)
+#define BHI_DTYPE_BF16 0
+#define BHI_DTYPE_FP16 1
+#define BHI_DTYPE_FP32 2
+#define BHI_ACT_SILU 0         /* g / (1 + exp(-g)) */
+#define BHI_ACT_GELU 1         /* g (1 + erf(g / sqrt 2)) / 2 */
+#define BHI_ACT_GELU_TANH 2    /* its approximation by tanh */
+
+/* W [M, K] of the named type, rows contiguous, to codes and scales: e = max(floor(log2 max|v|) - 2, -127), codes of v / 2^e
+ * rounded to the nearest (ties to even), saturated at 6; a block with an infinity or NaN becomes NaN. */
+int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
+
+/* Y bf16 [M, K]: the values (exact but for scales beyond BF16's range). */
+int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, uint16_t *Y, void *stream);
+
+/* Y bf16 [rows, M] = X [rows, K] W^T (+ bias bf16 [M] inside the 32-bit sum, or null). */
+int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *X, const uint16_t *bias,
+                     uint16_t *Y, int rows, void *stream);
+
+/* dX bf16 [rows, K] = dY W; rows of dY (bf16, M values) are ldy >= M values apart, a multiple of 8. */
+int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *dY, int ldy, uint16_t *dX,
+                          int rows, void *stream);
+
+/* W = [G; U] with 2 * inter rows, bias of 2 * inter values or null: H bf16 [rows, inter] = act(g) * u with g = X G^T, u = X U^T
+ * kept in 32 bits.  pre f32 [rows, 2 * inter] (or null) receives [g | u] for the gradient. */
+int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int K, const uint16_t *X, const uint16_t *bias,
+                    int activation, uint16_t *H, float *pre, int rows, void *stream);
+
+/* dpre bf16 [rows, ldp] = [dH u act'(g) | dH act(g)]; bhi_mxfp4_linear_grad turns it into the gradient of X. */
+int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows,
+                         void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,412 @@
+"""4-bit microscaled weights on the device, against plain computations in 64 bits.
+
+Tolerances.  A BF16 output is the exact value rounded once: off by at most 2^-8 of it, so the 2-norm of all errors is below 2^-8
+of the outputs' (the sums' own errors are far below that for the inputs here).  A single output may also be off by its 32-bit sum:
+K additions that lose at most 2^-23 each of the sum of the terms' magnitudes.  A gradient through the gated pair is
+rounded twice (the projections' gradients, which feed the product, and the result): 2^-7."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+GRID = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    import bf16_huffman_infer_b200
+    return bf16_huffman_infer_b200
+
+
+def normal(*shape, seed=0, std=1.0, dtype=torch.bfloat16):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).to(DEV)
+
+
+def plain_quantised(a):
+    """The format's values of a matrix, by distance to the grid in double precision (ties to the even code), and its scale bytes."""
+    v = a.double().cpu().view(a.shape[0], -1, 32)
+    top = v.abs().amax(-1, keepdim=True)
+    e = torch.where(top > 0, torch.frexp(top).exponent - 1 - 2, -127).clamp(min=-127)
+    q = torch.ldexp(v.abs(), -e).clamp(max=6)
+    dist = (q[..., None] - GRID).abs()
+    # of two codes at the same distance the even one comes first in this order
+    order = torch.tensor([0, 2, 4, 6, 1, 3, 5, 7])
+    code = order[dist[..., order].argmin(-1)]
+    value = torch.ldexp(GRID[code], e) * torch.where(torch.signbit(v), -1.0, 1.0)
+    return value.view(a.shape), (e + 127).squeeze(-1).to(torch.uint8)
+
+
+def made(pkg, M, K, seed=0, std=0.02):
+    """(weight, its dense values in 64 bits)"""
+    w = pkg.MXFP4Weight.compress(normal(M, K, seed=seed, std=std), to_cpu=False)
+    return w, w.get_weight().double()
+
+
+def close(y, want, magnitudes, K):
+    """Each output within a rounding and its sum's error, and all of them within a rounding by the 2-norm."""
+    err = (y.double() - want).abs()
+    assert bool((err <= want.abs() * 2.0 ** -8 + magnitudes * (K * 2.0 ** -23)).all()), float((err - want.abs() * 2.0 ** -8).max())
+    assert float(err.norm()) <= 2.0 ** -8 * float(want.norm()) + 1e-30
+    return True
+
+
+SHAPES = [(1, 32), (16, 128), (17, 96), (130, 512), (250, 2080), (1024, 4096), (300, 18944)]
+ROWS = [1, 2, 3, 5, 8, 9, 16, 17, 32, 33, 48, 64, 100, 128, 129, 200, 257, 700]
+
+
+# ---- quantisation ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,K", SHAPES[:6])
+def test_quantised_values(pkg, M, K, dtype):
+    a = normal(M, K, std=0.02, dtype=dtype)
+    w = pkg.MXFP4Weight.compress(a, to_cpu=False)
+    value, byte = plain_quantised(a)
+    assert torch.equal(w.get_weight().double().cpu(), value)
+    assert torch.equal(w.packed()[1].cpu(), byte)
+    codes, scales = w.packed()
+    again = pkg.MXFP4Weight.from_packed(codes, scales)
+    assert torch.equal(again.codes, w.codes) and torch.equal(again.scales, w.scales)      # padding included
+    assert all(torch.equal(x, y.cpu()) for x, y in zip(pkg.MXFP4Weight.compress(a.cpu()).buffers(), w.buffers()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantisation_at_the_edges(pkg, dtype):
+    """Every midpoint and its neighbours, both signs, at scales down to the smallest and up to the largest; zeros and blocks of zeros."""
+    marks = torch.tensor([0, 0.125, 0.25, 0.375, 0.5, 0.75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7, 7.5], dtype=torch.float64)
+    info = torch.finfo(dtype)
+    rows = []
+    for e in ([-14, -3, 0, 12] if dtype == torch.float16 else [-133, -130, -127, -126, -124, -60, 0, 60, 124, 125]):
+        for lead in (4.0, 6.0, 7.5):
+            if lead * 2.0 ** e > info.max:
+                continue
+            row = torch.zeros(64, dtype=torch.float64)
+            row[:19], row[19], row[32:51], row[51] = marks * 2.0 ** e, lead * 2.0 ** e, -marks * 2.0 ** e, -lead * 2.0 ** e
+            rows.append(row.clamp(min=-lead * 2.0 ** e, max=lead * 2.0 ** e))
+    a = torch.stack(rows + [torch.zeros(64, dtype=torch.float64)]).to(dtype)
+    w = pkg.MXFP4Weight.compress(a.to(DEV), to_cpu=False)
+    value, byte = plain_quantised(a)
+    assert torch.equal(w.packed()[1].cpu(), byte)
+    assert torch.equal(w.get_weight().double().cpu(), value)
+
+
+def test_infinities_and_nans_make_their_block_nan(pkg):
+    a = normal(20, 160, std=0.02)
+    a[3, 40], a[7, 0], a[19, 159] = float("inf"), float("nan"), -float("inf")
+    w = pkg.MXFP4Weight.compress(a, to_cpu=False)
+    dense = w.get_weight().view(20, 5, 32)
+    want = torch.zeros(20, 5, dtype=torch.bool, device=DEV)
+    want[3, 1] = want[7, 0] = want[19, 4] = True
+    assert torch.equal(dense.isnan().all(-1), want) and torch.equal(dense.isnan().any(-1), want)
+    for rows in (1, 40):
+        y = F.linear(normal(rows, 160, seed=1), w)
+        assert torch.equal(y.isnan().all(0), want.any(1)) and torch.equal(y.isnan().any(0), want.any(1))
+
+
+def test_quantisation_of_other_layouts(pkg):
+    a = normal(64, 256, std=0.02)
+    want = pkg.MXFP4Weight.compress(a, to_cpu=False).get_weight()
+    shifted = torch.empty(64 * 256 + 1, dtype=a.dtype, device=DEV)[1:].view(64, 256).copy_(a)
+    for view in (a.T.contiguous().T, torch.cat([a, a], 1)[:, :256], shifted, nn_parameter(a)):
+        assert torch.equal(pkg.MXFP4Weight.compress(view, to_cpu=False).get_weight(), want)
+    for bad in (a.double(), a[0], a[:, :40], a[:0], a.int()):
+        with pytest.raises((AssertionError, ValueError)):
+            pkg.MXFP4Weight.compress(bad)
+
+
+def nn_parameter(a):
+    return torch.nn.Parameter(a.clone())
+
+
+# ---- the product -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("M,K", SHAPES)
+def test_product(pkg, M, K, rows):
+    w, dense = made(pkg, M, K, seed=M + K)
+    x, bias = normal(rows, K, seed=rows), normal(M, seed=3)
+    mag = x.double().abs() @ dense.abs().T
+    assert close(F.linear(x, w), x.double() @ dense.T, mag, K)
+    assert close(F.linear(x, w, bias), x.double() @ dense.T + bias.double(), mag + bias.double().abs(), K)
+
+
+def test_product_of_other_layouts(pkg):
+    w, dense = made(pkg, 130, 512)
+    for rows in (3, 70):
+        x = normal(rows, 512, seed=rows)
+        want = F.linear(x, w)
+        shifted = torch.empty(rows * 512 + 1, dtype=x.dtype, device=DEV)[1:].view(rows, 512).copy_(x)
+        for view in (x.T.contiguous().T, torch.cat([x, x], 1)[:, 512:], shifted):
+            assert torch.equal(F.linear(view, w), want)
+        assert torch.equal(F.linear(x.view(1, rows, 1, 512), w), want.view(1, rows, 1, 130))
+    assert torch.equal(F.linear(x[0], w), F.linear(x[:1], w)[0])
+    assert F.linear(x[:0], w).shape == (0, 130) and F.linear(x.new_empty(2, 0, 512), w).shape == (2, 0, 130)
+    one = normal(1, 512)
+    assert torch.equal(F.linear(one.expand(40, 512), w), F.linear(one.repeat(40, 1), w))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_values_far_apart(pkg, rows):
+    """Rows of X and blocks of K whose magnitudes differ by many powers of two; scales from tiny to huge."""
+    g = torch.Generator().manual_seed(rows)
+    M, K = 48, 512
+    codes = torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, generator=g)
+    scales = torch.randint(60, 200, (M, 1), dtype=torch.uint8, generator=g) + torch.randint(0, 9, (M, K // 32), dtype=torch.uint8, generator=g)
+    w = pkg.MXFP4Weight.from_packed(codes.to(DEV), scales.to(DEV))
+    dense = w.get_weight().double()
+    x = torch.randn(rows, K, generator=g).double() * torch.exp2(torch.randint(-40, 20, (rows, 1), generator=g).double()) \
+        * torch.exp2(torch.randint(-20, 1, (rows, K), generator=g).double())
+    x = x.to(torch.bfloat16).to(DEV)
+    want, mag = x.double() @ dense.T, x.double().abs() @ dense.abs().T
+    err = (F.linear(x, w).double() - want).abs()
+    assert bool((err <= want.abs() * 2.0 ** -8 + mag * (K * 2.0 ** -23)).all())
+
+
+@pytest.mark.parametrize("rows", [1, 4, 20, 70])
+def test_infinities_and_nans_in_x(pkg, rows):
+    w, dense = made(pkg, 64, 384)
+    x = normal(rows, 384, seed=5)
+    clean = F.linear(x, w)
+    x[0, 130] = float("inf")
+    if rows > 1:
+        x[1, 7] = float("nan")
+    y = F.linear(x, w)
+    col = dense[:, 130]
+    assert torch.equal(y[0].isnan(), col == 0) and torch.equal(y[0][col != 0], torch.where(col > 0, math.inf, -math.inf)[col != 0].to(y.dtype))
+    if rows > 1:
+        assert bool(y[1].isnan().all())
+        assert torch.equal(y[2:], clean[2:])
+
+
+def test_refused_calls(pkg):
+    w, _ = made(pkg, 64, 128)
+    x = normal(2, 128)
+    for bad in (x.float(), x.half(), x.cpu()):
+        with pytest.raises(AssertionError):
+            F.linear(bad, w)
+    for bad in (x[:, :96], normal(2, 160), x.new_empty(())):
+        with pytest.raises(RuntimeError):
+            F.linear(bad, w)
+    bias = normal(64)
+    for bad in (bias[1:], bias.float(), bias.cpu(), bias[None], bias[0]):
+        with pytest.raises(RuntimeError):
+            F.linear(x, w, bad)
+    with pytest.raises(ValueError):
+        pkg.gated_mxfp4(x, w, activation="relu")
+    odd, _ = made(pkg, 63, 128)
+    with pytest.raises(RuntimeError):
+        pkg.gated_mxfp4(x, odd)
+
+
+# ---- its gradient --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 3, 9, 40, 129, 300])
+@pytest.mark.parametrize("M,K", SHAPES)
+def test_gradient_of_the_product(pkg, M, K, rows):
+    w, dense = made(pkg, M, K, seed=M + K)
+    x, bias = normal(rows, K, seed=rows).requires_grad_(), normal(M, seed=3).requires_grad_()
+    y = F.linear(x, w, bias)
+    assert torch.equal(y.detach(), F.linear(x.detach(), w, bias.detach()))
+    dy = normal(rows, M, seed=9)
+    dx, db = torch.autograd.grad(y, (x, bias), dy)
+    assert close(dx, dy.double() @ dense, dy.double().abs() @ dense.abs(), M)
+    assert close(db, dy.double().sum(0), dy.double().abs().sum(0), rows)
+
+
+def test_gradient_by_differences(pkg):
+    """(f(x + h) - f(x)) / h for the sum of squares / 2 of the outputs, in 64 bits outside the product."""
+    w, dense = made(pkg, 96, 256)
+    x = normal(12, 256, seed=2).requires_grad_()
+    y = F.linear(x, w)
+    dx, = torch.autograd.grad((y.float() ** 2).sum() / 2, x)
+
+    def f(v):
+        return float(((v @ dense.T) ** 2).sum() / 2)
+
+    x0 = x.detach().double()
+    g = torch.Generator().manual_seed(0)
+    for _ in range(5):
+        d = torch.randn(12, 256, generator=g).double().to(DEV)
+        numeric = (f(x0 + 1e-4 * d) - f(x0 - 1e-4 * d)) / 2e-4
+        # y and dx are rounded: each by at most 2^-8 of its norm
+        assert abs(numeric - float((dx.double() * d).sum())) <= 2.0 ** -7 * float(dx.double().norm() * d.norm())
+
+
+def test_gradients_of_views_and_broadcasts(pkg):
+    w, dense = made(pkg, 72, 256)
+    x = normal(1, 256, seed=2).requires_grad_()
+    y = F.linear(x.expand(24, 256), w)
+    y.sum().backward()                                           # dy is an expanded scalar
+    want = dense.sum(0)
+    assert float((x.grad[0].double() / 24 - want).norm()) <= 2.0 ** -7 * float(want.norm())        # the rows' gradients and their sum are rounded
+    x = normal(4, 6, 256, seed=3).requires_grad_()
+    F.linear(x, w).transpose(0, 1).contiguous().sum().backward()
+    assert x.grad.shape == x.shape
+    e = x.new_empty(0, 256).requires_grad_()
+    F.linear(e, w).sum().backward()
+    assert e.grad.shape == (0, 256)
+
+
+def test_other_derivatives(pkg):
+    w, dense = made(pkg, 72, 256)
+    x, t, bias = normal(5, 256), normal(5, 256, seed=1), normal(72, seed=2)
+    layer = pkg.CompressedLinear(w, None)
+    y, tangent = torch.func.jvp(layer, (x,), (t,))
+    assert torch.equal(y, layer(x)) and torch.equal(tangent, layer(t))
+    xs = torch.stack([x, t])
+    assert torch.equal(torch.func.vmap(layer)(xs), layer(xs))
+    assert torch.equal(torch.func.vmap(lambda v, b: F.linear(v, w, b), in_dims=(None, 0))(x, torch.stack([bias, -bias])),
+                       torch.stack([F.linear(x, w, bias), F.linear(x, w, -bias)]))
+    got = torch.func.grad(lambda v: layer(v).float().sum())(x)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(layer(x).float().sum(), x, create_graph=True)
+    assert torch.equal(got, dx.detach())
+    # dx is linear in dy, which does not depend on x here; through a square it does
+    y = layer(x)
+    dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    ddx, = torch.autograd.grad(dx.float().sum(), x)
+    want = 2 * (torch.ones(5, 256, device=DEV, dtype=torch.float64) @ dense.T) @ dense
+    assert float((ddx.double() - want).norm()) <= 2.0 ** -6 * float(want.norm())                    # four roundings on the way
+
+
+# ---- the gated pair --------------------------------------------------------------------------------------------------------
+def act64(g, name):
+    if name == "silu":
+        return g * torch.sigmoid(g)
+    return F.gelu(g, approximate="tanh" if name == "gelu_tanh" else "none")
+
+
+GATED = [(1, 32), (8, 128), (13, 96), (65, 512), (200, 2080), (1024, 1024), (50, 8192)]
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 16, 17, 33, 64, 130, 300])
+@pytest.mark.parametrize("inter,K", GATED)
+def test_gated(pkg, inter, K, rows, activation):
+    w, dense = made(pkg, 2 * inter, K, seed=inter + K, std=1.5 / math.sqrt(K))
+    x, bias, dh = normal(rows, K, seed=rows), normal(2 * inter, seed=3), normal(rows, inter, seed=4)
+    for b in (None, bias):
+        x64 = x.double().requires_grad_()
+        b64 = None if b is None else b.double().requires_grad_()
+        g, u = F.linear(x64, dense, b64).chunk(2, -1)
+        want = act64(g, activation) * u
+        h = pkg.gated_mxfp4(x, w, b, activation)
+        assert float((h.double() - want.detach()).norm()) <= 2.0 ** -8 * float(want.detach().norm())
+        leaf = x.clone().requires_grad_()
+        bleaf = None if b is None else b.clone().requires_grad_()
+        again = pkg.gated_mxfp4(leaf, w, bleaf, activation)
+        assert torch.equal(again.detach(), h)
+        leaves = [v for v in (leaf, bleaf) if v is not None]
+        for got, ref in zip(torch.autograd.grad(again, leaves, dh), torch.autograd.grad(want, [v for v in (x64, b64) if v is not None], dh.double())):
+            assert float((got.double() - ref).norm()) <= 2.0 ** -7 * float(ref.norm())
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_gated_far_from_zero(pkg, rows, activation):
+    """Gates from -60 to 60 and far beyond: neither overflow nor cancellation shows in value or gradient."""
+    inter, K = 64, 128
+    codes = torch.zeros(2 * inter, K // 2, dtype=torch.uint8)
+    codes[:, 0] = 2                                              # element 0 has the code of 1
+    w = pkg.MXFP4Weight.from_packed(codes.to(DEV), torch.full((2 * inter, K // 32), 127, dtype=torch.uint8, device=DEV))
+    x = torch.zeros(rows, K, device=DEV, dtype=torch.bfloat16)
+    x[:, 0] = torch.linspace(-60, 60, rows, device=DEV).to(x.dtype)
+    shift = torch.linspace(-30, 30, inter, device=DEV).to(x.dtype)
+    bias = torch.cat([shift, torch.ones(inter, device=DEV, dtype=x.dtype)])
+    x64 = x.double().requires_grad_()
+    g, u = x64[:, :1] + bias[:inter].double(), x64[:, :1] + 1
+    if activation == "gelu":
+        want = g * torch.special.ndtr(g) * u
+    elif activation == "gelu_tanh":
+        want = g * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)) * u
+    else:
+        want = g * torch.sigmoid(g) * u
+    leaf = x.clone().requires_grad_()
+    h = pkg.gated_mxfp4(leaf, w, bias, activation)
+    err = (h.double() - want).abs().detach()
+    # a rounding of the result; the function's own error, a few units of 2^-23 of arguments up to 90
+    assert bool((err <= want.detach().abs() * (2.0 ** -8 + 2.0 ** -14) + 1e-12).all())
+    dx, = torch.autograd.grad(h.float().sum(), leaf)
+    ref, = torch.autograd.grad(want.sum(), x64)
+    assert float((dx.double() - ref).norm()) <= 2.0 ** -7 * float(ref.norm())
+    far = x.clone()
+    far[:, 0] = torch.where(far[:, 0] < 0, -1e5, 1e5).to(far.dtype)
+    assert bool(pkg.gated_mxfp4(far, w, bias, activation).isfinite().all())
+
+
+def test_gated_layouts_and_empties(pkg):
+    w, dense = made(pkg, 80, 256, std=0.1)
+    x = normal(2, 3, 256)
+    h = pkg.gated_mxfp4(x, w)
+    assert h.shape == (2, 3, 40) and torch.equal(pkg.gated_mxfp4(x.transpose(0, 1).contiguous().transpose(0, 1), w), h)
+    assert pkg.gated_mxfp4(x[:0], w).shape == (0, 3, 40)
+    e = x[:0].clone().requires_grad_()
+    pkg.gated_mxfp4(e, w).sum().backward()
+    assert e.grad.shape == e.shape
+    leaf = x.clone().requires_grad_()
+    pkg.gated_mxfp4(leaf, w).sum().backward()                    # an expanded scalar as gradient
+    assert leaf.grad.shape == x.shape
+    y = pkg.gated_mxfp4(leaf, w)
+    dx, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+# ---- streams, graphs, launches --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 16, 40, 200])
+def test_same_results_every_time(pkg, rows):
+    w, _ = made(pkg, 1000, 4096)
+    x = normal(rows, 4096).requires_grad_()
+    y = F.linear(x, w)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    for _ in range(5):
+        again = F.linear(x, w)
+        assert torch.equal(again, y) and torch.equal(torch.autograd.grad(again, x, y.detach())[0], dx)
+
+
+def test_captured_and_on_two_streams(pkg):
+    """Two graphs of a block's products, replayed on two streams at once and then on new inputs, against eager calls."""
+    up, _ = made(pkg, 2 * 1000, 512, seed=1, std=0.05)
+    down, _ = made(pkg, 512, 1024, seed=2, std=0.05)             # 1000 gated values padded by hand to a multiple of 32
+
+    def block(x):
+        h = F.pad(pkg.gated_mxfp4(x, up), (0, 24))
+        return x + F.linear(h, down)
+
+    graphs = []
+    for rows in (2, 50):
+        x = normal(rows, 512, seed=rows)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block(x)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = block(block(x))
+        graphs.append((graph, x, y, torch.cuda.Stream()))
+    for seed in range(3):
+        for _, x, _, _ in graphs:
+            x.copy_(normal(*x.shape, seed=10 + seed))
+        torch.cuda.synchronize()
+        for graph, _, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, x, y, _ in graphs:
+            assert torch.equal(y, block(block(x)))
+
+
+def test_results_are_whole_for_the_next_kernel(pkg):
+    """A chain of products, each of which may start while the one before is still running, against the same with waits between."""
+    ws = [made(pkg, 2048, 2048, seed=s, std=0.022)[0] for s in range(3)]
+    x = normal(1, 2048)
+    y = x
+    for i in range(60):
+        y = F.linear(y, ws[i % 3])
+    z = x
+    for i in range(60):
+        z = F.linear(z, ws[i % 3])
+        torch.cuda.synchronize()
+    assert torch.equal(y, z)
