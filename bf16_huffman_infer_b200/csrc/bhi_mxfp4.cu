@@ -154,8 +154,7 @@ __global__ void __launch_bounds__(256) mx_linear_grad_kernel(MxWeight W, const u
     }
 }
 
-template <int kAct>
-__global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, uint16_t *H, float *pre, int64_t rows, int tiles_c) {
+__global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, int act, uint16_t *H, float *pre, int64_t rows, int tiles_c) {
     __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
     const int inter = W.M / 2;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
@@ -170,7 +169,7 @@ __global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_
             g[q] += bf16_at(bias, c);
             u[q] += bf16_at(bias, inter + c);
         }
-        H[r * inter + c] = f32_to_bf16_rn(mx_act<kAct>(g[q]) * u[q]);
+        H[r * inter + c] = f32_to_bf16_rn(mx_act(act, g[q]) * u[q]);
         if (pre) {
             pre[r * W.M + c] = g[q];
             pre[r * W.M + inter + c] = u[q];
@@ -179,13 +178,12 @@ __global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_
 }
 
 // ---- the gated pair's gradient: dg = dh u act'(g), du = dh act(g) --------------------------------------------------------
-template <int kAct>
-__global__ void __launch_bounds__(256) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, uint16_t *dpre, int inter, int ldp, int64_t n) {
+__global__ void __launch_bounds__(256) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, int act, uint16_t *dpre, int inter, int ldp, int64_t n) {
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = i / inter, c = i % inter;
         const float g = pre[r * 2 * inter + c], u = pre[r * 2 * inter + inter + c], dh = bf16_at(dH, i);
         float a, da;
-        mx_act_grad<kAct>(g, a, da);
+        mx_act_grad(act, g, a, da);
         dpre[r * ldp + c] = f32_to_bf16_rn(dh * u * da);
         dpre[r * ldp + inter + c] = f32_to_bf16_rn(dh * a);
     }
@@ -246,6 +244,10 @@ int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, 
     if (int rc = mx_check(codes, scales, M, K)) return rc;
     BHI_REQUIRE(rows >= 1, "no rows");
     BHI_REQUIRE(X && Y && aligned(X, 16) && aligned(Y, 2) && aligned(bias, 2), "X must be 16-byte aligned");
+    if (rows <= 32) {
+        const int rc = mx_rows_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
+        if (rc != kStagedDeclined) return rc;
+    }
     const int tiles_c = (M + kMxTile - 1) / kMxTile;
     const int64_t blocks = static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c;
     mx_linear_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), X, bias, Y, rows, tiles_c);
@@ -271,14 +273,14 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
     BHI_REQUIRE(X && H && aligned(X, 16) && aligned(H, 2) && aligned(bias, 2) && aligned(pre, 16), "X must be 16-byte aligned");
     const MxWeight W = mx_weight(codes, scales, 2 * inter, K);
+    if (rows <= 32) {
+        const int rc = mx_rows_launch(W, X, bias, H, true, activation, pre, rows, static_cast<cudaStream_t>(stream));
+        if (rc != kStagedDeclined) return rc;
+    }
     const int tiles_c = (inter + kMxTile - 1) / kMxTile;
     const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (activation) {
-    case BHI_ACT_SILU: mx_gated_kernel<BHI_ACT_SILU><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
-    case BHI_ACT_GELU: mx_gated_kernel<BHI_ACT_GELU><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
-    default: mx_gated_kernel<BHI_ACT_GELU_TANH><<<blocks, 256, 0, st>>>(W, X, bias, H, pre, rows, tiles_c); break;
-    }
+    mx_gated_kernel<<<blocks, 256, 0, st>>>(W, X, bias, activation, H, pre, rows, tiles_c);
     return mx_launched("gated product launch");
 }
 
@@ -289,11 +291,7 @@ int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int ac
     const int64_t n = static_cast<int64_t>(rows) * inter;
     const int grid = mx_stream_grid(n, 256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (activation) {
-    case BHI_ACT_SILU: mx_gated_grad_kernel<BHI_ACT_SILU><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
-    case BHI_ACT_GELU: mx_gated_grad_kernel<BHI_ACT_GELU><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
-    default: mx_gated_grad_kernel<BHI_ACT_GELU_TANH><<<grid, 256, 0, st>>>(pre, dH, dpre, inter, ldp, n); break;
-    }
+    mx_gated_grad_kernel<<<grid, 256, 0, st>>>(pre, dH, activation, dpre, inter, ldp, n);
     return mx_launched("gated gradient launch");
 }
 

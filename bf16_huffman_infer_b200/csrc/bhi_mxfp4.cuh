@@ -86,13 +86,12 @@ __device__ __forceinline__ void mx_word_to_f32(uint32_t w, float scale, float (&
 // and division are off by a few units of 2^-23 here: far below the one rounding to BF16 that follows.
 __device__ __forceinline__ float mx_logistic(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
-template <int kAct>
-__device__ __forceinline__ void mx_act_grad(float g, float &a, float &da) {
-    if constexpr (kAct == BHI_ACT_SILU) {
+__device__ __forceinline__ void mx_act_grad(int act, float g, float &a, float &da) {
+    if (act == BHI_ACT_SILU) {
         const float s = mx_logistic(g);
         a = g * s;
         da = s + a * (1.f - s);
-    } else if constexpr (kAct == BHI_ACT_GELU) {
+    } else if (act == BHI_ACT_GELU) {
         const float c = 0.5f * erfcf(g * -0.70710678118654752f);
         a = g * c;
         da = c + g * 0.39894228040143268f * __expf(-0.5f * g * g);
@@ -103,11 +102,14 @@ __device__ __forceinline__ void mx_act_grad(float g, float &a, float &da) {
         da = s + a * (1.f - s) * 1.59576912160573071f * (1.f + 0.134145f * g2);
     }
 }
-template <int kAct>
-__device__ __forceinline__ float mx_act(float g) {
-    float a, da;
-    mx_act_grad<kAct>(g, a, da);
-    return a;
+__device__ __forceinline__ float mx_act(int act, float g) {
+    if (act == BHI_ACT_SILU) return g * mx_logistic(g);
+    if (act == BHI_ACT_GELU) return g * (0.5f * erfcf(g * -0.70710678118654752f));
+    return g * mx_logistic(1.59576912160573071f * (g + 0.044715f * g * g * g));
 }
+
+// The products' launchers, whose source files are compiled side by side.  Each returns kStagedDeclined for what it does not serve.
+// `gated`: W.M = 2 * outputs; pre may be null.
+int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st);
 
 }  // namespace bhi
