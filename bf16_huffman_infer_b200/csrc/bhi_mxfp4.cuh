@@ -47,6 +47,11 @@ __device__ __forceinline__ void mx_word_to_f16(uint32_t w, uint32_t (&h)[4]) {
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
 
+// Four scale bytes as BF16 pairs; 255 becomes NaN.
+__device__ __forceinline__ void mx_scales_bf16(uint32_t s, uint32_t (&p)[2]) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.bf16x2.ue8m0x2 %0, l;\n\tcvt.rn.bf16x2.ue8m0x2 %1, h;\n\t}" : "=r"(p[0]), "=r"(p[1]) : "r"(s));
+}
+
 __device__ __forceinline__ float f16lo_to_f32(uint32_t pair) {
     float f;
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(pair));

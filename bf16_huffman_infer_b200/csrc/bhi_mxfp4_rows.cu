@@ -1,4 +1,6 @@
 // The products of 4-bit microscaled weights with few rows of X: which form, and its launch.
+#include <algorithm>
+
 #include "bhi_mxfp4_rows.cuh"
 
 namespace bhi {
@@ -7,73 +9,69 @@ bool overlap_launches();
 
 namespace {
 
-// The CTAs that share a step's columns (a cluster of 1, 2, 4 or 8): the fewest rounds of units, a cluster's joins counted as kJoin
-// units.
-struct RowsPlan {
-    int cluster = 0, part_groups = 0, clusters = 0;
-    uint32_t smem = 0;
-};
-constexpr double kJoin = 1.5;
+constexpr uint32_t kSmemRows = kSmemMax - 1024;      // what the barriers leave
+constexpr uint32_t kSmemHalf = 112 * 1024;           // of two CTAs an SM
+constexpr int kChunksMax = 8;
 
-template <int NT>
-RowsPlan rows_plan(int steps, int groups, int rows) {
-    RowsPlan best;
-    double best_cost = 1e30;
-    for (int c = 1; c <= kMxClusterMax && c <= groups; c *= 2) {
-        const int part = (groups + c - 1) / c;
-        const uint32_t smem = MxRowsPlan<NT>::total(rows, part, c);
-        if (smem > static_cast<uint32_t>(kSmemMax)) continue;
-        const int per_sm = smem <= 113u * 1024u ? 2 : 1;
-        const int clusters = sm_count() * per_sm / c;
-        const int rounds = (steps + clusters - 1) / clusters, units = (part + kMxRowWarps - 1) / kMxRowWarps;
-        const double cost = static_cast<double>(rounds) * units * per_sm + (c > 1 ? kJoin * ((rounds + kMxBatch - 1) / kMxBatch) : 0.0);
-        if (cost < best_cost - 1e-9) {
-            best_cost = cost;
-            best = {c, part, steps < clusters ? steps : clusters, smem};
+template <class Form>
+int launch(MxRowsArgs a, cudaStream_t st) {
+    constexpr int per = Form::kGated ? 16 : 16 * Form::MT;
+    a.steps = (a.outs + per - 1) / per;
+    const int groups = a.W.groups, grid = std::min(a.steps, sm_count() * Form::kPerSm), most_steps = (a.steps + grid - 1) / grid;
+    // as few chunks of K as shared memory takes
+    for (int chunks = 1; chunks <= (Form::kPerSm == 2 ? 1 : kChunksMax) && chunks <= groups; chunks++) {
+        a.chunk_groups = (groups + chunks - 1) / chunks;
+        const int last = groups - (groups - 1) / a.chunk_groups * a.chunk_groups;      // groups of the last chunk
+        a.consumers = std::min(Form::kWarps, last);
+        a.scale_off = static_cast<uint32_t>(a.rows) * Form::row_bytes(a.chunk_groups);
+        a.part_off = a.scale_off + static_cast<uint32_t>(a.chunk_groups) * 8 * Form::NT * 4;
+        for (a.parts = kMxPartsMax; a.parts >= 2; a.parts--) {
+            a.sum_off = a.part_off + a.parts * a.consumers * Form::kPart * 16u;
+            const uint64_t bytes = a.sum_off + (chunks > 1 ? static_cast<uint64_t>(most_steps) * Form::kSum * 16u : 0u);
+            if (bytes > (Form::kPerSm == 2 ? kSmemHalf : kSmemRows)) continue;
+            auto kernel = mx_rows_kernel<Form>;
+            if (int rc = staged_prepare(kernel, kSmemRows)) return rc;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(grid);
+            cfg.blockDim = dim3(32 * (a.consumers + Form::kFinishers));
+            cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = overlap_launches() ? 1 : 0;
+            cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+            return e == cudaSuccess ? BHI_OK : cuda_fail(e, "4-bit product launch");
         }
     }
-    return best;
-}
-
-template <int NT, int kDepth, bool kGated>
-int launch(MxRowsArgs a, cudaStream_t st) {
-    const RowsPlan p = rows_plan<NT>(a.steps, a.W.groups, a.rows);
-    if (p.cluster == 0) return kStagedDeclined;
-    auto kernel = mx_rows_kernel<NT, kDepth, kGated>;
-    if (int rc = staged_prepare(kernel)) return rc;
-    a.part_groups = p.part_groups;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.clusters * p.cluster);
-    cfg.blockDim = dim3(kMxRowThreads);
-    cfg.dynamicSmemBytes = p.smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (overlap_launches()) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (p.cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = p.cluster;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        n++;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    return e == cudaSuccess ? BHI_OK : cuda_fail(e, "4-bit product launch");
+    return kStagedDeclined;
 }
 
 }  // namespace
 
 int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st) {
-    const int outs = gated ? W.M / 2 : W.M, per = gated ? 8 : 16;
-    const MxRowsArgs a{W, X, bias, Y, pre, rows, outs, (outs + per - 1) / per, 0, activation};
-    if (rows <= 8) return gated ? launch<1, 4, true>(a, st) : launch<1, 4, false>(a, st);
-    if (rows <= 16) return gated ? launch<2, 4, true>(a, st) : launch<2, 4, false>(a, st);
-    if (rows <= 32) return gated ? launch<4, 2, true>(a, st) : launch<4, 2, false>(a, st);
+    MxRowsArgs a{};
+    a.W = W, a.X = X, a.bias = bias, a.Y = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
+    if (gated && a.outs % 16 == 0) {
+        if (rows <= 8) return launch<MxRowsForm<2, 1, 14, 2, 1, 2, true>>(a, st);
+        if (rows <= 16) return launch<MxRowsForm<2, 2, 14, 2, 1, 2, true>>(a, st);
+        if (rows <= 32) return launch<MxRowsForm<2, 4, 10, 2, 1, 1, true>>(a, st);
+    } else if (gated) {                              // ups lie across two tiles each
+        if (rows <= 8) return launch<MxRowsForm<3, 1, 14, 2, 1, 1, true>>(a, st);
+        if (rows <= 16) return launch<MxRowsForm<3, 2, 10, 2, 1, 1, true>>(a, st);
+        if (rows <= 32) return launch<MxRowsForm<3, 4, 10, 2, 1, 1, true>>(a, st);
+    } else {
+        int rc = kStagedDeclined;
+        if (rows <= 8) rc = W.M >= 128 * 2 * sm_count() ? launch<MxRowsForm<2, 1, 7, 1, 2, 2, false>>(a, st) : launch<MxRowsForm<1, 1, 7, 1, 2, 4, false>>(a, st);
+        if (rc != kStagedDeclined) return rc;
+        if (rows <= 8) return launch<MxRowsForm<2, 1, 14, 2, 1, 2, false>>(a, st);
+        if (rows <= 16) return launch<MxRowsForm<2, 2, 14, 2, 1, 2, false>>(a, st);
+        if (rows <= 32) return launch<MxRowsForm<1, 4, 14, 2, 1, 2, false>>(a, st);
+    }
     return kStagedDeclined;
 }
+
+cudaError_t take_mxfp4_rows_status(int *out) { return take_status(out); }
 
 }  // namespace bhi

@@ -3,25 +3,22 @@
 // y[r][m] = sum over blocks b of 2^(s[m][b] - 127) * sum over the block's k of code[m][k] x[r][k], and with kGated the rows g and u of a
 // stacked weight at once, h = act(g) u.
 //
-// Bound by the bytes of the weight.  A warp takes 16 rows and one group of 128 columns at a time, straight from global memory into
-// registers (two 16-byte loads a lane, kDepth such units in flight), turns the codes into FP16 by the hardware's conversion and
-// multiplies blocks of 32 columns by m16n8k16 products whose sums start at zero: a block's scale applies to its sum, in 32 bits, so
-// codes need no scaling of their own.  X is FP16 there: each row's 128 values of a group are brought to [2^14, 2^15) by a power of two
-// that the sum gives back.  That is exact for every value down to 2^-32 of the largest in its 128; below, the error is
-// under 2^-40 of that largest one, far less than a 32-bit sum with it loses.
+// Bound by the bytes of the weight.  A consumer warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
+// They come straight from global memory into registers, kDepth units ahead.  The codes are turned into FP16 by the hardware's conversion and multiplies blocks of 32 columns by m16n8k16 products whose sums start at zero: a block's scale applies
+// to its sum, in 32 bits, so codes need no scaling of their own.  X is FP16 there: each row's 128 values of a group are brought to
+// [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-32 of the largest in its 128;
+// below, the error is under 2^-40 of that largest one, far less than a 32-bit sum with it loses.
 //
-// The eight warps of a CTA (and the CTAs of a cluster, where K x rows is too much shared memory for one) divide the groups, each
-// adding up its own; the parts of kBatch steps are put together in shared memory at a time, in a fixed order.
+// The consumer warps take the units of all steps in turn, each adding up its own of a step; two warps put these parts together, in
+// order, and write the outputs while the consumers go on.  Where X is too large for shared memory, K is walked in chunks: all steps of the CTA with
+// one chunk's X, then with the next, the sums of each step kept in shared memory.
 #pragma once
 
 #include "bhi_mxfp4.cuh"
 
 namespace bhi {
 
-constexpr int kMxRowThreads = 256;
-constexpr int kMxRowWarps = 8;
-constexpr int kMxBatch = 4;                       // steps whose parts are put together at a time
-constexpr int kMxClusterMax = 8;
+constexpr int kMxPartsMax = 4;                    // steps whose parts lie in shared memory
 
 struct MxRowsArgs {
     MxWeight W;
@@ -30,10 +27,38 @@ struct MxRowsArgs {
     float *pre;                                   // gated, or null: [rows][2 * inter]
     int rows;
     int outs;                                     // M, or inter of a gated pair
-    int steps;                                    // 16 outputs a step (8 gated ones)
-    int part_groups;                              // groups of a CTA of the cluster
     int activation;
+    // the launch's plan
+    int steps;                                    // plain: of MT tiles; gated: of 16 outputs
+    int chunk_groups;                             // groups whose X lies in shared memory at a time
+    int consumers;                                // warps that multiply, at most as many as a chunk has groups
+    int parts;
+    uint32_t scale_off, part_off, sum_off;
 };
+
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A wait of at most about a second; when one runs out, the kernel's status word is set and no other wait of the CTA goes on: the CTA runs
+// to its end with whatever it has.
+__device__ __forceinline__ void mx_wait(uint32_t bar, uint32_t parity, int *dead, int status) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*static_cast<volatile int *>(dead)) return;
+        if (global_ns() - t0 > 1000000000ull) {
+            atomicExch(dead, 1);
+            atomicExch(&g_staged_status, status);
+            return;
+        }
+    }
+}
 
 __device__ __forceinline__ uint4 load_stream16(const uint8_t *p) {
     uint4 v;
@@ -45,283 +70,328 @@ __device__ __forceinline__ uint32_t load_stream4(const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
-__device__ __forceinline__ uint4 load_written16(const uint16_t *p) {
-    uint4 v;
-    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
-    return v;
-}
 
-// shared memory: X fragments, their scales, the warps' parts, the CTA's parts (two batches, only of a cluster)
-template <int NT>
-struct MxRowsPlan {
-    static constexpr int kCols = 8 * NT;
-    static constexpr int kParts = kMxBatch * kMxRowWarps * NT * 128;         // floats
-    static constexpr int kSums = kMxBatch * 16 * kCols;                      // floats of a batch
-    static __host__ __device__ uint32_t row_bytes(int part_groups) { return static_cast<uint32_t>(part_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
-    static __host__ __device__ uint32_t scale_off(int rows, int part_groups) { return static_cast<uint32_t>(rows) * row_bytes(part_groups); }
-    static __host__ __device__ uint32_t part_off(int rows, int part_groups) { return scale_off(rows, part_groups) + static_cast<uint32_t>(part_groups) * kCols * 4u; }
-    static __host__ __device__ uint32_t total(int rows, int part_groups, int cluster) {
-        return part_off(rows, part_groups) + kParts * 4u + (cluster > 1 ? 2u * kSums * 4u : 0u);
-    }
+// A form of the kernel: MT tiles of weight rows by NT blocks of eight rows of X, up to kWarps multiplying warps, kDepth units in flight a
+// warp, kFinishers warps for the outputs, kPerSm CTAs an SM.
+template <int MT_, int NT_, int kWarps_, int kFinishers_, int kPerSm_, int kDepth_, bool kGated_>
+struct MxRowsForm {
+    static constexpr int MT = MT_, NT = NT_, kWarps = kWarps_, kFinishers = kFinishers_, kPerSm = kPerSm_, kDepth = kDepth_;
+    static constexpr bool kGated = kGated_;
+    static constexpr int kThreads = 32 * (kWarps_ + kFinishers_);
+    static constexpr int kPart = MT * NT * 32;                               // float4s of a warp's part of a step
+    static constexpr int kSum = (kGated ? 2 : MT) * NT * 32;                 // float4s of a step's sums
+    static __host__ __device__ uint32_t row_bytes(int chunk_groups) { return static_cast<uint32_t>(chunk_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
 };
 
-template <int NT, int kDepth, bool kGated>
-__global__ void __launch_bounds__(kMxRowThreads, 2) mx_rows_kernel(const MxRowsArgs A) {
+// byte j of a scale word as 2^(s - 127); the smallest scale, 2^-127, counts as zero here, 255 as infinity (its codes are zero)
+__device__ __forceinline__ float scale_of(uint32_t word, int j) {
+    return __uint_as_float((j < 3 ? word << (23 - 8 * j) : word >> 1) & 0x7F800000u);
+}
+
+template <class Form>
+__global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(const MxRowsArgs A) {
+    constexpr int MT = Form::MT, NT = Form::NT, kDepth = Form::kDepth, kCols = 8 * NT;
+    constexpr bool kGated = Form::kGated;
     extern __shared__ __align__(1024) uint8_t smem[];
-    using Plan = MxRowsPlan<NT>;
+    __shared__ __align__(8) uint64_t bars[2 * kMxPartsMax + 1];
+    __shared__ int dead;                                                     // a wait has run out: no other one waits any more
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int size = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-    const int first_step = blockIdx.x / size, stride = gridDim.x / size;
-    const int group0 = rank * A.part_groups;
-    const int groups = max(0, min(A.W.groups - group0, A.part_groups));      // of this CTA
-    const int mine = (groups - warp + kMxRowWarps - 1) / kMxRowWarps;        // of this warp: warp, warp + 8, ...
-    const int my_steps = first_step < A.steps ? (A.steps - first_step + stride - 1) / stride : 0;
+    const int my_steps = (A.steps - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    const int chunks = (A.W.groups + A.chunk_groups - 1) / A.chunk_groups;
+    const uint32_t base = smem_addr(smem);
+    const uint32_t part_full = smem_addr(&bars[0]), part_empty = part_full + 8 * kMxPartsMax, x_bar = part_empty + 8 * kMxPartsMax;
 
     pdl_launch_dependents();
-
-    // ---- the stream of units: (step, group) pairs of this warp, kDepth ahead ---------------------------------------------
-    uint4 qa[kDepth], qb[kDepth];
-    uint32_t sa[kDepth], sb[kDepth];
-    const uint8_t *ca, *cb, *ea, *eb;                                        // rows of the step that is being requested
-    auto rows_of = [&](int step) {
-        int ma, mb;
-        if constexpr (kGated) {
-            ma = min(8 * step + g, A.outs - 1);                              // past the last one: nobody reads the result
-            mb = ma + A.outs;
-        } else {
-            ma = 16 * step + g;                                              // rows up to the end of the tile exist
-            mb = ma + 8;
+    if (tid == 0) {
+        for (int i = 0; i < A.parts; i++) {
+            mbar_init(part_full + 8 * i, A.consumers);
+            mbar_init(part_empty + 8 * i, Form::kFinishers);
         }
-        const int64_t at = group0 + warp;
-        ca = A.W.codes + mx_code_row(ma, A.W.groups) + at * kMxTileCodes + t * 16;
-        cb = A.W.codes + mx_code_row(mb, A.W.groups) + at * kMxTileCodes + t * 16;
-        ea = A.W.scales + mx_scale_row(ma, A.W.groups) + at * kMxTileScales;
-        eb = A.W.scales + mx_scale_row(mb, A.W.groups) + at * kMxTileScales;
-    };
-    const int total = mine > 0 ? my_steps * mine : 0;
-    int asked = 0, ask_group = 0, ask_step = first_step;
-    if (total > 0) rows_of(ask_step);
-    auto request = [&](int slot) {
-        if (asked < total) {
-            qa[slot] = load_stream16(ca);
-            qb[slot] = load_stream16(cb);
-            sa[slot] = load_stream4(ea);
-            sb[slot] = load_stream4(eb);
-            asked++;
-            ca += kMxRowWarps * kMxTileCodes;
-            cb += kMxRowWarps * kMxTileCodes;
-            ea += kMxRowWarps * kMxTileScales;
-            eb += kMxRowWarps * kMxTileScales;
-            if (++ask_group == mine) {
-                ask_group = 0;
-                ask_step += stride;
-                if (asked < total) rows_of(ask_step);
-            }
-        }
-    };
-#pragma unroll
-    for (int d = 0; d < kDepth; d++) request(d);
-
-    // ---- X to FP16 fragments: chunk (group, block, quarter) of a row is eight values, in the order of a word's nibbles --------
-    pdl_wait();
-    const uint32_t row_bytes = Plan::row_bytes(A.part_groups);
-    float *xscale = reinterpret_cast<float *>(smem + Plan::scale_off(A.rows, A.part_groups));
-    for (int i = tid >> 4; i < A.rows * groups; i += kMxRowThreads / 16) {
-        const int r = i / groups, gr = i % groups, c = lane & 15;
-        const int k = (group0 + gr) * kMxGroup + c * 8;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (k < A.W.K) v = load_written16(A.X + static_cast<int64_t>(r) * A.W.K + k);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t top = 0u;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t lo = w[j] & 0x7FFFu, hi = (w[j] >> 16) & 0x7FFFu;
-            top = max(top, lo < 0x7F80u ? lo : 0u);                          // infinities and NaNs keep themselves whatever the scale
-            top = max(top, hi < 0x7F80u ? hi : 0u);
-        }
-        const uint32_t half = 0xFFFFu << (lane & 16);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half, top, o));
-        const uint32_t up = min(268u - (top >> 7), 253u);                    // exponent field of 2^(14 - floor(log2 top))
-        const float scale = __uint_as_float(up << 23);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            f[2 * j] = bf16lo_to_f32(w[j]) * scale;
-            f[2 * j + 1] = bf16hi_to_f32(w[j]) * scale;
-        }
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            // (e0, e2) (e4, e6) (e1, e3) (e5, e7)
-            const int e = (j & 1) * 4 + (j >> 1);
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[j]) : "f"(f[e + 2]), "f"(f[e]));
-        }
-        *reinterpret_cast<uint4 *>(smem + r * row_bytes + gr * 256 + c * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (c == 0) xscale[gr * Plan::kCols + r] = __uint_as_float((254u - up) << 23);
+        mbar_init(x_bar, 1);
+        mbar_fence_init();
+        dead = 0;
     }
     __syncthreads();
 
-    // ---- the products -------------------------------------------------------------------------------------------------------
-    float *parts = reinterpret_cast<float *>(smem + Plan::part_off(A.rows, A.part_groups));
-    float *sums = parts + Plan::kParts;
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) acc[n][c] = 0.f;
+    float4 *parts = reinterpret_cast<float4 *>(smem + A.part_off);
+    if (warp >= A.consumers) {
+        // ---- sums over the warps and chunks, outputs ------------------------------------------------------------------------
+        const int finisher = warp - A.consumers;
+        float4 *sums = reinterpret_cast<float4 *>(smem + A.sum_off);
+        const int stride = A.consumers * Form::kPart;                        // of the parts of a step
+        auto store = [&](int m, int col, float v, float u) {                 // u: of a gated pair
+            if (m >= A.outs || col >= A.rows) return;
+            const int64_t at = static_cast<int64_t>(col) * A.outs + m;
+            if (A.bias != nullptr) {
+                v += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m)) << 16);
+                if constexpr (kGated) u += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + A.outs + m)) << 16);
+            }
+            if constexpr (kGated) {
+                A.Y[at] = f32_to_bf16_rn(mx_act(A.activation, v) * u);
+                if (A.pre != nullptr) {
+                    A.pre[at + static_cast<int64_t>(col) * A.outs] = v;
+                    A.pre[at + static_cast<int64_t>(col + 1) * A.outs] = u;
+                }
+            } else {
+                A.Y[at] = f32_to_bf16_rn(v);
+            }
+        };
+        pdl_wait();                                                          // outputs may be what the previous kernel reads, a bias what it writes
+        int slot = 0;
+        uint32_t phase = 0u;
+        for (int c = 0; c < chunks; c++) {
+            for (int i = 0; i < my_steps; i++) {
+                const int step = blockIdx.x + i * gridDim.x;
+                mx_wait(part_full + 8 * slot, phase, &dead, 12);
+                const float4 *src = parts + slot * stride;
+                constexpr int kItems = kGated ? NT : MT * NT;
+                for (int item = finisher; item < kItems; item += Form::kFinishers) {
+                    const int at = item * 32 + lane, n = item % NT;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+                    for (int w = 0; w < A.consumers; w++) {
+                        const float4 p = src[w * Form::kPart + at];
+                        v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+                    }
+                    if constexpr (kGated) {
+                        // up rows lie (outs mod 16) rows further on in their tiles
+                        const int r0 = (A.outs & 15) + g, r1 = r0 + 8;
+                        auto half = [&](int r) { return (((1 + (r >> 4)) * NT + n) * 32 + (r & 7) * 4 + t) * 2 + ((r >> 3) & 1); };
+                        const int h0 = half(r0), h1 = half(r1);
+                        for (int w = 0; w < A.consumers; w++) {
+                            const float2 *s2 = reinterpret_cast<const float2 *>(src + w * Form::kPart);
+                            const float2 p = s2[h0], q = s2[h1];
+                            u.x += p.x, u.y += p.y, u.z += q.x, u.w += q.y;
+                        }
+                    }
+                    float4 *keep = sums + i * Form::kSum + at;
+                    if (c > 0) {
+                        const float4 p = *keep;
+                        v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+                        if constexpr (kGated) {
+                            const float4 q = keep[NT * 32];
+                            u.x += q.x, u.y += q.y, u.z += q.z, u.w += q.w;
+                        }
+                    }
+                    if (c + 1 < chunks) {
+                        *keep = v;
+                        if constexpr (kGated) keep[NT * 32] = u;
+                        continue;
+                    }
+                    const int m = 16 * (kGated ? step : MT * step + item / NT) + g, col = 8 * n + 2 * t;
+                    store(m, col, v.x, u.x);
+                    store(m, col + 1, v.y, u.y);
+                    store(m + 8, col, v.z, u.z);
+                    store(m + 8, col + 1, v.w, u.w);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(part_empty + 8 * slot);
+                if (++slot == A.parts) slot = 0, phase ^= 1u;
+            }
+        }
+        return;
+    }
+
+    // ---- consumers ------------------------------------------------------------------------------------------------------------
+    const uint32_t row_bytes = Form::row_bytes(A.chunk_groups);
+    float *xscale = reinterpret_cast<float *>(smem + A.scale_off);
+    const int threads = 32 * A.consumers;
+    auto together = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
     uint32_t xat[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) xat[n] = static_cast<uint32_t>(min(8 * n + g, A.rows - 1)) * row_bytes + t * 16;
+    int part = 0;
+    uint32_t part_phase = 1u;
 
-    auto multiply = [&](const uint4 &wa, const uint4 &wb, uint32_t ka, uint32_t kb, int gr) {
-        const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
-        float cg[NT][4];
+
+    // ---- the warp's units of a chunk: (step, group) pairs numbered over all steps, every consumers-th one, kDepth ahead of their use -----
+    uint4 qa[kDepth][MT], qb[kDepth][MT];
+    uint32_t sa[kDepth][MT], sb[kDepth][MT];
+    // Tiles of the step that is being requested, at this lane's row and the next group: 16-byte units of codes, bytes of scales (a
+    // row's scales lie at a sixteenth of its codes' offset; row b is eight rows on).
+    const uint8_t *codes = A.W.codes + t * 16, *scales = A.W.scales;
+    uint32_t at[MT];
+    int ask_step, ask_group, asked, units;
+    auto tiles_of = [&](int c0) {
+        const int step = blockIdx.x + ask_step * gridDim.x, last = (A.W.M - 1) >> 4;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) cg[n][c] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t ha[4], hb[4];
-            mx_word_to_f16(va[j], ha);
-            mx_word_to_f16(vb[j], hb);
-            // byte j of the scale words to the exponent field; the smallest scale, 2^-127, counts as zero here
-            const float fa = __uint_as_float(j < 3 ? (ka << (23 - 8 * j)) & 0x7F800000u : (ka >> 1) & 0x7F800000u);
-            const float fb = __uint_as_float(j < 3 ? (kb << (23 - 8 * j)) & 0x7F800000u : (kb >> 1) & 0x7F800000u);
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(smem + xat[n] + gr * 256 + j * 64);
-                float c[4];
-                mma_f16_first(c, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
-                mma_f16(c, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
-                cg[n][0] = fmaf(c[0], fa, cg[n][0]);
-                cg[n][1] = fmaf(c[1], fa, cg[n][1]);
-                cg[n][2] = fmaf(c[2], fb, cg[n][2]);
-                cg[n][3] = fmaf(c[3], fb, cg[n][3]);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const float2 xs = *reinterpret_cast<const float2 *>(xscale + gr * Plan::kCols + 8 * n + 2 * t);
-            acc[n][0] = fmaf(cg[n][0], xs.x, acc[n][0]);
-            acc[n][1] = fmaf(cg[n][1], xs.y, acc[n][1]);
-            acc[n][2] = fmaf(cg[n][2], xs.x, acc[n][2]);
-            acc[n][3] = fmaf(cg[n][3], xs.y, acc[n][3]);
+        for (int q = 0; q < MT; q++) {                                       // a tile past the end: the last one, nobody reads its results
+            const int tile = kGated ? (q == 0 ? step : (A.outs >> 4) + step + q - 1) : MT * step + q;
+            at[q] = (static_cast<uint32_t>(min(tile, last)) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16) + g * 4;
         }
     };
-
-    // an output of a batch: value (row in step, column of X) as the sum of the warps' parts
-    auto part_sum = [&](int p, int row, int col) {
-        const float *src = parts + ((p * kMxRowWarps * NT + (col >> 3)) * 32 + (row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + (col & 1);
-        float s = 0.f;
+    auto request = [&](int slot, int c0, int groups) {                       // past the last unit: the last one again, without effect
 #pragma unroll
-        for (int w = 0; w < kMxRowWarps; w++) s += src[w * NT * 128];
-        return s;
-    };
-    auto finish = [&](int step0, int steps) {                                // `steps` steps from step0 on are in `parts`
-        __syncthreads();
-        const uint32_t sums_at = smem_addr(sums) + ((step0 / kMxBatch) & 1) * Plan::kSums * 4u;
-        if (size > 1) {
-            float *mine_sums = sums + ((step0 / kMxBatch) & 1) * Plan::kSums;
-            for (int i = tid; i < steps * 16 * A.rows; i += kMxRowThreads) {
-                const int row = i & 15, p = (i >> 4) % steps, col = (i >> 4) / steps;
-                mine_sums[(p * Plan::kCols + col) * 16 + row] = part_sum(p, row, col);
-            }
-            cluster_sync();
+        for (int q = 0; q < MT; q++) {
+            const uint8_t *p = codes + static_cast<uint64_t>(at[q]) * 16, *s = scales + at[q];
+            qa[slot][q] = load_stream16(p);
+            qb[slot][q] = load_stream16(p + 512);
+            sa[slot][q] = load_stream4(s);
+            sb[slot][q] = load_stream4(s + 32);
         }
-        auto value = [&](int p, int row, int col) {
-            if (size == 1) return part_sum(p, row, col);
-            float s = 0.f;
-            for (int q = 0; q < size; q++) s += cluster_load(sums_at + ((p * Plan::kCols + col) * 16 + row) * 4, q);
-            return s;
-        };
-        constexpr int kPer = kGated ? 8 : 16;
-        // row fastest: neighbouring threads write neighbouring outputs
-        for (int i = tid + rank * kMxRowThreads; i < steps * kPer * A.rows; i += kMxRowThreads * size) {
-            const int row = i % kPer, p = i / kPer % steps, col = i / (kPer * steps);
-            const int m = (first_step + (step0 + p) * stride) * kPer + row;
-            if (m >= A.outs) continue;
-            if constexpr (kGated) {
-                float gv = value(p, row, col), uv = value(p, row + 8, col);
-                if (A.bias != nullptr) {
-                    gv += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m)) << 16);
-                    uv += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + A.outs + m)) << 16);
-                }
-                A.Y[static_cast<int64_t>(col) * A.outs + m] = f32_to_bf16_rn(mx_act(A.activation, gv) * uv);
-                if (A.pre != nullptr) {
-                    A.pre[static_cast<int64_t>(col) * 2 * A.outs + m] = gv;
-                    A.pre[static_cast<int64_t>(col) * 2 * A.outs + A.outs + m] = uv;
-                }
+        if (++asked < units) {
+            ask_group += A.consumers;
+            if (ask_group >= groups) {
+                ask_group -= groups;
+                ask_step++;
+                tiles_of(c0);
             } else {
-                float v = value(p, row, col);
-                if (A.bias != nullptr) v += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m)) << 16);
-                A.Y[static_cast<int64_t>(col) * A.outs + m] = f32_to_bf16_rn(v);
+#pragma unroll
+                for (int q = 0; q < MT; q++) at[q] += A.consumers * (kMxTileCodes / 16);
             }
         }
-        __syncthreads();
     };
-
-    int step = 0, group = 0, gr = warp;
-    auto end_of_step = [&]() {                                               // this warp's part of a step is complete
-        float *dst = parts + (((step % kMxBatch) * kMxRowWarps + warp) * NT * 32 + lane) * 4;
+    auto begin_chunk = [&](int c0, int groups) {
+        ask_step = 0;
+        ask_group = warp;
+        asked = 0;
+        units = (my_steps * groups - warp + A.consumers - 1) / A.consumers;
+        if (units > 0) {
+            tiles_of(c0);
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            *reinterpret_cast<float4 *>(dst + n * 128) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-#pragma unroll
-            for (int c = 0; c < 4; c++) acc[n][c] = 0.f;
+            for (int d = 0; d < kDepth; d++) request(d, c0, groups);
         }
-        step++;
-        if (step % kMxBatch == 0) finish(step - kMxBatch, kMxBatch);
     };
-    if (total == 0) {
-        while (step < my_steps) end_of_step();                               // a warp without groups still adds its zeros
-    } else {
-        for (int u = 0; u < total; u += kDepth) {
+    begin_chunk(0, min(A.chunk_groups, A.W.groups));
+    for (int c = 0; c < chunks; c++) {
+        const int c0 = c * A.chunk_groups, groups = min(A.chunk_groups, A.W.groups - c0);
+
+        // X: rows as they are by the copy engine, then to FP16 fragments in place: chunk (group, block, quarter) is eight values, in the
+        // order of a word's nibbles
+        const int x_bytes = 2 * min(A.W.K - c0 * kMxGroup, groups * kMxGroup);       // of a row
+        if (c > 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            begin_chunk(c0, groups);
+            together();                                                      // nobody reads the last chunk's X any more
+        }
+        if (warp == 0) {
+            if (c == 0) pdl_wait();
+            if (lane == 0) mbar_expect_tx(x_bar, static_cast<uint32_t>(x_bytes * A.rows));
+            __syncwarp();
+            if (lane < A.rows) bulk_copy_g2s(base + lane * row_bytes, A.X + static_cast<int64_t>(lane) * A.W.K + c0 * kMxGroup, x_bytes, x_bar);
+        }
+        mx_wait(x_bar, c & 1, &dead, 10);
+        {
+            const int teams = threads / 16, ch = lane & 15;                  // half a warp takes a group of a row
+            const uint32_t half = 0xFFFFu << (lane & 16);
+            constexpr int kAtOnce = 4;
+            const int jobs = groups * A.rows;
+            for (int job0 = tid >> 4; job0 < jobs; job0 += teams * kAtOnce) {
+                uint32_t w[kAtOnce][4], top[kAtOnce], at[kAtOnce], xs_at[kAtOnce];
 #pragma unroll
-            for (int d = 0; d < kDepth; d++) {
-                if (u + d < total) {
-                    multiply(qa[d], qb[d], sa[d], sb[d], gr);
-                    request(d);
-                    gr += kMxRowWarps;
-                    if (++group == mine) {
-                        group = 0;
-                        gr = warp;
-                        end_of_step();
+                for (int q = 0; q < kAtOnce; q++) {
+                    const int job = min(job0 + q * teams, jobs - 1), gr = job / A.rows, r = job - gr * A.rows;
+                    at[q] = r * row_bytes + gr * 256 + ch * 16;
+                    xs_at[q] = gr * kCols + r;
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (gr * 256 + ch * 16 < x_bytes && job0 + q * teams < jobs) v = *reinterpret_cast<const uint4 *>(smem + at[q]);
+                    w[q][0] = v.x, w[q][1] = v.y, w[q][2] = v.z, w[q][3] = v.w;
+                    top[q] = 0u;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t lo = w[q][j] & 0x7FFFu, hi = (w[q][j] >> 16) & 0x7FFFu;
+                        top[q] = max(top[q], lo < 0x7F80u ? lo : 0u);        // infinities and NaNs keep themselves whatever the scale
+                        top[q] = max(top[q], hi < 0x7F80u ? hi : 0u);
+                    }
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                    for (int q = 0; q < kAtOnce; q++) top[q] = max(top[q], __shfl_xor_sync(half, top[q], o));
+#pragma unroll
+                for (int q = 0; q < kAtOnce; q++) {
+                    if (job0 + q * teams >= jobs) break;
+                    const uint32_t up = min(268u - (top[q] >> 7), 253u);     // exponent field of 2^(14 - floor(log2 top))
+                    const float scale = __uint_as_float(up << 23);
+                    uint32_t h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        // (e0, e2) (e4, e6) (e1, e3) (e5, e7): element e is half e & 1 of word e >> 1
+                        const uint32_t a = w[q][(j & 1) * 2], b = w[q][(j & 1) * 2 + 1];
+                        const float lo = (j >> 1 ? bf16hi_to_f32(a) : bf16lo_to_f32(a)) * scale, hi = (j >> 1 ? bf16hi_to_f32(b) : bf16lo_to_f32(b)) * scale;
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[j]) : "f"(hi), "f"(lo));
+                    }
+                    *reinterpret_cast<uint4 *>(smem + at[q]) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (ch == 0) xscale[xs_at[q]] = __uint_as_float((254u - up) << 23);
+                }
+            }
+        }
+        together();
+
+        float acc[MT][NT][4];
+#pragma unroll
+        for (int q = 0; q < MT; q++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[q][n][k] = 0.f;
+        int gr = warp;
+        auto multiply = [&](int d) {
+            float cg[MT][NT][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint4 x[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) x[n] = *reinterpret_cast<const uint4 *>(smem + xat[n] + gr * 256 + j * 64);
+#pragma unroll
+                for (int q = 0; q < MT; q++) {
+                    const uint4 &wa = qa[d][q], &wb = qb[d][q];
+                    uint32_t ha[4], hb[4];
+                    mx_word_to_f16(j == 0 ? wa.x : j == 1 ? wa.y : j == 2 ? wa.z : wa.w, ha);
+                    mx_word_to_f16(j == 0 ? wb.x : j == 1 ? wb.y : j == 2 ? wb.z : wb.w, hb);
+                    const float fa = scale_of(sa[d][q], j), fb = scale_of(sb[d][q], j);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float e[4];
+                        mma_f16_first(e, ha[0], hb[0], ha[1], hb[1], x[n].x, x[n].y);
+                        mma_f16(e, ha[2], hb[2], ha[3], hb[3], x[n].z, x[n].w);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) cg[q][n][k] = j == 0 ? e[k] * (k < 2 ? fa : fb) : fmaf(e[k], k < 2 ? fa : fb, cg[q][n][k]);
                     }
                 }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float2 xs = *reinterpret_cast<const float2 *>(xscale + gr * kCols + 8 * n + 2 * t);
+#pragma unroll
+                for (int q = 0; q < MT; q++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[q][n][k] = fmaf(cg[q][n][k], k & 1 ? xs.y : xs.x, acc[q][n][k]);
+            }
+            gr += A.consumers;
+        };
+        auto end_of_step = [&]() {                                           // this warp's part of a step is complete
+            gr -= groups;
+            mx_wait(part_empty + 8 * part, part_phase, &dead, 14);
+            float4 *dst = parts + (part * A.consumers + warp) * Form::kPart + lane;
+#pragma unroll
+            for (int q = 0; q < MT; q++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    dst[(q * NT + n) * 32] = make_float4(acc[q][n][0], acc[q][n][1], acc[q][n][2], acc[q][n][3]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[q][n][k] = 0.f;
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(part_full + 8 * part);
+            if (++part == A.parts) part = 0, part_phase ^= 1u;
+        };
+        int u = 0;
+        for (; u + kDepth <= units; u += kDepth) {
+#pragma unroll
+            for (int d = 0; d < kDepth; d++) {
+                multiply(d);
+                request(d, c0, groups);
+                if (gr >= groups) end_of_step();
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            if (u + d < units) {
+                multiply(d);
+                if (gr >= groups) end_of_step();
+            }
         }
     }
-    if (step % kMxBatch != 0) finish(step - step % kMxBatch, step % kMxBatch);
-    if (size > 1) cluster_sync();                                            // nobody reads this CTA's sums any more
 }
 
 }  // namespace bhi
