@@ -92,90 +92,7 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, i
     }
 }
 
-// ---- products: one value after another ---------------------------------------------------------------------------------
-__device__ __forceinline__ float mx_value(const MxWeight &W, int m, int k) {
-    const int g = k >> 7, j = (k >> 5) & 3, t = (k >> 3) & 3, e = k & 7;
-    const int nibble = (e >> 1) + (e & 1) * 4;
-    const uint32_t byte = W.codes[mx_code_row(m, W.groups) + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4 + (nibble >> 1)];
-    const uint32_t code = (byte >> ((nibble & 1) * 4)) & 15u;
-    uint32_t h[4];
-    mx_word_to_f16(code, h);
-    return f16lo_to_f32(h[0]) * mx_scale(W.scales[mx_scale_row(m, W.groups) + g * kMxTileScales + j]);
-}
-
-constexpr int kMxTile = 32;          // 32 x 32 outputs a block, 32 terms at a time
-
-// out[r][c] of a tile: sum over i of A(r, i) B(c, i), A rows of activations, B the weight (kGrad: B(c, i) = W[i][c])
-template <bool kGrad>
-__device__ __forceinline__ void mx_tile_sum(const MxWeight &W, const uint16_t *A, int64_t rows, int lda, int64_t r0, int c0, int cols, int terms, int w0,
-                                            float (&sa)[kMxTile][kMxTile + 1], float (&sb)[kMxTile][kMxTile + 1], float (&acc)[4]) {
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int i0 = 0; i0 < terms; i0 += kMxTile) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int r = ty + 8 * q;
-            sa[r][tx] = (r0 + r < rows && i0 + tx < terms) ? __uint_as_float(static_cast<uint32_t>(A[(r0 + r) * lda + i0 + tx]) << 16) : 0.f;
-            if constexpr (kGrad) sb[r][tx] = (i0 + r < terms && c0 + tx < cols) ? mx_value(W, i0 + r, c0 + tx) : 0.f;
-            else sb[r][tx] = (c0 + r < cols && i0 + tx < terms) ? mx_value(W, w0 + c0 + r, i0 + tx) : 0.f;
-        }
-        __syncthreads();
-        for (int i = 0; i < kMxTile; i++) {
-            const float b = kGrad ? sb[i][tx] : sb[tx][i];
-#pragma unroll
-            for (int q = 0; q < 4; q++) acc[q] = fmaf(sa[ty + 8 * q][i], b, acc[q]);
-        }
-        __syncthreads();
-    }
-}
-
 __device__ __forceinline__ float bf16_at(const uint16_t *p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
-
-__global__ void __launch_bounds__(256) mx_linear_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, int64_t rows, int tiles_c) {
-    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
-    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
-    float acc[4] = {};
-    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, W.M, W.K, 0, sa, sb, acc);
-    for (int q = 0; q < 4; q++) {
-        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
-        if (r < rows && c < W.M) Y[r * W.M + c] = f32_to_bf16_rn(acc[q] + (bias ? bf16_at(bias, c) : 0.f));
-    }
-}
-
-__global__ void __launch_bounds__(256) mx_linear_grad_kernel(MxWeight W, const uint16_t *dY, int ldy, uint16_t *dX, int64_t rows, int tiles_c) {
-    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
-    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
-    float acc[4] = {};
-    mx_tile_sum<true>(W, dY, rows, ldy, r0, c0, W.K, W.M, 0, sa, sb, acc);
-    for (int q = 0; q < 4; q++) {
-        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
-        if (r < rows && c < W.K) dX[r * W.K + c] = f32_to_bf16_rn(acc[q]);
-    }
-}
-
-__global__ void __launch_bounds__(256) mx_gated_kernel(MxWeight W, const uint16_t *X, const uint16_t *bias, int act, uint16_t *H, float *pre, int64_t rows, int tiles_c) {
-    __shared__ float sa[kMxTile][kMxTile + 1], sb[kMxTile][kMxTile + 1];
-    const int inter = W.M / 2;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x / tiles_c) * kMxTile;
-    const int c0 = static_cast<int>(blockIdx.x % tiles_c) * kMxTile, c = c0 + (threadIdx.x & 31);
-    float g[4] = {}, u[4] = {};
-    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, inter, W.K, 0, sa, sb, g);
-    mx_tile_sum<false>(W, X, rows, W.K, r0, c0, inter, W.K, inter, sa, sb, u);
-    for (int q = 0; q < 4; q++) {
-        const int64_t r = r0 + (threadIdx.x >> 5) + 8 * q;
-        if (r >= rows || c >= inter) continue;
-        if (bias) {
-            g[q] += bf16_at(bias, c);
-            u[q] += bf16_at(bias, inter + c);
-        }
-        H[r * inter + c] = f32_to_bf16_rn(mx_act(act, g[q]) * u[q]);
-        if (pre) {
-            pre[r * W.M + c] = g[q];
-            pre[r * W.M + inter + c] = u[q];
-        }
-    }
-}
 
 // ---- the gated pair's gradient: dg = dh u act'(g), du = dh act(g) --------------------------------------------------------
 __global__ void __launch_bounds__(256) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, int act, uint16_t *dpre, int inter, int ldp, int64_t n) {
@@ -248,10 +165,7 @@ int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, 
         const int rc = mx_rows_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }
-    const int tiles_c = (M + kMxTile - 1) / kMxTile;
-    const int64_t blocks = static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c;
-    mx_linear_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), X, bias, Y, rows, tiles_c);
-    return mx_launched("product launch");
+    return mx_tile_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
 }
 
 int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *dY, int ldy, uint16_t *dX, int rows, void *stream) {
@@ -259,10 +173,7 @@ int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, in
     BHI_REQUIRE(rows >= 1, "no rows");
     BHI_REQUIRE(ldy >= M && ldy % 8 == 0, "rows of dY must be a multiple of 8 values apart");
     BHI_REQUIRE(dY && dX && aligned(dY, 16) && aligned(dX, 16), "dY and dX must be 16-byte aligned");
-    const int tiles_c = (K + kMxTile - 1) / kMxTile;
-    const int64_t blocks = static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c;
-    mx_linear_grad_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), dY, ldy, dX, rows, tiles_c);
-    return mx_launched("gradient launch");
+    return mx_grad_launch(mx_weight(codes, scales, M, K), dY, ldy, dX, rows, static_cast<cudaStream_t>(stream));
 }
 
 int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int K, const uint16_t *X, const uint16_t *bias, int activation, uint16_t *H,
@@ -277,11 +188,7 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
         const int rc = mx_rows_launch(W, X, bias, H, true, activation, pre, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }
-    const int tiles_c = (inter + kMxTile - 1) / kMxTile;
-    const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>((rows + kMxTile - 1) / kMxTile) * tiles_c);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    mx_gated_kernel<<<blocks, 256, 0, st>>>(W, X, bias, activation, H, pre, rows, tiles_c);
-    return mx_launched("gated product launch");
+    return mx_tile_launch(W, X, bias, H, true, activation, pre, rows, static_cast<cudaStream_t>(stream));
 }
 
 int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows, void *stream) {

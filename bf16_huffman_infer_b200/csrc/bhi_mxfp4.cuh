@@ -116,5 +116,7 @@ __device__ __forceinline__ float mx_act(int act, float g) {
 // The products' launchers, whose source files are compiled side by side.  Each returns kStagedDeclined for what it does not serve.
 // `gated`: W.M = 2 * outputs; pre may be null.
 int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st);
+int mx_tile_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st);
+int mx_grad_launch(const MxWeight &W, const uint16_t *dY, int ldy, uint16_t *dX, int rows, cudaStream_t st);
 
 }  // namespace bhi
