@@ -8,8 +8,8 @@ namespace bhi {
 // nearest, ties to the even code, saturated at 6.  A power of two divides exactly, subnormal values included, and the
 // hardware's conversion rounds and saturates so: every code is the format's own.  A block with an infinity or a NaN is NaN.
 //
-// A thread makes one word (8 values), the four threads of a block share its maximum; a warp reads 256 values of a row in one
-// piece and writes two 64-byte pieces.  Bound by memory: read once, written once.
+// A thread makes a word (8 values) of each of kMxQuantRows rows at once, the four threads of a block share its maximum; a warp reads
+// 256 values of a row in one piece and writes eight 16-byte pieces a row, four rows side by side.  Bound by memory: read once, written once.
 template <class T>
 __device__ __forceinline__ void mx_load8(const T *p, uint32_t (&bits)[8]);
 template <>
@@ -40,55 +40,76 @@ __device__ __forceinline__ void mx_load8<float>(const float *p, uint32_t (&bits)
     for (int i = 0; i < 8; i++) bits[i] = w[i];
 }
 
-constexpr int kMxQuantThreads = 256;
+constexpr int kMxQuantThreads = 512;                                     // at most
+constexpr int kMxQuantRows = 4;
 
 template <class T>
-__global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W, int M, int K, int groups, int64_t words, uint8_t *codes, uint8_t *scales) {
-    const int per_row = groups * 16;                                      // words of a row
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kMxQuantThreads + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * kMxQuantThreads) {
-        const int m = static_cast<int>(i / per_row), at = static_cast<int>(i % per_row);      // words is a multiple of 64: whole warps
-        uint32_t v[8] = {};
-        if (m < M && at * 8 < K) mx_load8(W + static_cast<int64_t>(m) * K + at * 8, v);
-        uint32_t top = 0u;
+__global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W, int M, int K, int groups, uint8_t *codes, uint8_t *scales) {
+    const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
+    const bool in_row = at < groups * 16;
+    const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
+    const int tiles16 = (M + 15) / 16 * 16;
+    for (int m0 = blockIdx.y * kMxQuantRows; m0 < tiles16; m0 += gridDim.y * kMxQuantRows) {       // 16 is a multiple of kMxQuantRows
+        uint32_t v[kMxQuantRows][8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, v[j] & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const uint32_t field = top >> 23;                                 // floor(log2 top) + 127 of a normal value
-        const bool nan = field == 255u;
-        const uint32_t byte = nan ? 255u : field > 2u ? field - 2u : 0u;
-        const float inv = __uint_as_float((254u - byte) << 23);           // 2^(127 - byte); not used for a NaN
-        uint32_t word = 0u;
-        if (!nan) {
-            float f[8];
+        for (int r = 0; r < kMxQuantRows; r++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = __uint_as_float(v[j]) * inv;
-            // bytes: (e0, e2) (e4, e6) (e1, e3) (e5, e7), the first in the low half
-            asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b0, %3, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %7, %5;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b2, %4, %2;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %6;\n\t"
-                "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-                : "=r"(word) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+            for (int i = 0; i < 8; i++) v[r][i] = 0u;
+            if (m0 + r < M && at * 8 < K) mx_load8(W + static_cast<int64_t>(m0 + r) * K + at * 8, v[r]);
         }
-        const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
-        const int64_t row = mx_code_row(m, groups);
-        *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4) = word;
-        if (t == 0) scales[mx_scale_row(m, groups) + g * kMxTileScales + j] = static_cast<uint8_t>(byte);
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) {
+            uint32_t top = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = max(top, v[r][i] & 0x7FFFFFFFu);
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const uint32_t field = top >> 23;                             // floor(log2 top) + 127 of a normal value
+            const bool nan = field == 255u;
+            const uint32_t byte = nan ? 255u : field > 2u ? field - 2u : 0u;
+            const float inv = __uint_as_float((254u - byte) << 23);       // 2^(127 - byte); not used for a NaN
+            uint32_t word = 0u;
+            if (!nan) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) f[i] = __uint_as_float(v[r][i]) * inv;
+                // bytes: (e0, e2) (e4, e6) (e1, e3) (e5, e7), the first in the low half
+                asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+                    "cvt.rn.satfinite.e2m1x2.f32 b0, %3, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %7, %5;\n\t"
+                    "cvt.rn.satfinite.e2m1x2.f32 b2, %4, %2;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %6;\n\t"
+                    "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+                    : "=r"(word) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+            }
+            if (in_row) {
+                const int64_t row = mx_code_row(m0 + r, groups);
+                *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4) = word;
+                if (t == 0) scales[mx_scale_row(m0 + r, groups) + static_cast<int64_t>(g) * kMxTileScales + j] = static_cast<uint8_t>(byte);
+            }
+        }
     }
 }
 
 // ---- the dense matrix ------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, int64_t words, uint16_t *Y) {
-    const int per_row = W.K / 8;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kMxQuantThreads + threadIdx.x; i < words; i += static_cast<int64_t>(gridDim.x) * kMxQuantThreads) {
-        const int m = static_cast<int>(i / per_row), at = static_cast<int>(i % per_row);
-        const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t *>(W.codes + mx_code_row(m, W.groups) + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4));
-        const float scale = mx_scale(__ldg(W.scales + mx_scale_row(m, W.groups) + g * kMxTileScales + j));
-        float v[8];
-        mx_word_to_f32(word, scale, v);
-        *reinterpret_cast<uint4 *>(Y + static_cast<int64_t>(m) * W.K + at * 8) =
-            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+__global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, uint16_t *Y) {
+    const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
+    if (at * 8 >= W.K) return;
+    const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
+    const uint8_t *codes = W.codes + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4, *scales = W.scales + static_cast<int64_t>(g) * kMxTileScales + j;
+    for (int m0 = blockIdx.y * kMxQuantRows; m0 < W.M; m0 += gridDim.y * kMxQuantRows) {
+        uint32_t word[kMxQuantRows], scale[kMxQuantRows];
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) {                          // rows up to the end of a tile exist
+            word[r] = __ldg(reinterpret_cast<const uint32_t *>(codes + mx_code_row(m0 + r, W.groups)));
+            scale[r] = __ldg(scales + mx_scale_row(m0 + r, W.groups));
+        }
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) {
+            float v[8];
+            mx_word_to_f32(word[r], mx_scale(scale[r]), v);
+            if (m0 + r < W.M)
+                *reinterpret_cast<uint4 *>(Y + static_cast<int64_t>(m0 + r) * W.K + at * 8) =
+                    make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        }
     }
 }
 
@@ -125,6 +146,13 @@ static int mx_stream_grid(int64_t items, int threads) {
     const int64_t blocks = (items + threads - 1) / threads, most = static_cast<int64_t>(sm_count()) * 16;
     return static_cast<int>(blocks < most ? blocks : most);
 }
+// Blocks and threads over the words of a row (whole warps, as few idle ones as possible) by rows, some eight blocks an SM.
+static void mx_matrix_grid(int words, int M, dim3 &grid, dim3 &block) {
+    const int across = (words + kMxQuantThreads - 1) / kMxQuantThreads;
+    block = dim3(((words + across - 1) / across + 31) / 32 * 32);
+    const int rows = (M + kMxQuantRows - 1) / kMxQuantRows, per_sm = 2048 / static_cast<int>(block.x), most = (sm_count() * per_sm * 2 + across - 1) / across;
+    grid = dim3(across, rows < most ? rows : most);
+}
 
 }  // namespace bhi
 
@@ -137,13 +165,13 @@ int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, u
     BHI_REQUIRE(W && aligned(W, 16), "the matrix must be 16-byte aligned");
     BHI_REQUIRE(dtype >= BHI_DTYPE_BF16 && dtype <= BHI_DTYPE_FP32, "unknown type");
     const int groups = (K + kMxGroup - 1) / kMxGroup;
-    const int64_t words = static_cast<int64_t>((M + 15) / 16 * 16) * groups * 16;
-    const int grid = mx_stream_grid(words, kMxQuantThreads);
+    dim3 grid, block;
+    mx_matrix_grid(groups * 16, (M + 15) / 16 * 16, grid, block);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-    case BHI_DTYPE_BF16: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const __nv_bfloat16 *>(W), M, K, groups, words, codes, scales); break;
-    case BHI_DTYPE_FP16: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const __half *>(W), M, K, groups, words, codes, scales); break;
-    default: mx_quantize_kernel<<<grid, kMxQuantThreads, 0, st>>>(static_cast<const float *>(W), M, K, groups, words, codes, scales); break;
+    case BHI_DTYPE_BF16: mx_quantize_kernel<<<grid, block, 0, st>>>(static_cast<const __nv_bfloat16 *>(W), M, K, groups, codes, scales); break;
+    case BHI_DTYPE_FP16: mx_quantize_kernel<<<grid, block, 0, st>>>(static_cast<const __half *>(W), M, K, groups, codes, scales); break;
+    default: mx_quantize_kernel<<<grid, block, 0, st>>>(static_cast<const float *>(W), M, K, groups, codes, scales); break;
     }
     return mx_launched("quantisation launch");
 }
@@ -151,8 +179,9 @@ int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, u
 int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, uint16_t *Y, void *stream) {
     if (int rc = mx_check(codes, scales, M, K)) return rc;
     BHI_REQUIRE(Y && aligned(Y, 16), "the output must be 16-byte aligned");
-    const int64_t words = static_cast<int64_t>(M) * (K / 8);
-    mx_dense_kernel<<<mx_stream_grid(words, kMxQuantThreads), kMxQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), words, Y);
+    dim3 grid, block;
+    mx_matrix_grid(K / 8, M, grid, block);
+    mx_dense_kernel<<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(mx_weight(codes, scales, M, K), Y);
     return mx_launched("dense launch");
 }
 

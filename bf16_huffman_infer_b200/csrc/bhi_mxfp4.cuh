@@ -4,10 +4,10 @@
 // two exponent bits, one mantissa bit; 0, 0.5, 1, 1.5, 2, 3, 4, 6).
 //
 // The rows are cut into tiles of 16 and the columns into groups of 128; both are padded with zeros.  One (tile, group) pair is
-// 1 KB of codes and 64 bytes of scales, so whatever walks along K reads whole lines, and a lane of an m16n8k16 product finds
-// the four words it needs of a row in one 16-byte load:
+// 1 KB of codes and 64 bytes of scales, so whatever walks along K reads whole lines.  A lane of an m16n8k16 product finds the four
+// words it needs of a row in one 16-byte load, and lanes that take a row each read 16 bytes side by side:
 //
-//   codes  [ceil(M / 16)][ceil(K / 128)][16 rows][4 quarters t][4 blocks j][4 bytes]   word (t, j): elements 8 t .. 8 t + 7 of block j
+//   codes  [ceil(M / 16)][ceil(K / 128)][4 quarters t][16 rows][4 blocks j][4 bytes]   word (t, j): elements 8 t .. 8 t + 7 of block j
 //   scales [ceil(M / 16)][ceil(K / 128)][16 rows][4 blocks j]
 //
 // Inside a word, nibble i is element 2 i and nibble 4 + i element 2 i + 1 (i = 0..3): a mask leaves the pair (2 i, 2 i + 1) in
@@ -31,12 +31,31 @@ struct MxWeight {
     int M, K, groups;                           // groups = ceil(K / 128)
 };
 
-// byte offsets of row m, group 0
+constexpr int kMxQuarter = 256;                 // bytes from a quarter of a row to the next
+
+// byte offsets of row m, group 0 (codes: quarter 0)
 __host__ __device__ __forceinline__ int64_t mx_code_row(int m, int groups) {
-    return static_cast<int64_t>(m >> 4) * groups * kMxTileCodes + (m & 15) * 64;
+    return static_cast<int64_t>(m >> 4) * groups * kMxTileCodes + (m & 15) * 16;
 }
 __host__ __device__ __forceinline__ int64_t mx_scale_row(int m, int groups) {
     return static_cast<int64_t>(m >> 4) * groups * kMxTileScales + (m & 15) * 4;
+}
+
+// A wait of at most about a second; when one runs out, the kernel's status word is set and no other wait of the CTA goes on: the CTA
+// runs to its end with whatever it has.
+__device__ __forceinline__ void mx_wait(uint32_t bar, uint32_t parity, int *dead, int status) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1; !mbar_try_wait(bar, parity); i++) {
+        if ((i & 1023u) != 0u) continue;
+        if (*static_cast<volatile int *>(dead)) return;
+        const uint64_t now = global_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > 1000000000ull) {
+            atomicExch(dead, 1);
+            atomicExch(&g_staged_status, status);
+            return;
+        }
+    }
 }
 
 // Byte b of a code word as two FP16 values: nibble 2 b in the low half, 2 b + 1 in the high half.

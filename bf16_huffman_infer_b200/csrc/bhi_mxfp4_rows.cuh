@@ -45,21 +45,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A wait of at most about a second; when one runs out, the kernel's status word is set and no other wait of the CTA goes on: the CTA runs
-// to its end with whatever it has.
-__device__ __forceinline__ void mx_wait(uint32_t bar, uint32_t parity, int *dead, int status) {
-    if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = global_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*static_cast<volatile int *>(dead)) return;
-        if (global_ns() - t0 > 1000000000ull) {
-            atomicExch(dead, 1);
-            atomicExch(&g_staged_status, status);
-            return;
-        }
-    }
-}
-
 __device__ __forceinline__ uint4 load_stream16(const uint8_t *p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -206,9 +191,9 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
     // ---- the warp's units of a chunk: (step, group) pairs numbered over all steps, every consumers-th one, kDepth ahead of their use -----
     uint4 qa[kDepth][MT], qb[kDepth][MT];
     uint32_t sa[kDepth][MT], sb[kDepth][MT];
-    // Tiles of the step that is being requested, at this lane's row and the next group: 16-byte units of codes, bytes of scales (a
-    // row's scales lie at a sixteenth of its codes' offset; row b is eight rows on).
-    const uint8_t *codes = A.W.codes + t * 16, *scales = A.W.scales;
+    // Tiles of the step that is being requested, at the next group: 16-byte units of codes, bytes of scales (a pair's scales lie at
+    // a sixteenth of its codes' offset; row b is eight rows on).
+    const uint8_t *codes = A.W.codes + t * kMxQuarter + g * 16, *scales = A.W.scales + g * 4;
     uint32_t at[MT];
     int ask_step, ask_group, asked, units;
     auto tiles_of = [&](int c0) {
@@ -216,7 +201,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
 #pragma unroll
         for (int q = 0; q < MT; q++) {                                       // a tile past the end: the last one, nobody reads its results
             const int tile = kGated ? (q == 0 ? step : (A.outs >> 4) + step + q - 1) : MT * step + q;
-            at[q] = (static_cast<uint32_t>(min(tile, last)) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16) + g * 4;
+            at[q] = (static_cast<uint32_t>(min(tile, last)) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16);
         }
     };
     auto request = [&](int slot, int c0, int groups) {                       // past the last unit: the last one again, without effect
@@ -224,7 +209,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
         for (int q = 0; q < MT; q++) {
             const uint8_t *p = codes + static_cast<uint64_t>(at[q]) * 16, *s = scales + at[q];
             qa[slot][q] = load_stream16(p);
-            qb[slot][q] = load_stream16(p + 512);
+            qb[slot][q] = load_stream16(p + 128);
             sa[slot][q] = load_stream4(s);
             sb[slot][q] = load_stream4(s + 32);
         }

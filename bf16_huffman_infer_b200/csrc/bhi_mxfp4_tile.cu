@@ -7,6 +7,8 @@ bool overlap_launches();
 
 namespace {
 
+constexpr uint32_t kSmemTile = kSmemMax - 1024;      // what the barriers leave
+
 // The tensor-map encoder lives in the driver library, which this library does not link: it is looked up through the runtime once.
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                    const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -20,13 +22,15 @@ EncodeTiledFn encode_tiled() {
     return fn;
 }
 
-// Rows of a tile (a multiple of 16, at most 256): the fewest rounds of tiles over the SMs times a tile's cost, which is its rows where the
+enum Kind { kPlain, kGatedPair, kGradient };
+
+// Rows of a tile (a multiple of 16, at most `most`): the fewest rounds of tiles over the SMs times a tile's cost, which is its rows where the
 // tensor cores bound it and that of kExpand rows where the expansion of the weight does.
-constexpr int kExpand = 144;
-int rows_of_tile(int rows, int tiles_p) {
+constexpr int kExpand = 128;
+int rows_of_tile(int rows, int tiles_p, int most) {
     int best = 16;
     double best_cost = 1e30;
-    for (int nt = 16; nt <= 256; nt += 16) {
+    for (int nt = 16; nt <= most; nt += 16) {
         const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * tiles_p;
         const double cost = static_cast<double>((tiles + sm_count() - 1) / sm_count()) * (nt > kExpand ? nt : kExpand) + 1e-3 * nt;
         if (cost < best_cost - 1e-9) {
@@ -38,32 +42,40 @@ int rows_of_tile(int rows, int tiles_p) {
     return best;
 }
 
-template <int kKind>
+template <Kind kKind>
 int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStream_t st) {
     EncodeTiledFn encode = encode_tiled();
     if (!encode) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    const int per = kKind == kMxGatedPair ? 64 : 128;
+    const int per = kKind == kGatedPair ? 64 : 128;
     a.tiles_p = (a.outs + per - 1) / per;
-    a.nt = rows_of_tile(a.rows, a.tiles_p);
+    a.nt = rows_of_tile(a.rows, a.tiles_p, kKind == kGradient ? kMtGradRows : kMtForwardRows);
     a.tiles_n = (a.rows + a.nt - 1) / a.nt;
     a.stages_c = static_cast<int>((b_cols + kMtStage - 1) / kMtStage);
     BHI_REQUIRE(static_cast<int64_t>(a.tiles_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
-    const uint32_t stage = kMtABytes + static_cast<uint32_t>(a.nt) * 128u, most = kSmemMax - 1024 - kMtSwap;
-    a.stages = static_cast<int>(most / stage);
+    const uint32_t stage = (kKind == kGradient ? kMtABytes : 0u) + static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;
+    a.stages = static_cast<int>((kSmemTile - extra) / stage);
     if (a.stages > kMtStagesMax) a.stages = kMtStagesMax;
+    a.stages &= ~1;
     alignas(64) CUtensorMap map;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(b_cols), static_cast<cuuint64_t>(a.rows)}, strides[1] = {static_cast<cuuint64_t>(ldb) * 2};
     const cuuint32_t box[2] = {kMtStage, static_cast<cuuint32_t>(a.nt)}, estr[2] = {1, 1};
-    CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(B), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto encoded = [&]() {
+        return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(B), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult cr = encoded();
+    if (cr == CUDA_ERROR_INVALID_CONTEXT) {          // a thread that has not called the runtime yet (an autograd thread): bind the device's context
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) cr = encoded();
+    }
     if (cr != CUDA_SUCCESS) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(cr)));
-    auto kernel = mx_tile_kernel<kKind>;
-    if (int rc = staged_prepare(kernel, kSmemMax - 1024)) return rc;
+    auto kernel = kKind == kGradient ? mx_grad_kernel : mx_tile_kernel<kKind == kGatedPair>;
+    if (int rc = staged_prepare(kernel, kSmemTile)) return rc;
     const int tiles = a.tiles_p * a.tiles_n;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles < sm_count() ? tiles : sm_count());
     cfg.blockDim = dim3(kMtThreads);
-    cfg.dynamicSmemBytes = a.stages * stage + kMtSwap;
+    cfg.dynamicSmemBytes = a.stages * stage + extra;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -79,13 +91,13 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
 int mx_tile_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st) {
     MxTileArgs a{};
     a.W = W, a.bias = bias, a.out = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
-    return gated ? launch<kMxGatedPair>(a, X, W.K, W.K, st) : launch<kMxPlain>(a, X, W.K, W.K, st);
+    return gated ? launch<kGatedPair>(a, X, W.K, W.K, st) : launch<kPlain>(a, X, W.K, W.K, st);
 }
 
 int mx_grad_launch(const MxWeight &W, const uint16_t *dY, int ldy, uint16_t *dX, int rows, cudaStream_t st) {
     MxTileArgs a{};
     a.W = W, a.out = dX, a.rows = rows, a.outs = W.K;
-    return launch<kMxGradient>(a, dY, W.M, ldy, st);
+    return launch<kGradient>(a, dY, W.M, ldy, st);
 }
 
 cudaError_t take_mxfp4_tile_status(int *out) { return take_status(out); }

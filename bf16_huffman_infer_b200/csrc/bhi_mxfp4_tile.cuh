@@ -2,17 +2,14 @@
 //
 //   out[n][p] = sum over c of B[n][c] A(p, c)      forward: p a weight row m, c a column k, B = X;  gradient: p a column k, c a weight row m, B = dY
 //
-// A tile is 128 values of p (the lanes of an accumulator) by NT rows of B (its columns), walked in stages of 64 values of c.  Eight warps turn
-// codes into BF16 in shared memory, exactly (a code times a power of two fits), one thread requests B by TMA, one issues the products, four warps
-// read the accumulators back, two of which alternate between tiles.  The weight is expanded once for up to 256 rows, so the expansion
-// (19 instructions for eight values) stays behind the tensor cores:
-//   * forward, a stage is [128 rows][64 columns], K-major;  gradient, [64 rows][128 columns], which is the MN-major form of the same operand:
-//     a word of eight codes is eight neighbours along k and so one 16-byte unit of either, and nothing is transposed;
-//   * both with the 128-byte swizzle, stores of a quarter warp on 32 different banks.
+// A tile is 128 values of p (the lanes of an accumulator) by NT rows of B (its columns).  Sixteen warps turn codes into BF16, exactly (a code
+// times a power of two fits), one thread requests B by TMA, 64 values of c at a time, one issues the products, four warps read the accumulators
+// back, two of which alternate between tiles.  The weight is expanded once for all rows of a tile, so the expansion (19 instructions
+// for eight values) stays behind the tensor cores from some 130 rows on.
+//
 // A code's bits s eem are moved to a BF16's sign, lowest exponent and highest mantissa bits: that is its value times 2^-126, the
 // subnormal code 0.5 included, and one product by 2^(126 + s - 127) makes both the value and its scale.  Scales above 2 (2^(126 + s - 127) would
 // overflow) take two products.
-// kGated: 64 gate rows and 64 up rows of the same outputs make a tile; half of each accumulator block changes lanes through shared memory.
 #pragma once
 
 #include <cuda.h>      // CUtensorMap and the encode entry point's types; the driver library is not linked
@@ -21,15 +18,14 @@
 
 namespace bhi {
 
-enum MxTileKind { kMxPlain = 0, kMxGatedPair = 1, kMxGradient = 2 };
-
 constexpr int kMtLoader = 0, kMtIssuer = 1, kMtEpilogue = 4, kMtConverter = 8;      // warps; 2 and 3 idle
-constexpr int kMtConverters = 8;
-constexpr int kMtThreads = 32 * (kMtConverter + kMtConverters);
+constexpr int kMtTeam = 8;                        // warps of a team of converters; two teams
+constexpr int kMtThreads = 32 * (kMtConverter + 2 * kMtTeam);
 constexpr int kMtStage = 64;                      // values of c
 constexpr uint32_t kMtABytes = 128 * kMtStage * 2;
-constexpr int kMtStagesMax = 10;
-constexpr uint32_t kMtSwap = 32 * 64 * 4;         // bytes through which a gated block changes lanes
+constexpr int kMtStagesMax = 16;
+constexpr uint32_t kMtSwap = 16 * 64 * 4;         // bytes through which a gated block changes lanes
+constexpr int kMtForwardRows = 192, kMtGradRows = 256;       // most rows of a tile
 
 struct MxTileArgs {
     MxWeight W;
@@ -52,6 +48,34 @@ __device__ __forceinline__ void mt_mma(uint32_t d, uint64_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// the same with A in tensor memory: lanes are rows, a column holds two neighbours along K
+__device__ __forceinline__ void mt_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mt_store8(uint32_t to, const uint4 &a, const uint4 &b) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(to), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void mt_load(uint32_t from, float (&v)[N]) {
+    static_assert(N == 16, "one width");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+                   "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(from));
+}
+// One lane of a converged warp.  The issuing warp runs its loop as a whole and elects a lane for the products alone: operands that the
+// compiler knows to be the same in all lanes stay in uniform registers.
+__device__ __forceinline__ bool mt_elect() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0u;
+}
+__device__ __forceinline__ void mt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mt_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -86,36 +110,244 @@ __device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t s, bool la
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-// A wait of at most about a second; when one runs out, the kernel's status word is set and no other wait of the CTA goes on.
-__device__ __forceinline__ void mt_wait(uint32_t bar, uint32_t parity, int *dead, int status) {
-    if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = global_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*static_cast<volatile int *>(dead)) return;
-        if (global_ns() - t0 > 1000000000ull) {
-            atomicExch(dead, 1);
-            atomicExch(&g_staged_status, status);
-            return;
+// ---- sums to outputs: a thread's lane of the accumulator is value p, columns are rows of out --------------------------------------------
+// kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16 columns the first eight become the gate lanes', the
+// others the up lanes': each hands the other half over through shared memory.
+template <bool kGated, int kBuffer>
+__device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, uint32_t done, uint32_t free_, float *swap, int *dead, int warp, int lane) {
+    const int quarter = warp & 3, lane_p = quarter * 32 + lane, tiles = A.tiles_p * A.tiles_n;
+    int buf = 0;
+    uint32_t phase = 0u;
+    pdl_wait();                                                              // outputs may be what the previous kernel reads, a bias what it writes
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int p = tile % A.tiles_p, n0 = tile / A.tiles_p * A.nt, cols = min(A.nt, A.rows - n0);
+        const int m = kGated ? 64 * p + (lane_p & 63) : 128 * p + lane_p;
+        const bool up = kGated && lane_p >= 64, live = m < A.outs;
+        float bias = 0.f;
+        if (A.bias != nullptr && live) bias = __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m + (up ? A.outs : 0))) << 16);
+        mx_wait(done + 8 * buf, phase, dead, 24);
+        mt_fence_after();
+        const uint32_t from = tmem + buf * kBuffer + (static_cast<uint32_t>(quarter) << 21);
+        for (int c = 0; c < cols; c += 16) {
+            float v[16];
+            mt_load(from + c, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (c + 16 >= cols) {                                            // the accumulator is read: the issuer may have it back
+                mt_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(free_ + 8 * buf);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] += bias;
+            if constexpr (!kGated) {
+                if (live) {
+                    uint16_t *to = A.out + static_cast<int64_t>(n0 + c) * A.outs + m;
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (c + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(v[i]);
+                }
+            } else {
+                if (A.pre != nullptr && live) {
+                    float *to = A.pre + static_cast<int64_t>(n0 + c) * 2 * A.outs + m + (up ? A.outs : 0);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (c + i < cols) to[static_cast<int64_t>(i) * 2 * A.outs] = v[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) swap[((up ? 0 : 8) + i) * 64 + (lane_p & 63)] = up ? v[i] : v[8 + i];
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+                const int i0 = up ? 8 : 0;
+                if (live) {
+                    uint16_t *to = A.out + static_cast<int64_t>(n0 + c + i0) * A.outs + m;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float other = swap[(i0 + i) * 64 + (lane_p & 63)];
+                        const float g = up ? other : v[i], u = up ? v[8 + i] : other;
+                        if (c + i0 + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(mx_act(A.activation, g) * u);
+                    }
+                }
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+            }
+        }
+        if ((buf ^= 1) == 0) phase ^= 1u;
+    }
+}
+
+// ---- B: 64 values of c of a tile's rows a stage --------------------------------------------------------------------------------------
+__device__ __forceinline__ void mt_loader(const MxTileArgs &A, const CUtensorMap *map, uint32_t base, uint32_t stage_bytes, uint32_t full, uint32_t empty, int *dead) {
+    pdl_wait();
+    int slot = 0;
+    uint32_t phase = 1u;
+    for (int tile = blockIdx.x; tile < A.tiles_p * A.tiles_n; tile += gridDim.x) {
+        const int n0 = tile / A.tiles_p * A.nt;
+        for (int c = 0; c < A.stages_c; c++) {
+            mx_wait(empty + 8 * slot, phase, dead, 20);
+            mbar_expect_tx(full + 8 * slot, static_cast<uint32_t>(A.nt) * 128u);
+            mt_tma_2d(base + slot * stage_bytes, map, c * kMtStage, n0, full + 8 * slot);
+            if (++slot == A.stages) slot = 0, phase ^= 1u;
         }
     }
 }
 
-template <int kKind>
+__device__ __forceinline__ uint32_t mt_begin(uint32_t *tmem_slot, int warp) {        // every thread; after the barriers are initialised
+    if (warp == kMtIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    mt_fence_before();
+    __syncthreads();
+    mt_fence_after();
+    return __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+}
+__device__ __forceinline__ void mt_end(uint32_t tmem, const int *dead, int warp) {
+    mt_fence_before();
+    __syncthreads();
+    if (*dead)                                                               // copies and products under way land before the memory goes
+        for (int i = 0; i < 10; i++) __nanosleep(100000);
+    __syncthreads();
+    if (warp == kMtIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---- forward: A in tensor memory ------------------------------------------------------------------------------------------------------
+// A thread of a team expands half a row's group (64 values) in registers while the other team's group is being multiplied, and stores
+// it to its lane of tensor memory when the products that read the place are done: the weight costs shared memory nothing, which B's way in
+// and out fills.  A team's place is its own.  Tensor memory: two accumulators of 192 columns, two groups of 64.
+// kGated: 64 gate rows and the 64 up rows of the same outputs make a tile.
+template <bool kGated>
 __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs A, const __grid_constant__ CUtensorMap bmap) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[2 * kMtStagesMax + 8];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int dead;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
+    const uint32_t base = smem_addr(smem), stage_bytes = static_cast<uint32_t>(A.nt) * 128u;
+    const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16,
+                   a_full = done + 32, a_empty = done + 48;
+    const int tiles = A.tiles_p * A.tiles_n, groups = A.W.groups;
+
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < A.stages; i++) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(done + 8 * i, 1);
+            mbar_init(free_ + 8 * i, 4);
+            mbar_init(a_full + 8 * i, kMtTeam);
+            mbar_init(a_empty + 8 * i, 1);
+        }
+        mbar_fence_init();
+        dead = 0;
+    }
+    const uint32_t tmem = mt_begin(&tmem_slot, warp);
+
+    if (warp == kMtLoader) {
+        if (lane == 0) mt_loader(A, &bmap, base, stage_bytes, full, empty, &dead);
+    } else if (warp == kMtIssuer) {
+        // 32-bit sums, both operands BF16 and K-major
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
+        int slot = 0, buf = 0, place = 0;
+        uint32_t phase = 0u, buf_phase = 1u, a_phase = 0u;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
+            mt_fence_after();
+            for (int c = 0; c < A.stages_c; c++) {
+                if ((c & 1) == 0) mx_wait(a_full + 8 * place, a_phase, &dead, 25);
+                mx_wait(full + 8 * slot, phase, &dead, 22);
+                mt_fence_after();
+                const bool last_of_group = (c & 1) || c + 1 == A.stages_c;
+                if (mt_elect()) {
+                    const uint32_t a = tmem + 2 * kMtForwardRows + place * 64 + (c & 1) * 32, d = tmem + buf * kMtForwardRows;
+                    const uint64_t b = mt_desc(base + slot * stage_bytes, 1);
+#pragma unroll
+                    for (int k = 0; k < kMtStage / 16; k++) mt_mma_ta(d, a + k * 8, b + 2 * k, idesc, c > 0 || k > 0);
+                    mt_commit(empty + 8 * slot);
+                    if (last_of_group) mt_commit(a_empty + 8 * place);
+                    if (c + 1 == A.stages_c) mt_commit(done + 8 * buf);
+                }
+                __syncwarp();
+                if (++slot == A.stages) slot = 0, phase ^= 1u;
+                if (last_of_group && (place ^= 1) == 0) a_phase ^= 1u;
+            }
+            if ((buf ^= 1) == 0) buf_phase ^= 1u;
+        }
+    } else if (warp >= kMtConverter) {
+        const int team = (warp - kMtConverter) / kMtTeam, quarter = warp & 3, half = ((warp - kMtConverter) >> 2) & 1, row = quarter * 32 + lane;
+        const uint8_t *cp = nullptr, *sp = nullptr;
+        int tile = blockIdx.x, g = team;
+        auto rows_of = [&]() {                                               // past the end: some other row, nobody reads the results
+            const int p = tile % A.tiles_p;
+            const int m = kGated ? min(64 * p + (row & 63), A.outs - 1) + (row >= 64 ? A.outs : 0) : min(128 * p + row, A.W.M - 1);
+            cp = A.W.codes + mx_code_row(m, groups) + half * 2 * kMxQuarter;
+            sp = A.W.scales + mx_scale_row(m, groups);
+        };
+        auto settle = [&]() {                                                // (tile, g) with g past the tile's groups: into the next tiles
+            bool moved = false;
+            while (g >= groups && tile < tiles) g -= groups, tile += gridDim.x, moved = true;
+            return moved;
+        };
+        uint4 q0 = make_uint4(0u, 0u, 0u, 0u), q1 = q0;
+        uint32_t s = 0u;
+        auto load = [&]() {
+            const uint8_t *c = cp + static_cast<int64_t>(g) * kMxTileCodes;
+            q0 = __ldg(reinterpret_cast<const uint4 *>(c));
+            q1 = __ldg(reinterpret_cast<const uint4 *>(c + kMxQuarter));
+            s = __ldg(reinterpret_cast<const uint32_t *>(sp + static_cast<int64_t>(g) * kMxTileScales));
+        };
+        settle();
+        if (tile < tiles) {
+            rows_of();
+            load();
+        }
+        const uint32_t to = tmem + 2 * kMtForwardRows + team * 64 + half * 8 + (static_cast<uint32_t>(quarter) << 21);
+        uint32_t phase = 1u;
+        while (tile < tiles) {
+            uint4 h[8];
+            const bool large = (s & 0x80808080u) != 0u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t byte = (s >> (8 * j)) & 255u;
+                h[2 * j] = mx_word_to_bf16(j == 0 ? q0.x : j == 1 ? q0.y : j == 2 ? q0.z : q0.w, byte, large);
+                h[2 * j + 1] = mx_word_to_bf16(j == 0 ? q1.x : j == 1 ? q1.y : j == 2 ? q1.z : q1.w, byte, large);
+            }
+            g += 2;
+            if (settle() && tile < tiles) rows_of();
+            if (tile < tiles) load();
+            mx_wait(a_empty + 8 * team, phase, &dead, 23);
+            phase ^= 1u;
+            mt_fence_after();
+#pragma unroll
+            for (int j = 0; j < 4; j++) mt_store8(to + 16 * j, h[2 * j], h[2 * j + 1]);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            mt_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_full + 8 * team);
+        }
+    } else if (warp >= kMtEpilogue) {
+        mt_epilogue<kGated, kMtForwardRows>(A, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane);
+    }
+    mt_end(tmem, &dead, warp);
+}
+
+// ---- gradient: A in shared memory -------------------------------------------------------------------------------------------------------
+// A stage is 64 weight rows by a group of columns.  A word of eight codes is eight neighbours along p and so one 16-byte unit of the MN-major
+// form of the operand: nothing is transposed.  128-byte swizzle, stores of a quarter warp on 32 different banks.  The teams take the stages of
+// the ring in turn (their number is even, so that a slot is always the same team's).
+__global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs A, const __grid_constant__ CUtensorMap bmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[2 * kMtStagesMax + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t base = smem_addr(smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
+    const uint32_t base = smem_addr(smem), stage_bytes = kMtABytes + static_cast<uint32_t>(A.nt) * 128u;
     const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16;
-    const uint32_t b_bytes = static_cast<uint32_t>(A.nt) * 128u, stage_bytes = kMtABytes + b_bytes;
     const int tiles = A.tiles_p * A.tiles_n;
 
     pdl_launch_dependents();
     if (tid == 0) {
         for (int i = 0; i < A.stages; i++) {
-            mbar_init(full + 8 * i, kMtConverters + 1);
+            mbar_init(full + 8 * i, kMtTeam + 1);
             mbar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -125,235 +357,79 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         mbar_fence_init();
         dead = 0;
     }
-    if (warp == kMtIssuer) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = mt_begin(&tmem_slot, warp);
 
     if (warp == kMtLoader) {
-        if (lane == 0) {
-            pdl_wait();
-            int slot = 0;
-            uint32_t phase = 1u;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                const int n0 = tile / A.tiles_p * A.nt;
-                for (int c = 0; c < A.stages_c; c++) {
-                    mt_wait(empty + 8 * slot, phase, &dead, 20);
-                    mbar_expect_tx(full + 8 * slot, b_bytes);
-                    mt_tma_2d(base + slot * stage_bytes + kMtABytes, &bmap, c * kMtStage, n0, full + 8 * slot);
-                    if (++slot == A.stages) slot = 0, phase ^= 1u;
-                }
-            }
-        }
+        if (lane == 0) mt_loader(A, &bmap, base + kMtABytes, stage_bytes, full, empty, &dead);
     } else if (warp == kMtIssuer) {
-        if (lane == 0) {
-            // 32-bit sums, both operands BF16, B K-major, A K-major or (gradient) MN-major
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kKind == kMxGradient ? 1u << 15 : 0u) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
-            int slot = 0, buf = 0;
-            uint32_t phase = 0u, buf_phase = 1u;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                mt_wait(free_ + 8 * buf, buf_phase, &dead, 21);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int c = 0; c < A.stages_c; c++) {
-                    mt_wait(full + 8 * slot, phase, &dead, 22);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t a = base + slot * stage_bytes, b = a + kMtABytes;
-#pragma unroll
-                    for (int k = 0; k < kMtStage / 16; k++)
-                        mt_mma(tmem + buf * 256, kKind == kMxGradient ? mt_desc(a + k * 2048, 512) : mt_desc(a + k * 32, 1), mt_desc(b + k * 32, 1), idesc, c > 0 || k > 0);
-                    mt_commit(empty + 8 * slot);
-                    if (++slot == A.stages) slot = 0, phase ^= 1u;
-                }
-                mt_commit(done + 8 * buf);
-                if ((buf ^= 1) == 0) buf_phase ^= 1u;
-            }
-        }
-    } else if (warp >= kMtConverter) {
-        // ---- codes to BF16 ---------------------------------------------------------------------------------------------------
-        const int w = warp - kMtConverter, t = lane & 3;
-        const int r8 = (lane >> 3) | (lane & 4);                     // rows 0, 4, 1, 5, 2, 6, 3, 7: a quarter warp's units lie on 32 banks
-        int slot = 0;
-        uint32_t phase = 1u;
-        auto begin = [&]() { mt_wait(empty + 8 * slot, phase, &dead, 23); };
-        auto end = [&]() {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * slot);
-            if (++slot == A.stages) slot = 0, phase ^= 1u;
-        };
-        if constexpr (kKind == kMxGradient) {
-            // stage c: rows 64 c .. of the weight, group p of columns; this thread's row and quarter
-            const int row = w * 8 + r8, storage_tiles = (A.W.M + 15) >> 4;
-            const uint32_t to = (row >> 3) * 1024 + (row & 7) * 128;
-            auto load = [&](int p, int c, uint4 &q, uint32_t &s) {
-                const int tile = 4 * c + (row >> 4);
-                q = make_uint4(0u, 0u, 0u, 0u);
-                s = 0u;
-                if (tile < storage_tiles) {
-                    const int64_t at = static_cast<int64_t>(tile) * A.W.groups + p;
-                    q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + (row & 15) * 64 + t * 16));
-                    s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
-                }
-            };
-            uint4 q;
-            uint32_t s;
-            if (static_cast<int>(blockIdx.x) < tiles) load(blockIdx.x % A.tiles_p, 0, q, s);
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                const int p = tile % A.tiles_p;
-                for (int c = 0; c < A.stages_c; c++) {
-                    const uint4 now = q;
-                    const uint32_t sc = s;
-                    if (c + 1 < A.stages_c) load(p, c + 1, q, s);
-                    else if (tile + static_cast<int>(gridDim.x) < tiles) load((tile + gridDim.x) % A.tiles_p, 0, q, s);
-                    const bool large = (sc & 0x80808080u) != 0u;
-                    begin();
-                    uint8_t *dst = smem + slot * stage_bytes + to;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint4 v = mx_word_to_bf16(j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w, (sc >> (8 * j)) & 255u, large);
-                        *reinterpret_cast<uint4 *>(dst + (j >> 1) * 8192 + ((((j & 1) * 4 + t) ^ (row & 7)) << 4)) = v;
-                    }
-                    end();
-                }
-            }
-        } else {
-            // stage c: columns 64 c .. of 128 weight rows; this thread's two rows and quarter, a group (two stages) loaded at a time
-            int row[2];
-            row[0] = w * 8 + r8;
-            row[1] = row[0] + 64;
-            const uint8_t *cp[2], *sp[2];
-            auto rows_of = [&](int p) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    int m;
-                    if constexpr (kKind == kMxGatedPair) m = i == 0 ? min(64 * p + row[0], A.outs - 1) : A.outs + min(64 * p + row[0], A.outs - 1);
-                    else m = min(128 * p + row[i], A.W.M - 1);               // past the end: nobody reads the results
-                    cp[i] = A.W.codes + mx_code_row(m, A.W.groups) + t * 16;
-                    sp[i] = A.W.scales + mx_scale_row(m, A.W.groups);
-                }
-            };
-            uint4 q[2];
-            uint32_t s[2];
-            auto load = [&](int g) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    q[i] = __ldg(reinterpret_cast<const uint4 *>(cp[i] + static_cast<int64_t>(g) * kMxTileCodes));
-                    s[i] = __ldg(reinterpret_cast<const uint32_t *>(sp[i] + static_cast<int64_t>(g) * kMxTileScales));
-                }
-            };
-            if (static_cast<int>(blockIdx.x) < tiles) {
-                rows_of(blockIdx.x % A.tiles_p);
-                load(0);
-            }
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                for (int c = 0; c < A.stages_c; c += 2) {
-                    const uint4 now[2] = {q[0], q[1]};
-                    const uint32_t sc[2] = {s[0], s[1]};
-                    if (c + 2 < A.stages_c) {
-                        load((c + 2) >> 1);
-                    } else if (tile + static_cast<int>(gridDim.x) < tiles) {
-                        rows_of((tile + gridDim.x) % A.tiles_p);
-                        load(0);
-                    }
-                    const bool large = ((sc[0] | sc[1]) & 0x80808080u) != 0u;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        if (c + h >= A.stages_c) break;
-                        begin();
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            uint8_t *dst = smem + slot * stage_bytes + row[i] * 128;
-#pragma unroll
-                            for (int j = 0; j < 2; j++) {
-                                const uint32_t word = h == 0 ? (j == 0 ? now[i].x : now[i].y) : (j == 0 ? now[i].z : now[i].w);
-                                *reinterpret_cast<uint4 *>(dst + (((j * 4 + t) ^ (row[i] & 7)) << 4)) = mx_word_to_bf16(word, (sc[i] >> (8 * (2 * h + j))) & 255u, large);
-                            }
-                        }
-                        end();
-                    }
-                }
-            }
-        }
-    } else if (warp >= kMtEpilogue) {
-        // ---- sums to outputs: this thread's lane of the accumulator is value p, columns are rows of out ---------------------------------
-        const int quarter = warp & 3, lane_p = quarter * 32 + lane;
-        float *swap = reinterpret_cast<float *>(smem + A.stages * stage_bytes);
-        int buf = 0;
-        uint32_t buf_phase = 0u;
-        pdl_wait();                                                          // outputs may be what the previous kernel reads, a bias what it writes
+        // 32-bit sums, both operands BF16, A MN-major, B K-major
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
+        int slot = 0, buf = 0;
+        uint32_t phase = 0u, buf_phase = 1u;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            const int p = tile % A.tiles_p, n0 = tile / A.tiles_p * A.nt, cols = min(A.nt, A.rows - n0);
-            constexpr bool gated = kKind == kMxGatedPair;
-            const int m = gated ? 64 * p + (lane_p & 63) : 128 * p + lane_p;
-            const bool up = gated && lane_p >= 64, live = m < A.outs;
-            float bias = 0.f;
-            if (A.bias != nullptr && live) bias = __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m + (up ? A.outs : 0))) << 16);
-            mt_wait(done + 8 * buf, buf_phase, &dead, 24);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t from = tmem + buf * 256 + (static_cast<uint32_t>(quarter) << 21);
-            for (int c = 0; c < cols; c += 32) {
-                uint32_t r[32];
-                asm volatile(
-                    "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                    "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                      "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-                      "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                    : "r"(from + c));
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (c + 32 >= cols) {                                        // the accumulator is read: the issuer may have it back
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(free_ + 8 * buf);
+            mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
+            mt_fence_after();
+            for (int c = 0; c < A.stages_c; c++) {
+                mx_wait(full + 8 * slot, phase, &dead, 22);
+                mt_fence_after();
+                if (mt_elect()) {
+                    const uint32_t d = tmem + buf * kMtGradRows;
+                    const uint64_t a = mt_desc(base + slot * stage_bytes, 512), b = mt_desc(base + slot * stage_bytes + kMtABytes, 1);
+#pragma unroll
+                    for (int k = 0; k < kMtStage / 16; k++) mt_mma(d, a + 128 * k, b + 2 * k, idesc, c > 0 || k > 0);
+                    mt_commit(empty + 8 * slot);
+                    if (c + 1 == A.stages_c) mt_commit(done + 8 * buf);
                 }
-                if constexpr (!gated) {
-                    if (live) {
-                        uint16_t *to = A.out + static_cast<int64_t>(n0 + c) * A.outs + m;
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (c + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(__uint_as_float(r[i]) + bias);
-                    }
-                } else {
-                    float v[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]) + bias;
-                    if (A.pre != nullptr && live) {
-                        float *to = A.pre + static_cast<int64_t>(n0 + c) * 2 * A.outs + m + (up ? A.outs : 0);
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (c + i < cols) to[static_cast<int64_t>(i) * 2 * A.outs] = v[i];
-                    }
-                    // columns 0 .. 15 become the gate lanes', 16 .. 31 the up lanes': each hands the other half over
-#pragma unroll
-                    for (int i = 0; i < 16; i++) swap[((up ? 0 : 16) + i) * 64 + (lane_p & 63)] = up ? v[i] : v[16 + i];
-                    asm volatile("bar.sync 2, 128;" ::: "memory");
-                    if (live) {
-                        const int i0 = up ? 16 : 0;
-                        uint16_t *to = A.out + static_cast<int64_t>(n0 + c + i0) * A.outs + m;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float other = swap[(i0 + i) * 64 + (lane_p & 63)];
-                            const float g = up ? other : v[i], u = up ? v[16 + i] : other;
-                            if (c + i0 + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(mx_act(A.activation, g) * u);
-                        }
-                    }
-                    asm volatile("bar.sync 2, 128;" ::: "memory");
-                }
+                __syncwarp();
+                if (++slot == A.stages) slot = 0, phase ^= 1u;
             }
             if ((buf ^= 1) == 0) buf_phase ^= 1u;
         }
+    } else if (warp >= kMtConverter) {
+        const int team = (warp - kMtConverter) / kMtTeam, t = lane & 3;
+        const int row = ((warp - kMtConverter) & (kMtTeam - 1)) * 8 + ((lane >> 3) | (lane & 4));      // rows 0, 4, 1, 5, 2, 6, 3, 7
+        const uint32_t to = (row >> 3) * 1024 + (row & 7) * 128;
+        const int storage_tiles = (A.W.M + 15) >> 4;
+        int tile = blockIdx.x, c = team, slot = team;
+        uint32_t phase = 1u;
+        uint4 q;
+        uint32_t s;
+        auto settle = [&]() {
+            while (c >= A.stages_c && tile < tiles) c -= A.stages_c, tile += gridDim.x;
+        };
+        auto load = [&]() {
+            const int from = 4 * c + (row >> 4);
+            q = make_uint4(0u, 0u, 0u, 0u);
+            s = 0u;
+            if (tile < tiles && from < storage_tiles) {
+                const int64_t at = static_cast<int64_t>(from) * A.W.groups + tile % A.tiles_p;
+                q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16));
+                s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
+            }
+        };
+        settle();
+        load();
+        while (tile < tiles) {
+            uint4 v[4];
+            const bool large = (s & 0x80808080u) != 0u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = mx_word_to_bf16(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, (s >> (8 * j)) & 255u, large);
+            c += 2;
+            settle();
+            load();
+            mx_wait(empty + 8 * slot, phase, &dead, 23);
+            uint8_t *dst = smem + slot * stage_bytes + to;
+#pragma unroll
+            for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(dst + (j >> 1) * 8192 + ((((j & 1) * 4 + t) ^ (row & 7)) << 4)) = v[j];
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * slot);
+            if ((slot += 2) >= A.stages) slot = team, phase ^= 1u;
+        }
+    } else if (warp >= kMtEpilogue) {
+        mt_epilogue<false, kMtGradRows>(A, tmem, done, free_, nullptr, &dead, warp, lane);
     }
-
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (dead)                                                                // copies and products under way land before the memory goes
-        for (int i = 0; i < 10; i++) __nanosleep(100000);
-    __syncthreads();
-    if (warp == kMtIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    mt_end(tmem, &dead, warp);
 }
 
 }  // namespace bhi

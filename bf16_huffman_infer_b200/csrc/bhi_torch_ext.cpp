@@ -14,7 +14,6 @@
 
 #include <optional>
 #include <string>
-#include <utility>
 #include <vector>
 
 #include "../../include/bf16_huffman_b200.h"
@@ -684,14 +683,15 @@ int int_of(int64_t v, const char *name) {
 }
 
 MxView mx_of(const Tensor &codes, const Tensor &scales, int64_t M, int64_t K) {
-    want(codes, ScalarType::Byte, "codes", 4);
+    want(codes, ScalarType::Byte, "codes", 5);
     want(scales, ScalarType::Byte, "scales", 4);
     same_device(codes, scales, "scales");
     STD_TORCH_CHECK(M >= 1 && K >= 32 && K % 32 == 0 && M <= BHI_MXFP4_MAX_DIM && K <= BHI_MXFP4_MAX_DIM, "a weight has rows and a multiple of 32 columns");
     const int64_t tiles = (M + 15) / 16, groups = (K + 127) / 128;
-    for (const auto &[t, last] : {std::pair<const Tensor &, int64_t>(codes, 64), std::pair<const Tensor &, int64_t>(scales, 4)})
-        STD_TORCH_CHECK(t.dim() == 4 && t.size(0) == tiles && t.size(1) == groups && t.size(2) == 16 && t.size(3) == last,
-                        "codes must be [ceil(M/16), ceil(K/128), 16, 64], scales [ceil(M/16), ceil(K/128), 16, 4]");
+    STD_TORCH_CHECK(codes.dim() == 5 && codes.size(0) == tiles && codes.size(1) == groups && codes.size(2) == 4 && codes.size(3) == 16 && codes.size(4) == 16,
+                    "codes must be [ceil(M/16), ceil(K/128), 4, 16, 16]");
+    STD_TORCH_CHECK(scales.dim() == 4 && scales.size(0) == tiles && scales.size(1) == groups && scales.size(2) == 16 && scales.size(3) == 4,
+                    "scales must be [ceil(M/16), ceil(K/128), 16, 4]");
     return {ptr<const uint8_t>(codes), ptr<const uint8_t>(scales), static_cast<int>(M), static_cast<int>(K)};
 }
 

@@ -410,3 +410,23 @@ def test_results_are_whole_for_the_next_kernel(pkg):
         z = F.linear(z, ws[i % 3])
         torch.cuda.synchronize()
     assert torch.equal(y, z)
+
+
+def test_first_call_of_a_thread(pkg):
+    """A thread that has made no CUDA call of its own yet, as those of the autograd engine, on the tiled products."""
+    import threading
+    w, _ = made(pkg, 96, 256)
+    x, dy = normal(64, 256), normal(64, 96)
+    want = F.linear(x, w), pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, 96, 256)
+    got, calls = {}, {
+        "y": lambda: pkg.ops.forward_mxfp4(x, w.codes, w.scales, 96, None),
+        "dx": lambda: pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, 96, 256),
+    }
+    for name, call in calls.items():
+        def run(name=name, call=call):
+            got[name] = call()
+            torch.cuda.current_stream().synchronize()
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+    assert torch.equal(got["y"], want[0]) and torch.equal(got["dx"], want[1])
