@@ -1,4 +1,5 @@
 // The products of 4-bit microscaled weights in tiles: plans and launches.
+#include <cstdlib>
 #include "bhi_mxfp4_tile.cuh"
 
 namespace bhi {
@@ -49,16 +50,17 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     const int per = kKind == kGatedPair ? 64 : 128;
     a.tiles_p = (a.outs + per - 1) / per;
     a.nt = rows_of_tile(a.rows, a.tiles_p, kKind == kGradient ? kMtGradRows : kMtForwardRows);
+    if (getenv("MXN")) a.nt = atoi(getenv("MXN"));
     a.tiles_n = (a.rows + a.nt - 1) / a.nt;
-    a.stages_c = static_cast<int>((b_cols + kMtStage - 1) / kMtStage);
+    a.boxes_c = static_cast<int>((b_cols + kMtBox - 1) / kMtBox);
     BHI_REQUIRE(static_cast<int64_t>(a.tiles_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
-    const uint32_t stage = (kKind == kGradient ? kMtABytes : 0u) + static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;
+    const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 128u : static_cast<uint32_t>(a.nt) * 256u, extra = kKind == kGatedPair ? kMtSwap : 0u;
     a.stages = static_cast<int>((kSmemTile - extra) / stage);
     if (a.stages > kMtStagesMax) a.stages = kMtStagesMax;
-    a.stages &= ~1;
+    if (kKind == kGradient) a.stages &= ~1;          // a slot is always the same team's
     alignas(64) CUtensorMap map;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(b_cols), static_cast<cuuint64_t>(a.rows)}, strides[1] = {static_cast<cuuint64_t>(ldb) * 2};
-    const cuuint32_t box[2] = {kMtStage, static_cast<cuuint32_t>(a.nt)}, estr[2] = {1, 1};
+    const cuuint32_t box[2] = {kMtBox, static_cast<cuuint32_t>(a.nt)}, estr[2] = {1, 1};
     const auto encoded = [&]() {
         return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(B), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

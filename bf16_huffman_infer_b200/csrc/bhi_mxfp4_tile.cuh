@@ -21,8 +21,8 @@ namespace bhi {
 constexpr int kMtLoader = 0, kMtIssuer = 1, kMtEpilogue = 4, kMtConverter = 8;      // warps; 2 and 3 idle
 constexpr int kMtTeam = 8;                        // warps of a team of converters; two teams
 constexpr int kMtThreads = 32 * (kMtConverter + 2 * kMtTeam);
-constexpr int kMtStage = 64;                      // values of c
-constexpr uint32_t kMtABytes = 128 * kMtStage * 2;
+constexpr int kMtBox = 64;                        // values of c a TMA box
+constexpr uint32_t kMtABytes = 128 * kMtBox * 2;
 constexpr int kMtStagesMax = 16;
 constexpr uint32_t kMtSwap = 16 * 64 * 4;         // bytes through which a gated block changes lanes
 constexpr int kMtForwardRows = 192, kMtGradRows = 256;       // most rows of a tile
@@ -34,7 +34,7 @@ struct MxTileArgs {
     float *pre;                                   // gated, or null
     int rows, outs;                               // of out
     int activation;
-    int nt, tiles_p, tiles_n, stages_c;           // rows of a tile, tiles, stages of a tile
+    int nt, tiles_p, tiles_n, boxes_c;            // rows of a tile, tiles, boxes of a tile
     int stages;                                   // of the ring
 };
 
@@ -66,6 +66,12 @@ __device__ __forceinline__ void mt_load(uint32_t from, float (&v)[N]) {
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
                    "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
                  : "r"(from));
+}
+// Whether a phase is over, without waiting: asked for the next stage before this one's products are issued, so that the answer costs no time.
+__device__ __forceinline__ uint32_t mt_over(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
 }
 // One lane of a converged warp.  The issuing warp runs its loop as a whole and elects a lane for the products alone: operands that the
 // compiler knows to be the same in all lanes stay in uniform registers.
@@ -173,17 +179,20 @@ __device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, 
     }
 }
 
-// ---- B: 64 values of c of a tile's rows a stage --------------------------------------------------------------------------------------
+// ---- B: a stage is kBoxes times 64 values of c of a tile's rows ---------------------------------------------------------------------------
+template <int kBoxes>
 __device__ __forceinline__ void mt_loader(const MxTileArgs &A, const CUtensorMap *map, uint32_t base, uint32_t stage_bytes, uint32_t full, uint32_t empty, int *dead) {
+    const uint32_t box = static_cast<uint32_t>(A.nt) * 128u;
     pdl_wait();
     int slot = 0;
     uint32_t phase = 1u;
     for (int tile = blockIdx.x; tile < A.tiles_p * A.tiles_n; tile += gridDim.x) {
         const int n0 = tile / A.tiles_p * A.nt;
-        for (int c = 0; c < A.stages_c; c++) {
+        for (int c = 0; c < A.boxes_c; c += kBoxes) {
+            const int boxes = min(kBoxes, A.boxes_c - c);
             mx_wait(empty + 8 * slot, phase, dead, 20);
-            mbar_expect_tx(full + 8 * slot, static_cast<uint32_t>(A.nt) * 128u);
-            mt_tma_2d(base + slot * stage_bytes, map, c * kMtStage, n0, full + 8 * slot);
+            mbar_expect_tx(full + 8 * slot, boxes * box);
+            for (int i = 0; i < boxes; i++) mt_tma_2d(base + slot * stage_bytes + i * box, map, (c + i) * kMtBox, n0, full + 8 * slot);
             if (++slot == A.stages) slot = 0, phase ^= 1u;
         }
     }
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
     __shared__ uint32_t tmem_slot;
     __shared__ int dead;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t base = smem_addr(smem), stage_bytes = static_cast<uint32_t>(A.nt) * 128u;
+    const uint32_t base = smem_addr(smem), box = static_cast<uint32_t>(A.nt) * 128u, stage_bytes = 2 * box;
     const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16,
                    a_full = done + 32, a_empty = done + 48;
     const int tiles = A.tiles_p * A.tiles_n, groups = A.W.groups;
@@ -243,32 +252,38 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
     const uint32_t tmem = mt_begin(&tmem_slot, warp);
 
     if (warp == kMtLoader) {
-        if (lane == 0) mt_loader(A, &bmap, base, stage_bytes, full, empty, &dead);
+        if (lane == 0) mt_loader<2>(A, &bmap, base, stage_bytes, full, empty, &dead);
     } else if (warp == kMtIssuer) {
         // 32-bit sums, both operands BF16 and K-major
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
         int slot = 0, buf = 0, place = 0;
         uint32_t phase = 0u, buf_phase = 1u, a_phase = 0u;
+        uint32_t b_ok = 0u, a_ok = 0u;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
             mt_fence_after();
-            for (int c = 0; c < A.stages_c; c++) {
-                if ((c & 1) == 0) mx_wait(a_full + 8 * place, a_phase, &dead, 25);
-                mx_wait(full + 8 * slot, phase, &dead, 22);
+            for (int g = 0; g < groups; g++) {
+                if (!a_ok) mx_wait(a_full + 8 * place, a_phase, &dead, 25);
+                if (!b_ok) mx_wait(full + 8 * slot, phase, &dead, 22);
                 mt_fence_after();
-                const bool last_of_group = (c & 1) || c + 1 == A.stages_c;
+                const uint32_t a = tmem + 2 * kMtForwardRows + place * 64, d = tmem + buf * kMtForwardRows, used = slot, from = place;
+                const uint64_t b = mt_desc(base + slot * stage_bytes, 1);
+                if (++slot == A.stages) slot = 0, phase ^= 1u;
+                if ((place ^= 1) == 0) a_phase ^= 1u;
+                a_ok = mt_over(a_full + 8 * place, a_phase);
+                b_ok = mt_over(full + 8 * slot, phase);
                 if (mt_elect()) {
-                    const uint32_t a = tmem + 2 * kMtForwardRows + place * 64 + (c & 1) * 32, d = tmem + buf * kMtForwardRows;
-                    const uint64_t b = mt_desc(base + slot * stage_bytes, 1);
 #pragma unroll
-                    for (int k = 0; k < kMtStage / 16; k++) mt_mma_ta(d, a + k * 8, b + 2 * k, idesc, c > 0 || k > 0);
-                    mt_commit(empty + 8 * slot);
-                    if (last_of_group) mt_commit(a_empty + 8 * place);
-                    if (c + 1 == A.stages_c) mt_commit(done + 8 * buf);
+                    for (int k = 0; k < 4; k++) mt_mma_ta(d, a + k * 8, b + 2 * k, idesc, g > 0 || k > 0);
+                    if (2 * g + 1 < A.boxes_c) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) mt_mma_ta(d, a + 32 + k * 8, b + (box >> 4) + 2 * k, idesc, 1u);
+                    }
+                    mt_commit(empty + 8 * used);
+                    mt_commit(a_empty + 8 * from);
+                    if (g + 1 == groups) mt_commit(done + 8 * buf);
                 }
                 __syncwarp();
-                if (++slot == A.stages) slot = 0, phase ^= 1u;
-                if (last_of_group && (place ^= 1) == 0) a_phase ^= 1u;
             }
             if ((buf ^= 1) == 0) buf_phase ^= 1u;
         }
@@ -360,28 +375,29 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
     const uint32_t tmem = mt_begin(&tmem_slot, warp);
 
     if (warp == kMtLoader) {
-        if (lane == 0) mt_loader(A, &bmap, base + kMtABytes, stage_bytes, full, empty, &dead);
+        if (lane == 0) mt_loader<1>(A, &bmap, base + kMtABytes, stage_bytes, full, empty, &dead);
     } else if (warp == kMtIssuer) {
         // 32-bit sums, both operands BF16, A MN-major, B K-major
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
         int slot = 0, buf = 0;
-        uint32_t phase = 0u, buf_phase = 1u;
+        uint32_t phase = 0u, buf_phase = 1u, ok = 0u;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
             mt_fence_after();
-            for (int c = 0; c < A.stages_c; c++) {
-                mx_wait(full + 8 * slot, phase, &dead, 22);
+            for (int c = 0; c < A.boxes_c; c++) {
+                if (!ok) mx_wait(full + 8 * slot, phase, &dead, 22);
                 mt_fence_after();
+                const uint32_t d = tmem + buf * kMtGradRows, used = slot;
+                const uint64_t a = mt_desc(base + slot * stage_bytes, 512), b = mt_desc(base + slot * stage_bytes + kMtABytes, 1);
+                if (++slot == A.stages) slot = 0, phase ^= 1u;
+                ok = mt_over(full + 8 * slot, phase);
                 if (mt_elect()) {
-                    const uint32_t d = tmem + buf * kMtGradRows;
-                    const uint64_t a = mt_desc(base + slot * stage_bytes, 512), b = mt_desc(base + slot * stage_bytes + kMtABytes, 1);
 #pragma unroll
-                    for (int k = 0; k < kMtStage / 16; k++) mt_mma(d, a + 128 * k, b + 2 * k, idesc, c > 0 || k > 0);
-                    mt_commit(empty + 8 * slot);
-                    if (c + 1 == A.stages_c) mt_commit(done + 8 * buf);
+                    for (int k = 0; k < kMtBox / 16; k++) mt_mma(d, a + 128 * k, b + 2 * k, idesc, c > 0 || k > 0);
+                    mt_commit(empty + 8 * used);
+                    if (c + 1 == A.boxes_c) mt_commit(done + 8 * buf);
                 }
                 __syncwarp();
-                if (++slot == A.stages) slot = 0, phase ^= 1u;
             }
             if ((buf ^= 1) == 0) buf_phase ^= 1u;
         }
@@ -392,31 +408,37 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
         const int storage_tiles = (A.W.M + 15) >> 4;
         int tile = blockIdx.x, c = team, slot = team;
         uint32_t phase = 1u;
-        uint4 q;
-        uint32_t s;
-        auto settle = [&]() {
-            while (c >= A.stages_c && tile < tiles) c -= A.stages_c, tile += gridDim.x;
-        };
-        auto load = [&]() {
-            const int from = 4 * c + (row >> 4);
-            q = make_uint4(0u, 0u, 0u, 0u);
-            s = 0u;
-            if (tile < tiles && from < storage_tiles) {
-                const int64_t at = static_cast<int64_t>(from) * A.W.groups + tile % A.tiles_p;
-                q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16));
-                s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
+        // units are loaded two stages of the team ahead of their use
+        uint4 q, q_next;
+        uint32_t s, s_next;
+        int ask_tile = tile, ask_c = c;
+        auto load = [&](uint4 &to_q, uint32_t &to_s) {
+            while (ask_c >= A.boxes_c && ask_tile < tiles) ask_c -= A.boxes_c, ask_tile += gridDim.x;
+            const int from = 4 * ask_c + (row >> 4);
+            to_q = make_uint4(0u, 0u, 0u, 0u);
+            to_s = 0u;
+            if (ask_tile < tiles && from < storage_tiles) {
+                const int64_t at = static_cast<int64_t>(from) * A.W.groups + ask_tile % A.tiles_p;
+                to_q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16));
+                to_s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
             }
+            ask_c += 2;
+        };
+        auto settle = [&]() {
+            while (c >= A.boxes_c && tile < tiles) c -= A.boxes_c, tile += gridDim.x;
         };
         settle();
-        load();
+        load(q, s);
+        load(q_next, s_next);
         while (tile < tiles) {
             uint4 v[4];
             const bool large = (s & 0x80808080u) != 0u;
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] = mx_word_to_bf16(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, (s >> (8 * j)) & 255u, large);
+            q = q_next, s = s_next;
+            load(q_next, s_next);
             c += 2;
             settle();
-            load();
             mx_wait(empty + 8 * slot, phase, &dead, 23);
             uint8_t *dst = smem + slot * stage_bytes + to;
 #pragma unroll
