@@ -25,15 +25,15 @@ EncodeTiledFn encode_tiled() {
 
 enum Kind { kPlain, kGatedPair, kGradient };
 
-// Rows of a tile (a multiple of 16, at most `most`): the fewest rounds of tiles over the SMs times a tile's cost, which is its rows where the
-// tensor cores bound it and that of kExpand rows where the expansion of the weight does.
+// Rows of a tile (a multiple of 32, at most `most`): the fewest rounds of tiles over the pairs of SMs times a tile's cost, which is its rows where
+// the tensor cores bound it and that of kExpand rows where the expansion of the weight does.
 constexpr int kExpand = 128;
-int rows_of_tile(int rows, int tiles_p, int most) {
-    int best = 16;
+int rows_of_tile(int rows, int pairs_p, int most) {
+    int best = 32;
     double best_cost = 1e30;
-    for (int nt = 16; nt <= most; nt += 16) {
-        const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * tiles_p;
-        const double cost = static_cast<double>((tiles + sm_count() - 1) / sm_count()) * (nt > kExpand ? nt : kExpand) + 1e-3 * nt;
+    for (int nt = 32; nt <= most; nt += 32) {
+        const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p, pairs = sm_count() / 2;
+        const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * (nt > kExpand ? nt : kExpand) + 1e-3 * nt;
         if (cost < best_cost - 1e-9) {
             best_cost = cost;
             best = nt;
@@ -48,19 +48,19 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     EncodeTiledFn encode = encode_tiled();
     if (!encode) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     const int per = kKind == kGatedPair ? 64 : 128;
-    a.tiles_p = (a.outs + per - 1) / per;
-    a.nt = rows_of_tile(a.rows, a.tiles_p, kKind == kGradient ? kMtGradRows : kMtForwardRows);
+    a.pairs_p = (a.outs + 2 * per - 1) / (2 * per);
+    a.nt = rows_of_tile(a.rows, a.pairs_p, kKind == kGradient ? kMtGradRows : kMtForwardRows);
     if (getenv("MXN")) a.nt = atoi(getenv("MXN"));
     a.tiles_n = (a.rows + a.nt - 1) / a.nt;
     a.boxes_c = static_cast<int>((b_cols + kMtBox - 1) / kMtBox);
-    BHI_REQUIRE(static_cast<int64_t>(a.tiles_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
-    const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 128u : static_cast<uint32_t>(a.nt) * 256u, extra = kKind == kGatedPair ? kMtSwap : 0u;
+    BHI_REQUIRE(static_cast<int64_t>(a.pairs_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
+    const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 64u : static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;
     a.stages = static_cast<int>((kSmemTile - extra) / stage);
     if (a.stages > kMtStagesMax) a.stages = kMtStagesMax;
     if (kKind == kGradient) a.stages &= ~1;          // a slot is always the same team's
     alignas(64) CUtensorMap map;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(b_cols), static_cast<cuuint64_t>(a.rows)}, strides[1] = {static_cast<cuuint64_t>(ldb) * 2};
-    const cuuint32_t box[2] = {kMtBox, static_cast<cuuint32_t>(a.nt)}, estr[2] = {1, 1};
+    const cuuint32_t box[2] = {kMtBox, static_cast<cuuint32_t>(a.nt / 2)}, estr[2] = {1, 1};
     const auto encoded = [&]() {
         return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(B), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -73,17 +73,21 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     if (cr != CUDA_SUCCESS) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(cr)));
     auto kernel = kKind == kGradient ? mx_grad_kernel : mx_tile_kernel<kKind == kGatedPair>;
     if (int rc = staged_prepare(kernel, kSmemTile)) return rc;
-    const int tiles = a.tiles_p * a.tiles_n;
+    const int tiles = a.pairs_p * a.tiles_n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles < sm_count() ? tiles : sm_count());
+    const int pairs = sm_count() / 2;
+    cfg.gridDim = dim3(2 * (tiles < pairs ? tiles : pairs));
     cfg.blockDim = dim3(kMtThreads);
     cfg.dynamicSmemBytes = a.stages * stage + extra;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_launches() ? 1 : 0;
+    cfg.numAttrs = overlap_launches() ? 2 : 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, map);
     return e == cudaSuccess ? BHI_OK : cuda_fail(e, "4-bit tiled product launch");
 }

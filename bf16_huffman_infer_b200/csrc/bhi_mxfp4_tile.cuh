@@ -2,10 +2,13 @@
 //
 //   out[n][p] = sum over c of B[n][c] A(p, c)      forward: p a weight row m, c a column k, B = X;  gradient: p a column k, c a weight row m, B = dY
 //
-// A tile is 128 values of p (the lanes of an accumulator) by NT rows of B (its columns).  Sixteen warps turn codes into BF16, exactly (a code
-// times a power of two fits), one thread requests B by TMA, 64 values of c at a time, one issues the products, four warps read the accumulators
-// back, two of which alternate between tiles.  The weight is expanded once for all rows of a tile, so the expansion (19 instructions
-// for eight values) stays behind the tensor cores from some 130 rows on.
+// Two CTAs of a cluster, on a pair of SMs, share a tile of 256 values of p (each has 128, the lanes of its accumulator) by NT rows of B (the
+// accumulator's columns), of which each brings half into its shared memory: the pair's tensor cores read both halves (cta_group::2).  On
+// its own an SM would write and read all of B, 96 KB of shared memory for 192 rows and 128 values of c, 750 clocks at 128 bytes a clock, where
+// the products take 768: together with everything else that made 1030.
+// Sixteen warps of a CTA turn codes into BF16, exactly (a code times a power of two fits), one thread requests B by TMA, one of the pair issues the
+// products, four warps read the accumulators back, two of which alternate between tiles.  The weight is expanded once for all rows of a
+// tile, so the expansion (19 instructions for eight values) stays behind the tensor cores from some 130 rows on.
 //
 // A code's bits s eem are moved to a BF16's sign, lowest exponent and highest mantissa bits: that is its value times 2^-126, the
 // subnormal code 0.5 included, and one product by 2^(126 + s - 127) makes both the value and its scale.  Scales above 2 (2^(126 + s - 127) would
@@ -34,25 +37,31 @@ struct MxTileArgs {
     float *pre;                                   // gated, or null
     int rows, outs;                               // of out
     int activation;
-    int nt, tiles_p, tiles_n, boxes_c;            // rows of a tile, tiles, boxes of a tile
+    int nt, pairs_p, tiles_n, boxes_c;            // rows of a tile (a multiple of 32), pairs of tiles along p, tiles along n, boxes of 64 values of c
     int stages;                                   // of the ring
 };
 
+// a box into this CTA's shared memory; its bytes count at the barrier of this place in the CTA that issues the products (`bar`, by mt_leader)
 __device__ __forceinline__ void mt_tma_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t mt_leader(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
 }
 __device__ __forceinline__ void mt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // the same with A in tensor memory: lanes are rows, a column holds two neighbours along K
 __device__ __forceinline__ void mt_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void mt_store8(uint32_t to, const uint4 &a, const uint4 &b) {
@@ -82,8 +91,19 @@ __device__ __forceinline__ bool mt_elect() {
 }
 __device__ __forceinline__ void mt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// arrives at the barriers of this place in both CTAs when the products issued so far are done
 __device__ __forceinline__ void mt_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// arrives at the barrier of this place in the CTA that issues the products.  What is signalled lies in this CTA's own shared or tensor memory and
+// has been fenced there; a release at cluster scope would wait for every copy under way (it made the gradient three times as long).
+__device__ __forceinline__ void mt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mt_leader(bar)) : "memory"); }
+// of this CTA in its cluster of two; by the block's number, which the compiler knows to be the same in all lanes
+__device__ __forceinline__ uint32_t mt_rank() { return blockIdx.x & 1u; }
+__device__ __forceinline__ void mt_cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 128-byte swizzle, 8-row groups (K-major) or 8-column groups (MN-major) 1024 bytes apart; lbo in 16-byte units
 __device__ __forceinline__ uint64_t mt_desc(uint32_t addr, uint32_t lbo) {
@@ -120,13 +140,13 @@ __device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t s, bool la
 // kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16 columns the first eight become the gate lanes', the
 // others the up lanes': each hands the other half over through shared memory.
 template <bool kGated, int kBuffer>
-__device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, uint32_t done, uint32_t free_, float *swap, int *dead, int warp, int lane) {
-    const int quarter = warp & 3, lane_p = quarter * 32 + lane, tiles = A.tiles_p * A.tiles_n;
+__device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, uint32_t done, uint32_t free_, float *swap, int *dead, int warp, int lane, uint32_t rank) {
+    const int quarter = warp & 3, lane_p = quarter * 32 + lane, tiles = A.pairs_p * A.tiles_n, step = gridDim.x / 2;
     int buf = 0;
     uint32_t phase = 0u;
     pdl_wait();                                                              // outputs may be what the previous kernel reads, a bias what it writes
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int p = tile % A.tiles_p, n0 = tile / A.tiles_p * A.nt, cols = min(A.nt, A.rows - n0);
+    for (int tile = blockIdx.x / 2; tile < tiles; tile += step) {
+        const int p = 2 * (tile % A.pairs_p) + rank, n0 = tile / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0);
         const int m = kGated ? 64 * p + (lane_p & 63) : 128 * p + lane_p;
         const bool up = kGated && lane_p >= 64, live = m < A.outs;
         float bias = 0.f;
@@ -141,7 +161,7 @@ __device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, 
             if (c + 16 >= cols) {                                            // the accumulator is read: the issuer may have it back
                 mt_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(free_ + 8 * buf);
+                if (lane == 0) mt_arrive(free_ + 8 * buf);
             }
 #pragma unroll
             for (int i = 0; i < 16; i++) v[i] += bias;
@@ -179,20 +199,21 @@ __device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, 
     }
 }
 
-// ---- B: a stage is kBoxes times 64 values of c of a tile's rows ---------------------------------------------------------------------------
+// ---- B: a stage is kBoxes times 64 values of c of this CTA's half of a tile's rows ----------------------------------------------------------
 template <int kBoxes>
-__device__ __forceinline__ void mt_loader(const MxTileArgs &A, const CUtensorMap *map, uint32_t base, uint32_t stage_bytes, uint32_t full, uint32_t empty, int *dead) {
-    const uint32_t box = static_cast<uint32_t>(A.nt) * 128u;
+__device__ __forceinline__ void mt_loader(const MxTileArgs &A, const CUtensorMap *map, uint32_t base, uint32_t stage_bytes, uint32_t full, uint32_t empty, int *dead,
+                                          uint32_t rank) {
+    const uint32_t box = static_cast<uint32_t>(A.nt) * 64u;
     pdl_wait();
     int slot = 0;
     uint32_t phase = 1u;
-    for (int tile = blockIdx.x; tile < A.tiles_p * A.tiles_n; tile += gridDim.x) {
-        const int n0 = tile / A.tiles_p * A.nt;
+    for (int tile = blockIdx.x / 2; tile < A.pairs_p * A.tiles_n; tile += gridDim.x / 2) {
+        const int n0 = tile / A.pairs_p * A.nt + static_cast<int>(rank) * (A.nt / 2);
         for (int c = 0; c < A.boxes_c; c += kBoxes) {
             const int boxes = min(kBoxes, A.boxes_c - c);
             mx_wait(empty + 8 * slot, phase, dead, 20);
-            mbar_expect_tx(full + 8 * slot, boxes * box);
-            for (int i = 0; i < boxes; i++) mt_tma_2d(base + slot * stage_bytes + i * box, map, (c + i) * kMtBox, n0, full + 8 * slot);
+            if (rank == 0) mbar_expect_tx(full + 8 * slot, 2 * boxes * box);         // both CTAs' halves
+            for (int i = 0; i < boxes; i++) mt_tma_2d(base + slot * stage_bytes + i * box, map, (c + i) * kMtBox, n0, mt_leader(full + 8 * slot));
             if (++slot == A.stages) slot = 0, phase ^= 1u;
         }
     }
@@ -200,21 +221,21 @@ __device__ __forceinline__ void mt_loader(const MxTileArgs &A, const CUtensorMap
 
 __device__ __forceinline__ uint32_t mt_begin(uint32_t *tmem_slot, int warp) {        // every thread; after the barriers are initialised
     if (warp == kMtIssuer) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     mt_fence_before();
-    __syncthreads();
+    mt_cluster_sync();                                                       // the other CTA's barriers are ready too
     mt_fence_after();
     return __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
 }
 __device__ __forceinline__ void mt_end(uint32_t tmem, const int *dead, int warp) {
     mt_fence_before();
-    __syncthreads();
+    mt_cluster_sync();                                                       // nobody arrives here or reads this CTA's half any more
     if (*dead)                                                               // copies and products under way land before the memory goes
         for (int i = 0; i < 10; i++) __nanosleep(100000);
-    __syncthreads();
-    if (warp == kMtIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    mt_cluster_sync();
+    if (warp == kMtIssuer) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ---- forward: A in tensor memory ------------------------------------------------------------------------------------------------------
@@ -229,10 +250,11 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
     __shared__ uint32_t tmem_slot;
     __shared__ int dead;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t base = smem_addr(smem), box = static_cast<uint32_t>(A.nt) * 128u, stage_bytes = 2 * box;
+    const uint32_t base = smem_addr(smem), box = static_cast<uint32_t>(A.nt) * 64u, stage_bytes = 2 * box;
     const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16,
                    a_full = done + 32, a_empty = done + 48;
-    const int tiles = A.tiles_p * A.tiles_n, groups = A.W.groups;
+    const int tiles = A.pairs_p * A.tiles_n, groups = A.W.groups, step = gridDim.x / 2;
+    const uint32_t rank = mt_rank();
 
     pdl_launch_dependents();
     if (tid == 0) {
@@ -242,8 +264,8 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(done + 8 * i, 1);
-            mbar_init(free_ + 8 * i, 4);
-            mbar_init(a_full + 8 * i, kMtTeam);
+            mbar_init(free_ + 8 * i, 8);
+            mbar_init(a_full + 8 * i, 2 * kMtTeam);
             mbar_init(a_empty + 8 * i, 1);
         }
         mbar_fence_init();
@@ -252,14 +274,14 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
     const uint32_t tmem = mt_begin(&tmem_slot, warp);
 
     if (warp == kMtLoader) {
-        if (lane == 0) mt_loader<2>(A, &bmap, base, stage_bytes, full, empty, &dead);
-    } else if (warp == kMtIssuer) {
+        if (lane == 0) mt_loader<2>(A, &bmap, base, stage_bytes, full, empty, &dead, rank);
+    } else if (warp == kMtIssuer && rank == 0) {
         // 32-bit sums, both operands BF16 and K-major
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (16u << 24);
         int slot = 0, buf = 0, place = 0;
         uint32_t phase = 0u, buf_phase = 1u, a_phase = 0u;
         uint32_t b_ok = 0u, a_ok = 0u;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        for (int tile = blockIdx.x / 2; tile < tiles; tile += step) {
             mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
             mt_fence_after();
             for (int g = 0; g < groups; g++) {
@@ -290,16 +312,16 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
     } else if (warp >= kMtConverter) {
         const int team = (warp - kMtConverter) / kMtTeam, quarter = warp & 3, half = ((warp - kMtConverter) >> 2) & 1, row = quarter * 32 + lane;
         const uint8_t *cp = nullptr, *sp = nullptr;
-        int tile = blockIdx.x, g = team;
+        int tile = blockIdx.x / 2, g = team;
         auto rows_of = [&]() {                                               // past the end: some other row, nobody reads the results
-            const int p = tile % A.tiles_p;
+            const int p = 2 * (tile % A.pairs_p) + rank;
             const int m = kGated ? min(64 * p + (row & 63), A.outs - 1) + (row >= 64 ? A.outs : 0) : min(128 * p + row, A.W.M - 1);
             cp = A.W.codes + mx_code_row(m, groups) + half * 2 * kMxQuarter;
             sp = A.W.scales + mx_scale_row(m, groups);
         };
         auto settle = [&]() {                                                // (tile, g) with g past the tile's groups: into the next tiles
             bool moved = false;
-            while (g >= groups && tile < tiles) g -= groups, tile += gridDim.x, moved = true;
+            while (g >= groups && tile < tiles) g -= groups, tile += step, moved = true;
             return moved;
         };
         uint4 q0 = make_uint4(0u, 0u, 0u, 0u), q1 = q0;
@@ -337,10 +359,10 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             mt_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(a_full + 8 * team);
+            if (lane == 0) mt_arrive(a_full + 8 * team);
         }
     } else if (warp >= kMtEpilogue) {
-        mt_epilogue<kGated, kMtForwardRows>(A, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane);
+        mt_epilogue<kGated, kMtForwardRows>(A, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane, rank);
     }
     mt_end(tmem, &dead, warp);
 }
@@ -355,19 +377,20 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
     __shared__ uint32_t tmem_slot;
     __shared__ int dead;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t base = smem_addr(smem), stage_bytes = kMtABytes + static_cast<uint32_t>(A.nt) * 128u;
+    const uint32_t base = smem_addr(smem), stage_bytes = kMtABytes + static_cast<uint32_t>(A.nt) * 64u;
     const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16;
-    const int tiles = A.tiles_p * A.tiles_n;
+    const int tiles = A.pairs_p * A.tiles_n, step = gridDim.x / 2;
+    const uint32_t rank = mt_rank();
 
     pdl_launch_dependents();
     if (tid == 0) {
         for (int i = 0; i < A.stages; i++) {
-            mbar_init(full + 8 * i, kMtTeam + 1);
+            mbar_init(full + 8 * i, 1 + 2 * kMtTeam);                        // B, and a team of each CTA
             mbar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(done + 8 * i, 1);
-            mbar_init(free_ + 8 * i, 4);
+            mbar_init(free_ + 8 * i, 8);
         }
         mbar_fence_init();
         dead = 0;
@@ -375,13 +398,13 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
     const uint32_t tmem = mt_begin(&tmem_slot, warp);
 
     if (warp == kMtLoader) {
-        if (lane == 0) mt_loader<1>(A, &bmap, base + kMtABytes, stage_bytes, full, empty, &dead);
-    } else if (warp == kMtIssuer) {
+        if (lane == 0) mt_loader<1>(A, &bmap, base + kMtABytes, stage_bytes, full, empty, &dead, rank);
+    } else if (warp == kMtIssuer && rank == 0) {
         // 32-bit sums, both operands BF16, A MN-major, B K-major
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (8u << 24);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(A.nt >> 3) << 17) | (16u << 24);
         int slot = 0, buf = 0;
         uint32_t phase = 0u, buf_phase = 1u, ok = 0u;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        for (int tile = blockIdx.x / 2; tile < tiles; tile += step) {
             mx_wait(free_ + 8 * buf, buf_phase, &dead, 21);
             mt_fence_after();
             for (int c = 0; c < A.boxes_c; c++) {
@@ -406,26 +429,26 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
         const int row = ((warp - kMtConverter) & (kMtTeam - 1)) * 8 + ((lane >> 3) | (lane & 4));      // rows 0, 4, 1, 5, 2, 6, 3, 7
         const uint32_t to = (row >> 3) * 1024 + (row & 7) * 128;
         const int storage_tiles = (A.W.M + 15) >> 4;
-        int tile = blockIdx.x, c = team, slot = team;
+        int tile = blockIdx.x / 2, c = team, slot = team;
         uint32_t phase = 1u;
         // units are loaded two stages of the team ahead of their use
         uint4 q, q_next;
         uint32_t s, s_next;
         int ask_tile = tile, ask_c = c;
         auto load = [&](uint4 &to_q, uint32_t &to_s) {
-            while (ask_c >= A.boxes_c && ask_tile < tiles) ask_c -= A.boxes_c, ask_tile += gridDim.x;
+            while (ask_c >= A.boxes_c && ask_tile < tiles) ask_c -= A.boxes_c, ask_tile += step;
             const int from = 4 * ask_c + (row >> 4);
             to_q = make_uint4(0u, 0u, 0u, 0u);
             to_s = 0u;
             if (ask_tile < tiles && from < storage_tiles) {
-                const int64_t at = static_cast<int64_t>(from) * A.W.groups + ask_tile % A.tiles_p;
+                const int64_t at = static_cast<int64_t>(from) * A.W.groups + min(2 * (ask_tile % A.pairs_p) + static_cast<int>(rank), A.W.groups - 1);      // past the end: nobody reads the results
                 to_q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16));
                 to_s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
             }
             ask_c += 2;
         };
         auto settle = [&]() {
-            while (c >= A.boxes_c && tile < tiles) c -= A.boxes_c, tile += gridDim.x;
+            while (c >= A.boxes_c && tile < tiles) c -= A.boxes_c, tile += step;
         };
         settle();
         load(q, s);
@@ -445,11 +468,11 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
             for (int j = 0; j < 4; j++) *reinterpret_cast<uint4 *>(dst + (j >> 1) * 8192 + ((((j & 1) * 4 + t) ^ (row & 7)) << 4)) = v[j];
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * slot);
+            if (lane == 0) mt_arrive(full + 8 * slot);
             if ((slot += 2) >= A.stages) slot = team, phase ^= 1u;
         }
     } else if (warp >= kMtEpilogue) {
-        mt_epilogue<false, kMtGradRows>(A, tmem, done, free_, nullptr, &dead, warp, lane);
+        mt_epilogue<false, kMtGradRows>(A, tmem, done, free_, nullptr, &dead, warp, lane, rank);
     }
     mt_end(tmem, &dead, warp);
 }
