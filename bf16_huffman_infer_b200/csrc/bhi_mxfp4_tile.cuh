@@ -15,6 +15,8 @@
 // overflow) take two products.
 #pragma once
 
+#include <type_traits>
+
 #include <cuda.h>      // CUtensorMap and the encode entry point's types; the driver library is not linked
 
 #include "bhi_mxfp4.cuh"
@@ -116,25 +118,29 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     return d;
 }
 
-// Eight codes and their scale byte as eight BF16 values in element order.
-__device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t s, bool large) {
+// Eight codes as eight BF16 values in element order, times f (kLarge: times 2^126, then f).
+template <bool kLarge>
+__device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t f) {
     constexpr uint32_t kMag = 0x01C001C0u, kSign = 0x80008000u;
     uint32_t h[4];
     h[0] = ((w << 6) & kMag) | ((w << 12) & kSign);
     h[1] = ((w << 2) & kMag) | ((w << 8) & kSign);
     h[2] = ((w >> 2) & kMag) | ((w << 4) & kSign);
     h[3] = ((w >> 6) & kMag) | (w & kSign);
-    if (!large) {
-        const uint32_t f = s * 0x00800080u + 0x3F003F00u;                    // 2^(s - 1)
 #pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = mul_bf16x2(h[i], f);
-    } else {
-        const uint32_t f = s == 0u ? 0x00400040u : s * 0x00800080u;          // 2^(s - 127); 255: infinity, and its codes are zero
-#pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = mul_bf16x2(mul_bf16x2(h[i], 0x7E807E80u), f);
-    }
+    for (int i = 0; i < 4; i++) h[i] = mul_bf16x2(kLarge ? mul_bf16x2(h[i], 0x7E807E80u) : h[i], f);
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
+// The factors of a row's four blocks: 2^(s - 1), or of large scales 2^(s - 127) (255: infinity, and its codes are zero).
+template <bool kLarge>
+__device__ __forceinline__ void mx_factors(uint32_t scales, uint32_t (&f)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t s = (scales >> (8 * j)) & 255u;
+        f[j] = kLarge ? (s == 0u ? 0x00400040u : s * 0x00800080u) : s * 0x00800080u + 0x3F003F00u;
+    }
+}
+__device__ __forceinline__ uint32_t word_of(const uint4 &q, int j) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; }
 
 // ---- sums to outputs: a thread's lane of the accumulator is value p, columns are rows of out --------------------------------------------
 // kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16 columns the first eight become the gate lanes', the
@@ -316,8 +322,8 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         auto rows_of = [&]() {                                               // past the end: some other row, nobody reads the results
             const int p = 2 * (tile % A.pairs_p) + rank;
             const int m = kGated ? min(64 * p + (row & 63), A.outs - 1) + (row >= 64 ? A.outs : 0) : min(128 * p + row, A.W.M - 1);
-            cp = A.W.codes + mx_code_row(m, groups) + half * 2 * kMxQuarter;
-            sp = A.W.scales + mx_scale_row(m, groups);
+            cp = A.W.codes + mx_code_row(m, groups) + half * 2 * kMxQuarter + g * kMxTileCodes;
+            sp = A.W.scales + mx_scale_row(m, groups) + g * kMxTileScales;
         };
         auto settle = [&]() {                                                // (tile, g) with g past the tile's groups: into the next tiles
             bool moved = false;
@@ -327,10 +333,9 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         uint4 q0 = make_uint4(0u, 0u, 0u, 0u), q1 = q0;
         uint32_t s = 0u;
         auto load = [&]() {
-            const uint8_t *c = cp + static_cast<int64_t>(g) * kMxTileCodes;
-            q0 = __ldg(reinterpret_cast<const uint4 *>(c));
-            q1 = __ldg(reinterpret_cast<const uint4 *>(c + kMxQuarter));
-            s = __ldg(reinterpret_cast<const uint32_t *>(sp + static_cast<int64_t>(g) * kMxTileScales));
+            q0 = __ldg(reinterpret_cast<const uint4 *>(cp));
+            q1 = __ldg(reinterpret_cast<const uint4 *>(cp + kMxQuarter));
+            s = __ldg(reinterpret_cast<const uint32_t *>(sp));
         };
         settle();
         if (tile < tiles) {
@@ -341,14 +346,21 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         uint32_t phase = 1u;
         while (tile < tiles) {
             uint4 h[8];
-            const bool large = (s & 0x80808080u) != 0u;
+            auto expand = [&](auto large) {
+                constexpr bool kLarge = decltype(large)::value;
+                uint32_t f[4];
+                mx_factors<kLarge>(s, f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t byte = (s >> (8 * j)) & 255u;
-                h[2 * j] = mx_word_to_bf16(j == 0 ? q0.x : j == 1 ? q0.y : j == 2 ? q0.z : q0.w, byte, large);
-                h[2 * j + 1] = mx_word_to_bf16(j == 0 ? q1.x : j == 1 ? q1.y : j == 2 ? q1.z : q1.w, byte, large);
-            }
+                for (int j = 0; j < 4; j++) {
+                    h[2 * j] = mx_word_to_bf16<kLarge>(word_of(q0, j), f[j]);
+                    h[2 * j + 1] = mx_word_to_bf16<kLarge>(word_of(q1, j), f[j]);
+                }
+            };
+            if (__any_sync(0xFFFFFFFFu, (s & 0x80808080u) != 0u)) expand(std::true_type{});
+            else expand(std::false_type{});
             g += 2;
+            cp += 2 * kMxTileCodes;
+            sp += 2 * kMxTileScales;
             if (settle() && tile < tiles) rows_of();
             if (tile < tiles) load();
             mx_wait(a_empty + 8 * team, phase, &dead, 23);
@@ -435,29 +447,44 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
         uint4 q, q_next;
         uint32_t s, s_next;
         int ask_tile = tile, ask_c = c;
-        auto load = [&](uint4 &to_q, uint32_t &to_s) {
+        const uint8_t *cp = nullptr, *sp = nullptr;
+        const int64_t codes_on = static_cast<int64_t>(8) * A.W.groups * kMxTileCodes, scales_on = static_cast<int64_t>(8) * A.W.groups * kMxTileScales;
+        auto place = [&]() {                                                 // of stage ask_c of ask_tile; p past the end: nobody reads the results
             while (ask_c >= A.boxes_c && ask_tile < tiles) ask_c -= A.boxes_c, ask_tile += step;
-            const int from = 4 * ask_c + (row >> 4);
+            const int64_t at = static_cast<int64_t>(4 * ask_c + (row >> 4)) * A.W.groups + min(2 * (ask_tile % A.pairs_p) + static_cast<int>(rank), A.W.groups - 1);
+            cp = A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16;
+            sp = A.W.scales + at * kMxTileScales + (row & 15) * 4;
+        };
+        auto load = [&](uint4 &to_q, uint32_t &to_s) {
             to_q = make_uint4(0u, 0u, 0u, 0u);
             to_s = 0u;
-            if (ask_tile < tiles && from < storage_tiles) {
-                const int64_t at = static_cast<int64_t>(from) * A.W.groups + min(2 * (ask_tile % A.pairs_p) + static_cast<int>(rank), A.W.groups - 1);      // past the end: nobody reads the results
-                to_q = __ldg(reinterpret_cast<const uint4 *>(A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16));
-                to_s = __ldg(reinterpret_cast<const uint32_t *>(A.W.scales + at * kMxTileScales + (row & 15) * 4));
+            if (ask_tile < tiles && 4 * ask_c + (row >> 4) < storage_tiles) {
+                to_q = __ldg(reinterpret_cast<const uint4 *>(cp));
+                to_s = __ldg(reinterpret_cast<const uint32_t *>(sp));
             }
             ask_c += 2;
+            cp += codes_on;
+            sp += scales_on;
+            if (ask_c >= A.boxes_c) place();
         };
         auto settle = [&]() {
             while (c >= A.boxes_c && tile < tiles) c -= A.boxes_c, tile += step;
         };
         settle();
+        place();
         load(q, s);
         load(q_next, s_next);
         while (tile < tiles) {
             uint4 v[4];
-            const bool large = (s & 0x80808080u) != 0u;
+            auto expand = [&](auto large) {
+                constexpr bool kLarge = decltype(large)::value;
+                uint32_t f[4];
+                mx_factors<kLarge>(s, f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mx_word_to_bf16(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, (s >> (8 * j)) & 255u, large);
+                for (int j = 0; j < 4; j++) v[j] = mx_word_to_bf16<kLarge>(word_of(q, j), f[j]);
+            };
+            if (__any_sync(0xFFFFFFFFu, (s & 0x80808080u) != 0u)) expand(std::true_type{});
+            else expand(std::false_type{});
             q = q_next, s = s_next;
             load(q_next, s_next);
             c += 2;
