@@ -25,15 +25,16 @@ EncodeTiledFn encode_tiled() {
 
 enum Kind { kPlain, kGatedPair, kGradient };
 
-// Rows of a tile (a multiple of 32, at most `most`): the fewest rounds of tiles over the pairs of SMs times a tile's cost, which is its rows where
-// the tensor cores bound it and that of kExpand rows where the expansion of the weight does.
-constexpr int kExpand = 128;
-int rows_of_tile(int rows, int pairs_p, int most) {
+// Rows of a tile (a multiple of 32): the fewest rounds of tiles over the pairs of SMs times what a tile costs, by its rows: measured (4096
+// columns, ns for 128 of them) 425 + 0.85 rows forward, twice (395 + 0.55 rows) for a gradient; an accumulator on its own (above 128 rows, forward)
+// keeps the products waiting while it is read.
+int rows_of_tile(int rows, int pairs_p, int groups, bool gradient) {
     int best = 32;
     double best_cost = 1e30;
-    for (int nt = 32; nt <= most; nt += 32) {
+    for (int nt = 32; nt <= kMtRows; nt += 32) {
         const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p, pairs = sm_count() / 2;
-        const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * (nt > kExpand ? nt : kExpand) + 1e-3 * nt;
+        const double tile = gradient ? groups * 2 * (395 + 0.55 * nt) : groups * (425 + 0.85 * nt) + (nt > kMtTwoRows ? 6.0 * nt : 0.0);
+        const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * tile + 1e-3 * nt;
         if (cost < best_cost - 1e-9) {
             best_cost = cost;
             best = nt;
@@ -49,9 +50,10 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     if (!encode) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     const int per = kKind == kGatedPair ? 64 : 128;
     a.pairs_p = (a.outs + 2 * per - 1) / (2 * per);
-    a.nt = rows_of_tile(a.rows, a.pairs_p, kKind == kGradient ? kMtGradRows : kMtForwardRows);
+    a.nt = rows_of_tile(a.rows, a.pairs_p, static_cast<int>((b_cols + 127) / 128), kKind == kGradient);
     if (getenv("MXN")) a.nt = atoi(getenv("MXN"));
     a.tiles_n = (a.rows + a.nt - 1) / a.nt;
+    a.buffers = kKind == kGradient || a.nt <= kMtTwoRows ? 2 : 1;
     a.boxes_c = static_cast<int>((b_cols + kMtBox - 1) / kMtBox);
     BHI_REQUIRE(static_cast<int64_t>(a.pairs_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
     const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 64u : static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;

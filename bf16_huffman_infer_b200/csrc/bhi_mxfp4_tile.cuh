@@ -7,7 +7,7 @@
 // its own an SM would write and read all of B, 96 KB of shared memory for 192 rows and 128 values of c, 750 clocks at 128 bytes a clock, where
 // the products take 768: together with everything else that made 1030.
 // Sixteen warps of a CTA turn codes into BF16, exactly (a code times a power of two fits), one thread requests B by TMA, one of the pair issues the
-// products, four warps read the accumulators back, two of which alternate between tiles.  The weight is expanded once for all rows of a
+// products, eight warps read the accumulators back.  The weight is expanded once for all rows of a
 // tile, so the expansion (19 instructions for eight values) stays behind the tensor cores from some 130 rows on.
 //
 // A code's bits s eem are moved to a BF16's sign, lowest exponent and highest mantissa bits: that is its value times 2^-126, the
@@ -23,14 +23,17 @@
 
 namespace bhi {
 
-constexpr int kMtLoader = 0, kMtIssuer = 1, kMtEpilogue = 4, kMtConverter = 8;      // warps; 2 and 3 idle
+constexpr int kMtLoader = 0, kMtIssuer = 1, kMtEpilogue = 4, kMtConverter = 12;     // warps; 2 and 3 idle
+constexpr int kMtPlaces = 4;                      // groups of A in tensor memory
+constexpr int kMtPlaceAt = 256;                   // their first column
 constexpr int kMtTeam = 8;                        // warps of a team of converters; two teams
 constexpr int kMtThreads = 32 * (kMtConverter + 2 * kMtTeam);
 constexpr int kMtBox = 64;                        // values of c a TMA box
 constexpr uint32_t kMtABytes = 128 * kMtBox * 2;
 constexpr int kMtStagesMax = 16;
-constexpr uint32_t kMtSwap = 16 * 64 * 4;         // bytes through which a gated block changes lanes
-constexpr int kMtForwardRows = 192, kMtGradRows = 256;       // most rows of a tile
+constexpr uint32_t kMtSwap = 2 * 16 * 64 * 4;         // bytes through which a gated block changes lanes
+constexpr int kMtRows = 256;                      // most rows of a tile
+constexpr int kMtTwoRows = 128;                   // forward: most rows of a tile with two accumulators
 
 struct MxTileArgs {
     MxWeight W;
@@ -41,6 +44,7 @@ struct MxTileArgs {
     int activation;
     int nt, pairs_p, tiles_n, boxes_c;            // rows of a tile (a multiple of 32), pairs of tiles along p, tiles along n, boxes of 64 values of c
     int stages;                                   // of the ring
+    int buffers;                                  // accumulators
 };
 
 // a box into this CTA's shared memory; its bytes count at the barrier of this place in the CTA that issues the products (`bar`, by mt_leader)
@@ -143,13 +147,19 @@ __device__ __forceinline__ void mx_factors(uint32_t scales, uint32_t (&f)[4]) {
 __device__ __forceinline__ uint32_t word_of(const uint4 &q, int j) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; }
 
 // ---- sums to outputs: a thread's lane of the accumulator is value p, columns are rows of out --------------------------------------------
-// kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16 columns the first eight become the gate lanes', the
-// others the up lanes': each hands the other half over through shared memory.
+// Two warps have the same lanes and take 16 columns in turn.  kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16
+// columns the first eight become the gate lanes', the others the up lanes': each hands the other half over through shared memory.
 template <bool kGated, int kBuffer>
 __device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, uint32_t done, uint32_t free_, float *swap, int *dead, int warp, int lane, uint32_t rank) {
-    const int quarter = warp & 3, lane_p = quarter * 32 + lane, tiles = A.pairs_p * A.tiles_n, step = gridDim.x / 2;
+    const int quarter = warp & 3, half = (warp - kMtEpilogue) >> 2, lane_p = quarter * 32 + lane, tiles = A.pairs_p * A.tiles_n, step = gridDim.x / 2;
     int buf = 0;
     uint32_t phase = 0u;
+    swap += half * (kMtSwap / 8);
+    auto read = [&]() {                                                      // this warp's columns are read: the issuer may have them back
+        mt_fence_before();
+        __syncwarp();
+        if (lane == 0) mt_arrive(free_ + 8 * buf);
+    };
     pdl_wait();                                                              // outputs may be what the previous kernel reads, a bias what it writes
     for (int tile = blockIdx.x / 2; tile < tiles; tile += step) {
         const int p = 2 * (tile % A.pairs_p) + rank, n0 = tile / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0);
@@ -160,48 +170,50 @@ __device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, uint32_t tmem, 
         mx_wait(done + 8 * buf, phase, dead, 24);
         mt_fence_after();
         const uint32_t from = tmem + buf * kBuffer + (static_cast<uint32_t>(quarter) << 21);
-        for (int c = 0; c < cols; c += 16) {
+        if (16 * half >= cols) read();
+        for (int c = 16 * half; c < cols; c += 32) {
             float v[16];
             mt_load(from + c, v);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (c + 16 >= cols) {                                            // the accumulator is read: the issuer may have it back
-                mt_fence_before();
-                __syncwarp();
-                if (lane == 0) mt_arrive(free_ + 8 * buf);
-            }
+            if (c + 32 >= cols) read();
 #pragma unroll
             for (int i = 0; i < 16; i++) v[i] += bias;
             if constexpr (!kGated) {
                 if (live) {
                     uint16_t *to = A.out + static_cast<int64_t>(n0 + c) * A.outs + m;
+                    if (c + 16 <= cols) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (c + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(v[i]);
+                        for (int i = 0; i < 16; i++, to += A.outs) *to = f32_to_bf16_rn(v[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++, to += A.outs)
+                            if (c + i < cols) *to = f32_to_bf16_rn(v[i]);
+                    }
                 }
             } else {
                 if (A.pre != nullptr && live) {
                     float *to = A.pre + static_cast<int64_t>(n0 + c) * 2 * A.outs + m + (up ? A.outs : 0);
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (c + i < cols) to[static_cast<int64_t>(i) * 2 * A.outs] = v[i];
+                    for (int i = 0; i < 16; i++, to += 2 * static_cast<int64_t>(A.outs))
+                        if (c + i < cols) *to = v[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) swap[((up ? 0 : 8) + i) * 64 + (lane_p & 63)] = up ? v[i] : v[8 + i];
-                asm volatile("bar.sync 2, 128;" ::: "memory");
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
                 const int i0 = up ? 8 : 0;
                 if (live) {
                     uint16_t *to = A.out + static_cast<int64_t>(n0 + c + i0) * A.outs + m;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 8; i++, to += A.outs) {
                         const float other = swap[(i0 + i) * 64 + (lane_p & 63)];
                         const float g = up ? other : v[i], u = up ? v[8 + i] : other;
-                        if (c + i0 + i < cols) to[static_cast<int64_t>(i) * A.outs] = f32_to_bf16_rn(mx_act(A.activation, g) * u);
+                        if (c + i0 + i < cols) *to = f32_to_bf16_rn(mx_act(A.activation, g) * u);
                     }
                 }
-                asm volatile("bar.sync 2, 128;" ::: "memory");
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
             }
         }
-        if ((buf ^= 1) == 0) phase ^= 1u;
+        if (++buf == A.buffers) buf = 0, phase ^= 1u;
     }
 }
 
@@ -245,20 +257,22 @@ __device__ __forceinline__ void mt_end(uint32_t tmem, const int *dead, int warp)
 }
 
 // ---- forward: A in tensor memory ------------------------------------------------------------------------------------------------------
-// A thread of a team expands half a row's group (64 values) in registers while the other team's group is being multiplied, and stores
-// it to its lane of tensor memory when the products that read the place are done: the weight costs shared memory nothing, which B's way in
-// and out fills.  A team's place is its own.  Tensor memory: two accumulators of 192 columns, two groups of 64.
+// A thread of a team expands half a row's group (64 values) in registers while others are being multiplied, and stores it to its lane of tensor
+// memory when the products that read the place are done: the weight costs shared memory nothing, which B's way in and out fills.
+// Tensor memory: 256 columns of accumulators, two of up to 128 rows or one of up to 256, and four places of 64 columns, a group each, the even
+// ones one team's and the odd ones the other's.  (With two places the way from one group's last product to the next in its place, some
+// 1200 clocks, showed: 20.2 us for a tile of 192 rows and 4096 columns where the products take 15.)
 // kGated: 64 gate rows and the 64 up rows of the same outputs make a tile.
 template <bool kGated>
 __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs A, const __grid_constant__ CUtensorMap bmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * kMtStagesMax + 8];
+    __shared__ __align__(8) uint64_t bars[2 * kMtStagesMax + 4 + 2 * kMtPlaces];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
     const uint32_t base = smem_addr(smem), box = static_cast<uint32_t>(A.nt) * 64u, stage_bytes = 2 * box;
     const uint32_t full = smem_addr(&bars[0]), empty = smem_addr(&bars[kMtStagesMax]), done = smem_addr(&bars[2 * kMtStagesMax]), free_ = done + 16,
-                   a_full = done + 32, a_empty = done + 48;
+                   a_full = done + 32, a_empty = a_full + 8 * kMtPlaces;
     const int tiles = A.pairs_p * A.tiles_n, groups = A.W.groups, step = gridDim.x / 2;
     const uint32_t rank = mt_rank();
 
@@ -270,7 +284,9 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(done + 8 * i, 1);
-            mbar_init(free_ + 8 * i, 8);
+            mbar_init(free_ + 8 * i, 16);
+        }
+        for (int i = 0; i < kMtPlaces; i++) {
             mbar_init(a_full + 8 * i, 2 * kMtTeam);
             mbar_init(a_empty + 8 * i, 1);
         }
@@ -294,10 +310,10 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
                 if (!a_ok) mx_wait(a_full + 8 * place, a_phase, &dead, 25);
                 if (!b_ok) mx_wait(full + 8 * slot, phase, &dead, 22);
                 mt_fence_after();
-                const uint32_t a = tmem + 2 * kMtForwardRows + place * 64, d = tmem + buf * kMtForwardRows, used = slot, from = place;
+                const uint32_t a = tmem + kMtPlaceAt + place * 64, d = tmem + buf * kMtTwoRows, used = slot, from = place;
                 const uint64_t b = mt_desc(base + slot * stage_bytes, 1);
                 if (++slot == A.stages) slot = 0, phase ^= 1u;
-                if ((place ^= 1) == 0) a_phase ^= 1u;
+                if (++place == kMtPlaces) place = 0, a_phase ^= 1u;
                 a_ok = mt_over(a_full + 8 * place, a_phase);
                 b_ok = mt_over(full + 8 * slot, phase);
                 if (mt_elect()) {
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
                 }
                 __syncwarp();
             }
-            if ((buf ^= 1) == 0) buf_phase ^= 1u;
+            if (++buf == A.buffers) buf = 0, buf_phase ^= 1u;
         }
     } else if (warp >= kMtConverter) {
         const int team = (warp - kMtConverter) / kMtTeam, quarter = warp & 3, half = ((warp - kMtConverter) >> 2) & 1, row = quarter * 32 + lane;
@@ -342,7 +358,8 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
             rows_of();
             load();
         }
-        const uint32_t to = tmem + 2 * kMtForwardRows + team * 64 + half * 8 + (static_cast<uint32_t>(quarter) << 21);
+        const uint32_t to = tmem + kMtPlaceAt + half * 8 + (static_cast<uint32_t>(quarter) << 21);
+        int place = team;
         uint32_t phase = 1u;
         while (tile < tiles) {
             uint4 h[8];
@@ -363,18 +380,18 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
             sp += 2 * kMxTileScales;
             if (settle() && tile < tiles) rows_of();
             if (tile < tiles) load();
-            mx_wait(a_empty + 8 * team, phase, &dead, 23);
-            phase ^= 1u;
+            mx_wait(a_empty + 8 * place, phase, &dead, 23);
             mt_fence_after();
 #pragma unroll
-            for (int j = 0; j < 4; j++) mt_store8(to + 16 * j, h[2 * j], h[2 * j + 1]);
+            for (int j = 0; j < 4; j++) mt_store8(to + place * 64 + 16 * j, h[2 * j], h[2 * j + 1]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             mt_fence_before();
             __syncwarp();
-            if (lane == 0) mt_arrive(a_full + 8 * team);
+            if (lane == 0) mt_arrive(a_full + 8 * place);
+            if ((place += 2) >= kMtPlaces) place = team, phase ^= 1u;
         }
     } else if (warp >= kMtEpilogue) {
-        mt_epilogue<kGated, kMtForwardRows>(A, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane, rank);
+        mt_epilogue<kGated, kMtTwoRows>(A, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane, rank);
     }
     mt_end(tmem, &dead, warp);
 }
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(done + 8 * i, 1);
-            mbar_init(free_ + 8 * i, 8);
+            mbar_init(free_ + 8 * i, 16);
         }
         mbar_fence_init();
         dead = 0;
@@ -422,7 +439,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
             for (int c = 0; c < A.boxes_c; c++) {
                 if (!ok) mx_wait(full + 8 * slot, phase, &dead, 22);
                 mt_fence_after();
-                const uint32_t d = tmem + buf * kMtGradRows, used = slot;
+                const uint32_t d = tmem + buf * kMtRows, used = slot;
                 const uint64_t a = mt_desc(base + slot * stage_bytes, 512), b = mt_desc(base + slot * stage_bytes + kMtABytes, 1);
                 if (++slot == A.stages) slot = 0, phase ^= 1u;
                 ok = mt_over(full + 8 * slot, phase);
@@ -434,7 +451,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
                 }
                 __syncwarp();
             }
-            if ((buf ^= 1) == 0) buf_phase ^= 1u;
+            if (++buf == A.buffers) buf = 0, buf_phase ^= 1u;
         }
     } else if (warp >= kMtConverter) {
         const int team = (warp - kMtConverter) / kMtTeam, t = lane & 3;
@@ -499,7 +516,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
             if ((slot += 2) >= A.stages) slot = team, phase ^= 1u;
         }
     } else if (warp >= kMtEpilogue) {
-        mt_epilogue<false, kMtGradRows>(A, tmem, done, free_, nullptr, &dead, warp, lane, rank);
+        mt_epilogue<false, kMtRows>(A, tmem, done, free_, nullptr, &dead, warp, lane, rank);
     }
     mt_end(tmem, &dead, warp);
 }
