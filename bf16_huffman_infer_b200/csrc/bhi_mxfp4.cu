@@ -113,19 +113,47 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, u
     }
 }
 
-__device__ __forceinline__ float bf16_at(const uint16_t *p, int64_t i) { return __uint_as_float(static_cast<uint32_t>(p[i]) << 16); }
-
 // ---- the gated pair's gradient: dg = dh u act'(g), du = dh act(g) --------------------------------------------------------
-__global__ void __launch_bounds__(256) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, int act, uint16_t *dpre, int inter, int ldp, int64_t n) {
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / inter, c = i % inter;
-        const float g = pre[r * 2 * inter + c], u = pre[r * 2 * inter + inter + c], dh = bf16_at(dH, i);
-        float a, da;
-        mx_act_grad(act, g, a, da);
-        dpre[r * ldp + c] = f32_to_bf16_rn(dh * u * da);
-        dpre[r * ldp + inter + c] = f32_to_bf16_rn(dh * a);
+// Bound by memory: 8 bytes of projections and 2 of dh in, 4 out.  A thread takes kVec neighbours of a row.
+constexpr int kMxPairThreads = 256;
+
+template <int kVec>
+__global__ void __launch_bounds__(kMxPairThreads) mx_gated_grad_kernel(const float *pre, const uint16_t *dH, int act, uint16_t *dpre, int inter, int ldp, int rows) {
+    const int c = (blockIdx.x * kMxPairThreads + threadIdx.x) * kVec;
+    if (c >= inter) return;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float *from = pre + static_cast<int64_t>(r) * 2 * inter + c;
+        uint16_t *to = dpre + static_cast<int64_t>(r) * ldp + c;
+        const uint16_t *dh = dH + static_cast<int64_t>(r) * inter + c;
+        float g[kVec], u[kVec], d[kVec], dg[kVec], du[kVec];
+        if constexpr (kVec == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4 *>(from)), b = __ldcs(reinterpret_cast<const float4 *>(from + inter));
+            const uint2 h = __ldcs(reinterpret_cast<const uint2 *>(dh));
+            g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, u[0] = b.x, u[1] = b.y, u[2] = b.z, u[3] = b.w;
+            d[0] = bf16lo_to_f32(h.x), d[1] = bf16hi_to_f32(h.x), d[2] = bf16lo_to_f32(h.y), d[3] = bf16hi_to_f32(h.y);
+        } else {
+            g[0] = from[0], u[0] = from[inter], d[0] = bf16lo_to_f32(dh[0]);
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            float a, da;
+            mx_act_grad(act, g[i], a, da);
+            dg[i] = d[i] * u[i] * da;
+            du[i] = d[i] * a;
+        }
+        if constexpr (kVec == 4) {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(dg[0], dg[1]), pack_bf16(dg[2], dg[3]));
+            *reinterpret_cast<uint2 *>(to + inter) = make_uint2(pack_bf16(du[0], du[1]), pack_bf16(du[2], du[3]));
+        } else {
+            to[0] = f32_to_bf16_rn(dg[0]);
+            to[inter] = f32_to_bf16_rn(du[0]);
+        }
     }
 }
+
+// Does nothing, after the quantisation: a kernel with launch overlap that follows may read the weight before it has waited for the kernel
+// in front of it, which is then this one, and this one starts when the weight is complete.
+__global__ void mx_settle_kernel() {}
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 static int mx_check(const void *codes, const void *scales, int M, int K) {
@@ -141,10 +169,6 @@ static MxWeight mx_weight(const uint8_t *codes, const uint8_t *scales, int M, in
 static int mx_launched(const char *what) {
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? BHI_OK : cuda_fail(e, what);
-}
-static int mx_stream_grid(int64_t items, int threads) {
-    const int64_t blocks = (items + threads - 1) / threads, most = static_cast<int64_t>(sm_count()) * 16;
-    return static_cast<int>(blocks < most ? blocks : most);
 }
 // Blocks and threads over the words of a row (whole warps, as few idle ones as possible) by rows, some eight blocks an SM.
 static void mx_matrix_grid(int words, int M, dim3 &grid, dim3 &block) {
@@ -173,6 +197,7 @@ int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, u
     case BHI_DTYPE_FP16: mx_quantize_kernel<<<grid, block, 0, st>>>(static_cast<const __half *>(W), M, K, groups, codes, scales); break;
     default: mx_quantize_kernel<<<grid, block, 0, st>>>(static_cast<const float *>(W), M, K, groups, codes, scales); break;
     }
+    mx_settle_kernel<<<1, 32, 0, st>>>();
     return mx_launched("quantisation launch");
 }
 
@@ -222,12 +247,14 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
 
 int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows, void *stream) {
     BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2 && rows >= 1, "empty gradient");
-    BHI_REQUIRE(pre && dH && dpre && aligned(pre, 16) && aligned(dH, 2) && aligned(dpre, 16) && ldp >= 2 * inter, "bad gradient buffers");
+    BHI_REQUIRE(pre && dH && dpre && aligned(pre, 16) && aligned(dH, 2) && aligned(dpre, 16) && ldp >= 2 * inter && ldp % 4 == 0, "bad gradient buffers");
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
-    const int64_t n = static_cast<int64_t>(rows) * inter;
-    const int grid = mx_stream_grid(n, 256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    mx_gated_grad_kernel<<<grid, 256, 0, st>>>(pre, dH, activation, dpre, inter, ldp, n);
+    const bool wide = inter % 4 == 0 && aligned(dH, 8);
+    const int across = (inter + kMxPairThreads * (wide ? 4 : 1) - 1) / (kMxPairThreads * (wide ? 4 : 1)), most = (sm_count() * 16 + across - 1) / across;
+    const dim3 grid(across, rows < most ? rows : most);
+    if (wide) mx_gated_grad_kernel<4><<<grid, kMxPairThreads, 0, st>>>(pre, dH, activation, dpre, inter, ldp, rows);
+    else mx_gated_grad_kernel<1><<<grid, kMxPairThreads, 0, st>>>(pre, dH, activation, dpre, inter, ldp, rows);
     return mx_launched("gated gradient launch");
 }
 

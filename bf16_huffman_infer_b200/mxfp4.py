@@ -43,9 +43,9 @@ class MXFP4Weight(nn.Module):
         for name, t, shape in (("codes", codes, (tiles, groups, 4, 16, 16)), ("scales", scales, (tiles, groups, 16, 4))):
             if t.dtype != torch.uint8 or tuple(t.shape) != shape:
                 raise ValueError(f"{name} of a {out_features} x {in_features} weight must be u8 {shape}, not {t.dtype} {tuple(t.shape)}")
-        self.codes = nn.Buffer(codes)
-        self.scales = nn.Buffer(scales)
-        self.out_features, self.in_features = int(out_features), int(in_features)
+        # as register_buffer and nn.Module's attributes leave them, in a quarter of the time
+        self._buffers.update(codes=codes, scales=scales)
+        self.__dict__.update(out_features=int(out_features), in_features=int(in_features))
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -80,8 +80,9 @@ class MXFP4Weight(nn.Module):
         a = a.detach()
         if not a.is_cuda and not torch.cuda.is_available():
             raise RuntimeError("bf16_huffman_infer_b200 needs a CUDA device: there is no CPU implementation")
-        home = a.device
-        a = a.to(home if a.is_cuda else torch.device("cuda", torch.cuda.current_device())).contiguous()
+        if not a.is_cuda:
+            a = a.to(torch.device("cuda", torch.cuda.current_device()))
+        a = a.contiguous()
         if a.data_ptr() % 16:
             a = a.clone()
         tiles, groups = _padded(*a.shape)
@@ -90,9 +91,6 @@ class MXFP4Weight(nn.Module):
         ops.mxfp4_quantize(a, codes, scales)
         if to_cpu:
             codes, scales = transfer.download(codes), transfer.download(scales)
-        else:
-            # the buffers must be complete in memory before a kernel with launch overlap reads them
-            torch.cuda.current_stream(a.device).synchronize()
         return cls(codes, scales, *a.shape)
 
     @classmethod
@@ -137,25 +135,33 @@ def _padded(M: int, K: int) -> Tuple[int, int]:
     return (M + 15) // 16, (K + 127) // 128
 
 
-def _differentiable(*tensors: Optional[Tensor]) -> bool:
-    """Whether a derivative or a transformation of torch.func may be asked of a call on these tensors."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+_is_grad_enabled, _interpreter = torch.is_grad_enabled, torch._C._functorch.peek_interpreter_stack
+
+
+def _recorded(x: Tensor, bias: Optional[Tensor]) -> bool:
+    """Whether a call on these tensors is to be recorded for a backward pass."""
+    return _is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
+
+
+def _transformed() -> bool:
+    """Whether a tangent, a batch dimension or a gradient of torch.func may ride on a tensor."""
+    return forward_ad._current_level >= 0 or _interpreter() is not None
 
 
 def _plain(x: Tensor) -> Tensor:
     """``x`` as the kernels read it: rows one after another from a 16-byte boundary."""
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x.clone() if x.data_ptr() % 16 else x
 
 
-def _check(input: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor], outputs: int) -> None:
-    assert input.is_cuda and input.dtype == torch.bfloat16, (input.device, input.dtype)
+def _check(input: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor]) -> None:
+    """What the operators do not see for themselves."""
+    assert input.is_cuda and input.dtype is torch.bfloat16, (input.device, input.dtype)
     if input.dim() < 1 or input.size(-1) != weight.in_features:
         raise RuntimeError(f"input of shape {tuple(input.shape)} does not fit a weight of {weight.in_features} columns")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (outputs,) or bias.device != input.device):
-        raise RuntimeError(f"bias must be a BF16 vector of {outputs} values on {input.device}")
+    if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (weight.out_features,) or bias.device != input.device):
+        raise RuntimeError(f"bias must be a BF16 vector of {weight.out_features} values on {input.device}")
 
 
 def _product(x: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor]) -> Tensor:
@@ -184,7 +190,30 @@ class _Held:
         self.weight = weight
 
 
+def _linear_backward(ctx, dy: Tensor):
+    dx = db = None
+    if ctx.needs_input_grad[0]:
+        dx = _LinearGradient.apply(dy, ctx.held) if _recorded(dy, None) or _transformed() else _input_gradient(dy, ctx.held.weight)
+    if ctx.needs_input_grad[2]:
+        db = dy.flatten(0, -2).sum(0, dtype=torch.float32).to(dy.dtype)
+    return dx, None, db
+
+
 class _Linear(torch.autograd.Function):
+    """The product where only backward passes are asked of it: the form with a separate ``setup_context`` binds its arguments by signature
+    in every call, which takes longer than the product of a small layer."""
+
+    @staticmethod
+    def forward(ctx, x, held, bias):
+        ctx.held = held
+        return _product(x, held.weight, bias)
+
+    backward = staticmethod(_linear_backward)
+
+
+class _LinearTransformed(torch.autograd.Function):
+    """The same under the transformations of torch.func and forward-mode derivatives."""
+
     @staticmethod
     def forward(x, held, bias):
         return _product(x, held.weight, bias)
@@ -193,11 +222,7 @@ class _Linear(torch.autograd.Function):
     def setup_context(ctx, inputs, output):
         ctx.held, ctx.shape = inputs[1], output.shape
 
-    @staticmethod
-    def backward(ctx, dy):
-        dx = _LinearGradient.apply(dy, ctx.held) if ctx.needs_input_grad[0] else None
-        db = dy.flatten(0, -2).sum(0, dtype=torch.float32).to(dy.dtype) if ctx.needs_input_grad[2] else None
-        return dx, None, db
+    backward = staticmethod(_linear_backward)
 
     @staticmethod
     def jvp(ctx, dx, _, db):
@@ -210,14 +235,18 @@ class _Linear(torch.autograd.Function):
         return _batched(info, in_dims, x, bias, lambda x, bias: linear_mxfp4(x, held.weight, bias))
 
 
+def _input_gradient(dy: Tensor, weight: "MXFP4Weight") -> Tensor:
+    b = weight.__dict__["_buffers"]
+    dx = ops.mxfp4_linear_grad(_rows_of_eight(dy), b["codes"], b["scales"], weight.out_features, weight.in_features)
+    return dx if dy.dim() == 2 else dx.view(*dy.shape[:-1], weight.in_features)
+
+
 class _LinearGradient(torch.autograd.Function):
     """dx = dy W, itself linear in dy."""
 
     @staticmethod
     def forward(dy, held):
-        w = held.weight
-        b = w.__dict__["_buffers"]
-        return ops.mxfp4_linear_grad(_rows_of_eight(dy), b["codes"], b["scales"], w.out_features, w.in_features).view(*dy.shape[:-1], w.in_features)
+        return _input_gradient(dy, held.weight)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -248,8 +277,10 @@ def _batched(info, in_dims, x: Tensor, bias: Optional[Tensor], call: Callable) -
 def linear_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = None) -> Tensor:
     """``F.linear`` on a 4-bit weight: ``input`` BF16 ``[..., K]``, any number of rows; the bias (BF16, a value for each output) is part
     of the 32-bit sum.  Differentiable with respect to the input and the bias."""
-    _check(input, weight, bias, weight.out_features)
-    if _differentiable(input, bias):
+    _check(input, weight, bias)
+    if _transformed():
+        return _LinearTransformed.apply(input, _Held(weight), bias)
+    if _recorded(input, bias):
         return _Linear.apply(input, _Held(weight), bias)
     return _product(input, weight, bias)
 
@@ -296,8 +327,8 @@ def gated_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = Non
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
     if weight.out_features % 2:
         raise RuntimeError(f"a stacked weight has an even number of rows, not {weight.out_features}")
-    _check(input, weight, bias, weight.out_features)
-    if _differentiable(input, bias):
+    _check(input, weight, bias)
+    if _recorded(input, bias) or _transformed():
         return _Gated.apply(input, _Held(weight), bias, ACTIVATIONS[activation])
     return _gated(input, weight, bias, ACTIVATIONS[activation], None)
 

@@ -296,7 +296,7 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
 #define BHI_ACT_GELU_TANH 2    /* its approximation by tanh */
 
 /* W [M, K] of the named type, rows contiguous, to codes and scales: e = max(floor(log2 max|v|) - 2, -127), codes of v / 2^e
- * rounded to the nearest (ties to even), saturated at 6; a block with an infinity or NaN becomes NaN. */
+ * rounded to the nearest (ties to even), saturated at 6; a block with an infinity or NaN becomes NaN.  The products may follow on the same stream, launch overlap or not. */
 int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
 
 /* Y bf16 [M, K]: the values (exact but for scales beyond BF16's range). */
@@ -315,7 +315,7 @@ int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, in
 int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int K, const uint16_t *X, const uint16_t *bias,
                     int activation, uint16_t *H, float *pre, int rows, void *stream);
 
-/* dpre bf16 [rows, ldp] = [dH u act'(g) | dH act(g)]; bhi_mxfp4_linear_grad turns it into the gradient of X. */
+/* dpre bf16 [rows, ldp] (ldp a multiple of 4) = [dH u act'(g) | dH act(g)]; bhi_mxfp4_linear_grad turns it into the gradient of X. */
 int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows,
                          void *stream);
 
