@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "bhi_staged.cuh"
 
 namespace bhi {
@@ -87,6 +89,39 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
+
+// A code's bits s eem are moved to a BF16's sign, lowest exponent and highest mantissa bits: that is its value times 2^-126, the
+// subnormal code 0.5 included, and one product by 2^(126 + s - 127) makes both the value and its scale.  Scales above 2 (2^(126 + s - 127) would
+// overflow) take two products.
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// Eight codes as eight BF16 values in element order, times f (kLarge: times 2^126, then f).
+template <bool kLarge>
+__device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t f) {
+    constexpr uint32_t kMag = 0x01C001C0u, kSign = 0x80008000u;
+    uint32_t h[4];
+    h[0] = ((w << 6) & kMag) | ((w << 12) & kSign);
+    h[1] = ((w << 2) & kMag) | ((w << 8) & kSign);
+    h[2] = ((w >> 2) & kMag) | ((w << 4) & kSign);
+    h[3] = ((w >> 6) & kMag) | (w & kSign);
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = mul_bf16x2(kLarge ? mul_bf16x2(h[i], 0x7E807E80u) : h[i], f);
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+// The factors of a row's four blocks: 2^(s - 1), or of large scales 2^(s - 127) (255: infinity, and its codes are zero).
+template <bool kLarge>
+__device__ __forceinline__ void mx_factors(uint32_t scales, uint32_t (&f)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t s = (scales >> (8 * j)) & 255u;
+        f[j] = kLarge ? (s == 0u ? 0x00400040u : s * 0x00800080u) : s * 0x00800080u + 0x3F003F00u;
+    }
+}
+__device__ __forceinline__ uint32_t word_of(const uint4 &q, int j) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; }
 
 // 2^(s - 127); 255 gives infinity here (its codes are zero, so that their product is NaN)
 __device__ __forceinline__ float mx_scale(uint32_t s) { return __uint_as_float(s == 0u ? 0x00400000u : s << 23); }

@@ -1,5 +1,6 @@
 // The products of 4-bit microscaled weights with few rows of X: which form, and its launch.
 #include <algorithm>
+#include <cstdlib>
 
 #include "bhi_mxfp4_rows.cuh"
 
@@ -53,18 +54,27 @@ int launch(MxRowsArgs a, cudaStream_t st) {
 int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, uint16_t *Y, bool gated, int activation, float *pre, int rows, cudaStream_t st) {
     MxRowsArgs a{};
     a.W = W, a.X = X, a.bias = bias, a.Y = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
+    static const int f = getenv("MXF") ? atoi(getenv("MXF")) : 0;
     if (gated && a.outs % 16 == 0) {
+        if (f == 1 && rows <= 8) return launch<MxRowsForm<2, 1, 18, 2, 1, 1, true>>(a, st);
+        if (f == 1 && rows <= 16) return launch<MxRowsForm<2, 2, 18, 2, 1, 1, true>>(a, st);
+        if (f == 2 && rows <= 16) return launch<MxRowsForm<2, 2, 22, 2, 1, 1, true>>(a, st);
         if (rows <= 8) return launch<MxRowsForm<2, 1, 14, 2, 1, 2, true>>(a, st);
         if (rows <= 16) return launch<MxRowsForm<2, 2, 14, 2, 1, 2, true>>(a, st);
-        if (rows <= 32) return launch<MxRowsForm<2, 4, 10, 2, 1, 1, true>>(a, st);
+        if (rows <= 32) return launch<MxRowsForm<2, 4, 14, 2, 1, 1, true>>(a, st);
     } else if (gated) {                              // ups lie across two tiles each
         if (rows <= 8) return launch<MxRowsForm<3, 1, 14, 2, 1, 1, true>>(a, st);
-        if (rows <= 16) return launch<MxRowsForm<3, 2, 10, 2, 1, 1, true>>(a, st);
+        if (rows <= 16) return launch<MxRowsForm<3, 2, 14, 2, 1, 1, true>>(a, st);
         if (rows <= 32) return launch<MxRowsForm<3, 4, 10, 2, 1, 1, true>>(a, st);
     } else {
         int rc = kStagedDeclined;
         if (rows <= 8) rc = W.M >= 128 * 2 * sm_count() ? launch<MxRowsForm<2, 1, 7, 1, 2, 2, false>>(a, st) : launch<MxRowsForm<1, 1, 7, 1, 2, 4, false>>(a, st);
         if (rc != kStagedDeclined) return rc;
+        if (f == 1 && rows <= 16) return launch<MxRowsForm<2, 2, 18, 2, 1, 1, false>>(a, st);
+        if (f == 2 && rows <= 16) return launch<MxRowsForm<1, 2, 18, 2, 1, 3, false>>(a, st);
+        if (f == 3 && rows <= 16) return launch<MxRowsForm<1, 2, 22, 2, 1, 2, false>>(a, st);
+        if (f == 1 && rows <= 32) return launch<MxRowsForm<2, 4, 14, 2, 1, 1, false>>(a, st);
+        if (f == 2 && rows <= 32) return launch<MxRowsForm<1, 4, 18, 2, 1, 2, false>>(a, st);
         if (rows <= 8) return launch<MxRowsForm<2, 1, 14, 2, 1, 2, false>>(a, st);
         if (rows <= 16) return launch<MxRowsForm<2, 2, 14, 2, 1, 2, false>>(a, st);
         if (rows <= 32) return launch<MxRowsForm<1, 4, 14, 2, 1, 2, false>>(a, st);

@@ -4,10 +4,14 @@
 // stacked weight at once, h = act(g) u.
 //
 // Bound by the bytes of the weight.  A consumer warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
-// They come straight from global memory into registers, kDepth units ahead.  The codes are turned into FP16 by the hardware's conversion and multiplies blocks of 32 columns by m16n8k16 products whose sums start at zero: a block's scale applies
-// to its sum, in 32 bits, so codes need no scaling of their own.  X is FP16 there: each row's 128 values of a group are brought to
-// [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-32 of the largest in its 128;
-// below, the error is under 2^-40 of that largest one, far less than a 32-bit sum with it loses.
+// They come straight from global memory into registers, kDepth units ahead, and are multiplied by m16n8k16 products.
+//
+// Up to eight rows of X the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32
+// columns start at zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared
+// memory: each row's 128 values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to
+// 2^-32 of the largest in its 128; below, the error is under 2^-40 of that largest one, far less than a 32-bit sum with it loses.
+// With more rows that takes longer than it saves (0.7 us a row), and so do the scales of more sums: codes are expanded to BF16 with their
+// scales, X is read as it is, and the products add up through all of K.
 //
 // The consumer warps take the units of all steps in turn, each adding up its own of a step; two warps put these parts together, in
 // order, and write the outputs while the consumers go on.  Where X is too large for shared memory, K is walked in chunks: all steps of the CTA with
@@ -62,11 +66,18 @@ template <int MT_, int NT_, int kWarps_, int kFinishers_, int kPerSm_, int kDept
 struct MxRowsForm {
     static constexpr int MT = MT_, NT = NT_, kWarps = kWarps_, kFinishers = kFinishers_, kPerSm = kPerSm_, kDepth = kDepth_;
     static constexpr bool kGated = kGated_;
+    static constexpr bool kHalf = NT_ == 1;                                  // FP16 products
     static constexpr int kThreads = 32 * (kWarps_ + kFinishers_);
     static constexpr int kPart = MT * NT * 32;                               // float4s of a warp's part of a step
     static constexpr int kSum = (kGated ? 2 : MT) * NT * 32;                 // float4s of a step's sums
     static __host__ __device__ uint32_t row_bytes(int chunk_groups) { return static_cast<uint32_t>(chunk_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
 };
+
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 
 // byte j of a scale word as 2^(s - 127); the smallest scale, 2^-127, counts as zero here, 255 as infinity (its codes are zero)
 __device__ __forceinline__ float scale_of(uint32_t word, int j) {
@@ -255,28 +266,28 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             if (lane < A.rows) bulk_copy_g2s(base + lane * row_bytes, A.X + static_cast<int64_t>(lane) * A.W.K + c0 * kMxGroup, x_bytes, x_bar);
         }
         mx_wait(x_bar, c & 1, &dead, 10);
-        {
-            const int teams = threads / 16, ch = lane & 15;                  // half a warp takes a group of a row
-            const uint32_t half = 0xFFFFu << (lane & 16);
+        if constexpr (Form::kHalf) {
+            // to FP16 in place: chunk (group, block, quarter) is eight values, in the order of a word's nibbles; half a warp takes a group of a
+            // row, four of them at once
             constexpr int kAtOnce = 4;
-            const int jobs = groups * A.rows;
+            const int teams = threads / 16, ch = lane & 15, jobs = groups * A.rows, on = teams / A.rows, more = teams - on * A.rows;
+            const uint32_t half = 0xFFFFu << (lane & 16);
+            int xg = (tid >> 4) / A.rows, xr = (tid >> 4) - xg * A.rows;
             for (int job0 = tid >> 4; job0 < jobs; job0 += teams * kAtOnce) {
-                uint32_t w[kAtOnce][4], top[kAtOnce], at[kAtOnce], xs_at[kAtOnce];
+                uint32_t w[kAtOnce][4], top[kAtOnce], at_x[kAtOnce], at_s[kAtOnce];
 #pragma unroll
                 for (int q = 0; q < kAtOnce; q++) {
-                    const int job = min(job0 + q * teams, jobs - 1), gr = job / A.rows, r = job - gr * A.rows;
-                    at[q] = r * row_bytes + gr * 256 + ch * 16;
-                    xs_at[q] = gr * kCols + r;
+                    at_x[q] = xr * row_bytes + xg * 256 + ch * 16;
+                    at_s[q] = xg * kCols + xr;
                     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (gr * 256 + ch * 16 < x_bytes && job0 + q * teams < jobs) v = *reinterpret_cast<const uint4 *>(smem + at[q]);
+                    if (job0 + q * teams < jobs && xg * 256 + ch * 16 < x_bytes) v = *reinterpret_cast<const uint4 *>(smem + at_x[q]);
                     w[q][0] = v.x, w[q][1] = v.y, w[q][2] = v.z, w[q][3] = v.w;
-                    top[q] = 0u;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t lo = w[q][j] & 0x7FFFu, hi = (w[q][j] >> 16) & 0x7FFFu;
-                        top[q] = max(top[q], lo < 0x7F80u ? lo : 0u);        // infinities and NaNs keep themselves whatever the scale
-                        top[q] = max(top[q], hi < 0x7F80u ? hi : 0u);
-                    }
+                    // magnitudes as bits; an infinity or NaN makes the whole row one, whatever becomes of its other values
+                    const uint32_t m = max_bf16x2(max_bf16x2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), max_bf16x2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+                    top[q] = max(m & 0xFFFFu, m >> 16);
+                    xg += on;
+                    xr += more;
+                    if (xr >= A.rows) xr -= A.rows, xg++;
                 }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1)
@@ -295,10 +306,13 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                         const float lo = (j >> 1 ? bf16hi_to_f32(a) : bf16lo_to_f32(a)) * scale, hi = (j >> 1 ? bf16hi_to_f32(b) : bf16lo_to_f32(b)) * scale;
                         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[j]) : "f"(hi), "f"(lo));
                     }
-                    *reinterpret_cast<uint4 *>(smem + at[q]) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if (ch == 0) xscale[xs_at[q]] = __uint_as_float((254u - up) << 23);
+                    *reinterpret_cast<uint4 *>(smem + at_x[q]) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (ch == 0) xscale[at_s[q]] = __uint_as_float((254u - up) << 23);
                 }
             }
+        } else {
+            const int pad = groups * 256 - x_bytes;                          // past the last column: zeros
+            for (int i = tid * 16; i < A.rows * pad; i += threads * 16) *reinterpret_cast<uint4 *>(smem + i / pad * row_bytes + x_bytes + i % pad) = make_uint4(0u, 0u, 0u, 0u);
         }
         together();
 
@@ -310,7 +324,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
 #pragma unroll
                 for (int k = 0; k < 4; k++) acc[q][n][k] = 0.f;
         int gr = warp;
-        auto multiply = [&](int d) {
+        auto multiply_f16 = [&](int d) {
             float cg[MT][NT][4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -341,6 +355,41 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 for (int q = 0; q < MT; q++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) acc[q][n][k] = fmaf(cg[q][n][k], k & 1 ? xs.y : xs.x, acc[q][n][k]);
+            }
+        };
+        auto multiply_bf16 = [&](int d, auto large) {
+            constexpr bool kLarge = decltype(large)::value;
+            uint32_t fa[MT][4], fb[MT][4];
+#pragma unroll
+            for (int q = 0; q < MT; q++) {
+                mx_factors<kLarge>(sa[d][q], fa[q]);
+                mx_factors<kLarge>(sb[d][q], fb[q]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint4 x[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) x[n] = *reinterpret_cast<const uint4 *>(smem + xat[n] + gr * 256 + j * 64);
+#pragma unroll
+                for (int q = 0; q < MT; q++) {
+                    const uint4 a = mx_word_to_bf16<kLarge>(word_of(qa[d][q], j), fa[q][j]), b = mx_word_to_bf16<kLarge>(word_of(qb[d][q], j), fb[q][j]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma_bf16_16x8x16(acc[q][n], a.x, b.x, a.y, b.y, x[n].x, x[n].y);
+                        mma_bf16_16x8x16(acc[q][n], a.z, b.z, a.w, b.w, x[n].z, x[n].w);
+                    }
+                }
+            }
+        };
+        auto multiply = [&](int d) {
+            if constexpr (Form::kHalf) {
+                multiply_f16(d);
+            } else {
+                uint32_t any = 0u;
+#pragma unroll
+                for (int q = 0; q < MT; q++) any |= sa[d][q] | sb[d][q];
+                if (__any_sync(0xFFFFFFFFu, (any & 0x80808080u) != 0u)) multiply_bf16(d, std::true_type{});
+                else multiply_bf16(d, std::false_type{});
             }
             gr += A.consumers;
         };

@@ -9,13 +9,7 @@
 // Sixteen warps of a CTA turn codes into BF16, exactly (a code times a power of two fits), one thread requests B by TMA, one of the pair issues the
 // products, eight warps read the accumulators back.  The weight is expanded once for all rows of a
 // tile, so the expansion (19 instructions for eight values) stays behind the tensor cores from some 130 rows on.
-//
-// A code's bits s eem are moved to a BF16's sign, lowest exponent and highest mantissa bits: that is its value times 2^-126, the
-// subnormal code 0.5 included, and one product by 2^(126 + s - 127) makes both the value and its scale.  Scales above 2 (2^(126 + s - 127) would
-// overflow) take two products.
 #pragma once
-
-#include <type_traits>
 
 #include <cuda.h>      // CUtensorMap and the encode entry point's types; the driver library is not linked
 
@@ -116,36 +110,6 @@ __device__ __forceinline__ uint64_t mt_desc(uint32_t addr, uint32_t lbo) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lbo) << 16) | (static_cast<uint64_t>(64u) << 32) |
            (static_cast<uint64_t>(1u) << 46) | (static_cast<uint64_t>(2u) << 61);
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-// Eight codes as eight BF16 values in element order, times f (kLarge: times 2^126, then f).
-template <bool kLarge>
-__device__ __forceinline__ uint4 mx_word_to_bf16(uint32_t w, uint32_t f) {
-    constexpr uint32_t kMag = 0x01C001C0u, kSign = 0x80008000u;
-    uint32_t h[4];
-    h[0] = ((w << 6) & kMag) | ((w << 12) & kSign);
-    h[1] = ((w << 2) & kMag) | ((w << 8) & kSign);
-    h[2] = ((w >> 2) & kMag) | ((w << 4) & kSign);
-    h[3] = ((w >> 6) & kMag) | (w & kSign);
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = mul_bf16x2(kLarge ? mul_bf16x2(h[i], 0x7E807E80u) : h[i], f);
-    return make_uint4(h[0], h[1], h[2], h[3]);
-}
-// The factors of a row's four blocks: 2^(s - 1), or of large scales 2^(s - 127) (255: infinity, and its codes are zero).
-template <bool kLarge>
-__device__ __forceinline__ void mx_factors(uint32_t scales, uint32_t (&f)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t s = (scales >> (8 * j)) & 255u;
-        f[j] = kLarge ? (s == 0u ? 0x00400040u : s * 0x00800080u) : s * 0x00800080u + 0x3F003F00u;
-    }
-}
-__device__ __forceinline__ uint32_t word_of(const uint4 &q, int j) { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; }
-
 // ---- sums to outputs: a thread's lane of the accumulator is value p, columns are rows of out --------------------------------------------
 // Two warps have the same lanes and take 16 columns in turn.  kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16
 // columns the first eight become the gate lanes', the others the up lanes': each hands the other half over through shared memory.
