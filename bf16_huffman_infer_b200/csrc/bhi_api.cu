@@ -241,7 +241,7 @@ int bhi_debug_status(int *status_out) {
     BHI_REQUIRE(status_out, "null output");
     int v = 0;
     cudaError_t e = cudaDeviceSynchronize();
-    for (auto take : {take_gemv_huffman_status, take_gemv_ans_status, take_tiles_status}) {
+    for (auto take : {take_gemv_huffman_status, take_gemv_ans_status, take_tiles_status, take_mxfp4_rows_status, take_mxfp4_tile_status}) {
         int one = 0;
         if (e == cudaSuccess) e = take(&one);
         if (one) v = one;

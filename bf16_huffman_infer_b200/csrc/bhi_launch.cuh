@@ -20,5 +20,7 @@ int tileq_launch(const Layer &L, const typename Codec::Args &targs, const uint8_
 cudaError_t take_gemv_huffman_status(int *out);
 cudaError_t take_gemv_ans_status(int *out);
 cudaError_t take_tiles_status(int *out);
+cudaError_t take_mxfp4_rows_status(int *out);
+cudaError_t take_mxfp4_tile_status(int *out);
 
 }  // namespace bhi

@@ -215,7 +215,7 @@ int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, 
     if (int rc = mx_check(codes, scales, M, K)) return rc;
     BHI_REQUIRE(rows >= 1, "no rows");
     BHI_REQUIRE(X && Y && aligned(X, 16) && aligned(Y, 2) && aligned(bias, 2), "X must be 16-byte aligned");
-    if (rows <= 32) {
+    if (rows <= kMxRowsMost) {
         const int rc = mx_rows_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }
@@ -238,7 +238,7 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
     BHI_REQUIRE(X && H && aligned(X, 16) && aligned(H, 2) && aligned(bias, 2) && aligned(pre, 16), "X must be 16-byte aligned");
     const MxWeight W = mx_weight(codes, scales, 2 * inter, K);
-    if (rows <= 32) {
+    if (rows <= kMxRowsMost) {
         const int rc = mx_rows_launch(W, X, bias, H, true, activation, pre, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }

@@ -3,7 +3,7 @@
 // y[r][m] = sum over blocks b of 2^(s[m][b] - 127) * sum over the block's k of code[m][k] x[r][k], and with kGated the rows g and u of a
 // stacked weight at once, h = act(g) u.
 //
-// Bound by the bytes of the weight.  A consumer warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
+// Bound by the bytes of the weight.  A warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
 // They come straight from global memory into registers, kDepth units ahead, and are multiplied by m16n8k16 products.
 //
 // Up to eight rows of X the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32
@@ -13,16 +13,18 @@
 // With more rows that takes longer than it saves (0.7 us a row), and so do the scales of more sums: codes are expanded to BF16 with their
 // scales, X is read as it is, and the products add up through all of K.
 //
-// The consumer warps take the units of all steps in turn, each adding up its own of a step; two warps put these parts together, in
-// order, and write the outputs while the consumers go on.  Where X is too large for shared memory, K is walked in chunks: all steps of the CTA with
-// one chunk's X, then with the next, the sums of each step kept in shared memory.
+// The units of a CTA's steps, numbered through, are divided into one run for each warp: a step is one warp's but for those that the ends of
+// runs cut.  The warp with a cut step's beginning adds the parts of the warps after it, in order (they had them at the beginning of their runs)
+// and writes its outputs.  (With a step's groups dealt out to all warps, adding up fourteen parts a step took longer than the products
+// from 16 rows on, whichever warps did it.)  Where X is too large for shared memory, K is walked in chunks: all steps of the CTA with one
+// chunk's X, then with the next, the sums of each step kept in shared memory.
 #pragma once
 
 #include "bhi_mxfp4.cuh"
 
 namespace bhi {
 
-constexpr int kMxPartsMax = 4;                    // steps whose parts lie in shared memory
+constexpr int kMxRowWarpsMax = 16;
 
 struct MxRowsArgs {
     MxWeight W;
@@ -35,8 +37,6 @@ struct MxRowsArgs {
     // the launch's plan
     int steps;                                    // plain: of MT tiles; gated: of 16 outputs
     int chunk_groups;                             // groups whose X lies in shared memory at a time
-    int consumers;                                // warps that multiply, at most as many as a chunk has groups
-    int parts;
     uint32_t scale_off, part_off, sum_off;
 };
 
@@ -60,14 +60,15 @@ __device__ __forceinline__ uint32_t load_stream4(const uint8_t *p) {
     return v;
 }
 
-// A form of the kernel: MT tiles of weight rows by NT blocks of eight rows of X, up to kWarps multiplying warps, kDepth units in flight a
-// warp, kFinishers warps for the outputs, kPerSm CTAs an SM.
-template <int MT_, int NT_, int kWarps_, int kFinishers_, int kPerSm_, int kDepth_, bool kGated_>
+// A form of the kernel: MT tiles of weight rows by NT blocks of eight rows of X, kWarps warps, kDepth units in flight a warp, kPerSm CTAs an SM.
+template <int MT_, int NT_, int kWarps_, int kPerSm_, int kDepth_, bool kGated_>
 struct MxRowsForm {
-    static constexpr int MT = MT_, NT = NT_, kWarps = kWarps_, kFinishers = kFinishers_, kPerSm = kPerSm_, kDepth = kDepth_;
+    static constexpr int MT = MT_, NT = NT_, kWarps = kWarps_, kPerSm = kPerSm_, kDepth = kDepth_;
     static constexpr bool kGated = kGated_;
     static constexpr bool kHalf = NT_ == 1;                                  // FP16 products
-    static constexpr int kThreads = 32 * (kWarps_ + kFinishers_);
+    static constexpr int kThreads = 32 * kWarps_;
+    static constexpr int kPlaces = kDepth_ + 1;                              // of a warp: the steps that end in a turn of kDepth units, and a part for another warp
+    static_assert(kWarps <= kMxRowWarpsMax, "barriers");
     static constexpr int kPart = MT * NT * 32;                               // float4s of a warp's part of a step
     static constexpr int kSum = (kGated ? 2 : MT) * NT * 32;                 // float4s of a step's sums
     static __host__ __device__ uint32_t row_bytes(int chunk_groups) { return static_cast<uint32_t>(chunk_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
@@ -89,124 +90,58 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
     constexpr int MT = Form::MT, NT = Form::NT, kDepth = Form::kDepth, kCols = 8 * NT;
     constexpr bool kGated = Form::kGated;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * kMxPartsMax + 1];
+    __shared__ __align__(8) uint64_t bars[kMxRowWarpsMax + 1];
     __shared__ int dead;                                                     // a wait has run out: no other one waits any more
+    constexpr int kWarps = Form::kWarps, threads = Form::kThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int my_steps = (A.steps - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
     const int chunks = (A.W.groups + A.chunk_groups - 1) / A.chunk_groups;
     const uint32_t base = smem_addr(smem);
-    const uint32_t part_full = smem_addr(&bars[0]), part_empty = part_full + 8 * kMxPartsMax, x_bar = part_empty + 8 * kMxPartsMax;
+    const uint32_t part_bar = smem_addr(&bars[0]), x_bar = part_bar + 8 * kMxRowWarpsMax;
+    float4 *places = reinterpret_cast<float4 *>(smem + A.part_off), *sums = reinterpret_cast<float4 *>(smem + A.sum_off);
 
     pdl_launch_dependents();
     if (tid == 0) {
-        for (int i = 0; i < A.parts; i++) {
-            mbar_init(part_full + 8 * i, A.consumers);
-            mbar_init(part_empty + 8 * i, Form::kFinishers);
-        }
+        for (int i = 0; i < kWarps; i++) mbar_init(part_bar + 8 * i, 1);
         mbar_init(x_bar, 1);
         mbar_fence_init();
         dead = 0;
     }
     __syncthreads();
 
-    float4 *parts = reinterpret_cast<float4 *>(smem + A.part_off);
-    if (warp >= A.consumers) {
-        // ---- sums over the warps and chunks, outputs ------------------------------------------------------------------------
-        const int finisher = warp - A.consumers;
-        float4 *sums = reinterpret_cast<float4 *>(smem + A.sum_off);
-        const int stride = A.consumers * Form::kPart;                        // of the parts of a step
-        auto store = [&](int m, int col, float v, float u) {                 // u: of a gated pair
-            if (m >= A.outs || col >= A.rows) return;
-            const int64_t at = static_cast<int64_t>(col) * A.outs + m;
-            if (A.bias != nullptr) {
-                v += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m)) << 16);
-                if constexpr (kGated) u += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + A.outs + m)) << 16);
-            }
-            if constexpr (kGated) {
-                A.Y[at] = f32_to_bf16_rn(mx_act(A.activation, v) * u);
-                if (A.pre != nullptr) {
-                    A.pre[at + static_cast<int64_t>(col) * A.outs] = v;
-                    A.pre[at + static_cast<int64_t>(col + 1) * A.outs] = u;
-                }
-            } else {
-                A.Y[at] = f32_to_bf16_rn(v);
-            }
-        };
-        pdl_wait();                                                          // outputs may be what the previous kernel reads, a bias what it writes
-        int slot = 0;
-        uint32_t phase = 0u;
-        for (int c = 0; c < chunks; c++) {
-            for (int i = 0; i < my_steps; i++) {
-                const int step = blockIdx.x + i * gridDim.x;
-                mx_wait(part_full + 8 * slot, phase, &dead, 12);
-                const float4 *src = parts + slot * stride;
-                constexpr int kItems = kGated ? NT : MT * NT;
-                for (int item = finisher; item < kItems; item += Form::kFinishers) {
-                    const int at = item * 32 + lane, n = item % NT;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
-                    for (int w = 0; w < A.consumers; w++) {
-                        const float4 p = src[w * Form::kPart + at];
-                        v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
-                    }
-                    if constexpr (kGated) {
-                        // up rows lie (outs mod 16) rows further on in their tiles
-                        const int r0 = (A.outs & 15) + g, r1 = r0 + 8;
-                        auto half = [&](int r) { return (((1 + (r >> 4)) * NT + n) * 32 + (r & 7) * 4 + t) * 2 + ((r >> 3) & 1); };
-                        const int h0 = half(r0), h1 = half(r1);
-                        for (int w = 0; w < A.consumers; w++) {
-                            const float2 *s2 = reinterpret_cast<const float2 *>(src + w * Form::kPart);
-                            const float2 p = s2[h0], q = s2[h1];
-                            u.x += p.x, u.y += p.y, u.z += q.x, u.w += q.y;
-                        }
-                    }
-                    float4 *keep = sums + i * Form::kSum + at;
-                    if (c > 0) {
-                        const float4 p = *keep;
-                        v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
-                        if constexpr (kGated) {
-                            const float4 q = keep[NT * 32];
-                            u.x += q.x, u.y += q.y, u.z += q.z, u.w += q.w;
-                        }
-                    }
-                    if (c + 1 < chunks) {
-                        *keep = v;
-                        if constexpr (kGated) keep[NT * 32] = u;
-                        continue;
-                    }
-                    const int m = 16 * (kGated ? step : MT * step + item / NT) + g, col = 8 * n + 2 * t;
-                    store(m, col, v.x, u.x);
-                    store(m, col + 1, v.y, u.y);
-                    store(m + 8, col, v.z, u.z);
-                    store(m + 8, col + 1, v.w, u.w);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(part_empty + 8 * slot);
-                if (++slot == A.parts) slot = 0, phase ^= 1u;
-            }
+    auto store = [&](int m, int col, float v, float u) {                     // u: of a gated pair
+        if (m >= A.outs || col >= A.rows) return;
+        const int64_t at = static_cast<int64_t>(col) * A.outs + m;
+        if (A.bias != nullptr) {
+            v += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m)) << 16);
+            if constexpr (kGated) u += __uint_as_float(static_cast<uint32_t>(load_written(A.bias + A.outs + m)) << 16);
         }
-        return;
-    }
+        if constexpr (kGated) {
+            A.Y[at] = f32_to_bf16_rn(mx_act(A.activation, v) * u);
+            if (A.pre != nullptr) {
+                A.pre[at + static_cast<int64_t>(col) * A.outs] = v;
+                A.pre[at + static_cast<int64_t>(col + 1) * A.outs] = u;
+            }
+        } else {
+            A.Y[at] = f32_to_bf16_rn(v);
+        }
+    };
 
-    // ---- consumers ------------------------------------------------------------------------------------------------------------
     const uint32_t row_bytes = Form::row_bytes(A.chunk_groups);
     float *xscale = reinterpret_cast<float *>(smem + A.scale_off);
-    const int threads = 32 * A.consumers;
-    auto together = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
     uint32_t xat[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) xat[n] = static_cast<uint32_t>(min(8 * n + g, A.rows - 1)) * row_bytes + t * 16;
-    int part = 0;
-    uint32_t part_phase = 1u;
 
-
-    // ---- the warp's units of a chunk: (step, group) pairs numbered over all steps, every consumers-th one, kDepth ahead of their use -----
+    // ---- the warp's run of units of a chunk, (step, group) pairs, kDepth ahead of their use ------------------------------------------------
     uint4 qa[kDepth][MT], qb[kDepth][MT];
     uint32_t sa[kDepth][MT], sb[kDepth][MT];
     // Tiles of the step that is being requested, at the next group: 16-byte units of codes, bytes of scales (a pair's scales lie at
     // a sixteenth of its codes' offset; row b is eight rows on).
     const uint8_t *codes = A.W.codes + t * kMxQuarter + g * 16, *scales = A.W.scales + g * 4;
     uint32_t at[MT];
-    int ask_step, ask_group, asked, units;
+    int ask_step, ask_group, asked, run, units;
+    auto run_of = [&](int w, int groups) { return static_cast<int>(static_cast<int64_t>(my_steps) * groups * w / kWarps); };      // where warp w's begins
     auto tiles_of = [&](int c0) {
         const int step = blockIdx.x + ask_step * gridDim.x, last = (A.W.M - 1) >> 4;
 #pragma unroll
@@ -225,22 +160,22 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             sb[slot][q] = load_stream4(s + 32);
         }
         if (++asked < units) {
-            ask_group += A.consumers;
-            if (ask_group >= groups) {
-                ask_group -= groups;
+            if (++ask_group == groups) {
+                ask_group = 0;
                 ask_step++;
                 tiles_of(c0);
             } else {
 #pragma unroll
-                for (int q = 0; q < MT; q++) at[q] += A.consumers * (kMxTileCodes / 16);
+                for (int q = 0; q < MT; q++) at[q] += kMxTileCodes / 16;
             }
         }
     };
     auto begin_chunk = [&](int c0, int groups) {
-        ask_step = 0;
-        ask_group = warp;
+        run = run_of(warp, groups);
+        units = run_of(warp + 1, groups) - run;
+        ask_step = run / groups;
+        ask_group = run - ask_step * groups;
         asked = 0;
-        units = (my_steps * groups - warp + A.consumers - 1) / A.consumers;
         if (units > 0) {
             tiles_of(c0);
 #pragma unroll
@@ -257,7 +192,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
         if (c > 0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             begin_chunk(c0, groups);
-            together();                                                      // nobody reads the last chunk's X any more
+            __syncthreads();                                                      // nobody reads the last chunk's X any more
         }
         if (warp == 0) {
             if (c == 0) pdl_wait();
@@ -314,7 +249,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             const int pad = groups * 256 - x_bytes;                          // past the last column: zeros
             for (int i = tid * 16; i < A.rows * pad; i += threads * 16) *reinterpret_cast<uint4 *>(smem + i / pad * row_bytes + x_bytes + i % pad) = make_uint4(0u, 0u, 0u, 0u);
         }
-        together();
+        __syncthreads();
 
         float acc[MT][NT][4];
 #pragma unroll
@@ -323,7 +258,9 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) acc[q][n][k] = 0.f;
-        int gr = warp;
+        const int run_step = run / groups;                                   // the local step in which the run begins
+        int i = run_step, gr = run - i * groups, first = i;                  // step and group of the unit at hand; the first step not dealt with
+        const bool begun = gr == 0;                                          // the run begins with its step
         auto multiply_f16 = [&](int d) {
             float cg[MT][NT][4];
 #pragma unroll
@@ -391,12 +328,11 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 if (__any_sync(0xFFFFFFFFu, (any & 0x80808080u) != 0u)) multiply_bf16(d, std::true_type{});
                 else multiply_bf16(d, std::false_type{});
             }
-            gr += A.consumers;
+            gr++;
         };
-        auto end_of_step = [&]() {                                           // this warp's part of a step is complete
-            gr -= groups;
-            mx_wait(part_empty + 8 * part, part_phase, &dead, 14);
-            float4 *dst = parts + (part * A.consumers + warp) * Form::kPart + lane;
+        // the sums so far to one of this warp's places, and to zero
+        auto put = [&](int place) {
+            float4 *dst = places + (warp * Form::kPlaces + place) * Form::kPart + lane;
 #pragma unroll
             for (int q = 0; q < MT; q++)
 #pragma unroll
@@ -405,9 +341,76 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
 #pragma unroll
                     for (int k = 0; k < 4; k++) acc[q][n][k] = 0.f;
                 }
+        };
+        // Every warp once a chunk: its part of a step that another one began, if it has any, is in its last place.
+        auto hand_over = [&]() {
             __syncwarp();
-            if (lane == 0) mbar_arrive(part_full + 8 * part);
-            if (++part == A.parts) part = 0, part_phase ^= 1u;
+            if (lane == 0) mbar_arrive(part_bar + 8 * warp);
+        };
+        // the outputs of a step from one of this warp's places and the parts of the warps up to `others`
+        auto finish = [&](int local, int place, int others) {
+            const int step = blockIdx.x + local * gridDim.x;
+            const float4 *own = places + (warp * Form::kPlaces + place) * Form::kPart;
+            if (lane < others - warp) mx_wait(part_bar + 8 * (warp + 1 + lane), c & 1, &dead, 12);
+            __syncwarp();
+            const bool few = my_steps * groups < kWarps;                     // some runs are empty
+            constexpr int kItems = kGated ? NT : MT * NT, kUnroll = kItems == 1 && !kGated ? 4 : 1;       // (more code costs more than it hides)
+#pragma unroll 1
+            for (int item = 0; item < kItems; item++) {
+                const int at_v = item * 32 + lane, n = item % NT;
+                // up rows lie (outs mod 16) rows further on in their tiles
+                const int r0 = (A.outs & 15) + g, r1 = r0 + 8;
+                auto half = [&](int r) { return (((1 + (r >> 4)) * NT + n) * 32 + (r & 7) * 4 + t) * 2 + ((r >> 3) & 1); };
+                float4 v = own[at_v], u = make_float4(0.f, 0.f, 0.f, 0.f);
+                if constexpr (kGated) {
+                    const float2 p = reinterpret_cast<const float2 *>(own)[half(r0)], q = reinterpret_cast<const float2 *>(own)[half(r1)];
+                    u = make_float4(p.x, p.y, q.x, q.y);
+                }
+#pragma unroll(kUnroll)
+                for (int w = warp + 1; w <= others; w++) {
+                    if (few && run_of(w, groups) == run_of(w + 1, groups)) continue;
+                    const float4 *src = places + (w * Form::kPlaces + kDepth) * Form::kPart;
+                    const float4 p = src[at_v];
+                    v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+                    if constexpr (kGated) {
+                        const float2 a = reinterpret_cast<const float2 *>(src)[half(r0)], b = reinterpret_cast<const float2 *>(src)[half(r1)];
+                        u.x += a.x, u.y += a.y, u.z += b.x, u.w += b.y;
+                    }
+                }
+                float4 *keep = sums + local * Form::kSum + at_v;
+                if (c > 0) {
+                    const float4 p = *keep;
+                    v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+                    if constexpr (kGated) {
+                        const float4 q = keep[NT * 32];
+                        u.x += q.x, u.y += q.y, u.z += q.z, u.w += q.w;
+                    }
+                }
+                if (c + 1 < chunks) {
+                    *keep = v;
+                    if constexpr (kGated) keep[NT * 32] = u;
+                    continue;
+                }
+                const int m = 16 * (kGated ? step : MT * step + item / NT) + g, col = 8 * n + 2 * t;
+                store(m, col, v.x, u.x);
+                store(m, col + 1, v.y, u.y);
+                store(m + 8, col, v.z, u.z);
+                store(m + 8, col + 1, v.w, u.w);
+            }
+            __syncwarp();                                                    // every lane has read the place
+        };
+        bool handed = false;
+        auto end_of_step = [&]() {
+            gr = 0;
+            put(i == run_step && !begun ? kDepth : i - first);
+            i++;
+        };
+        auto finish_steps = [&]() {                                          // those that ended since the last time
+            __syncwarp();
+            for (int place = 0; first < i; first++, place++) {
+                if (first == run_step && !begun) hand_over(), handed = true;
+                else finish(first, place, warp);
+            }
         };
         int u = 0;
         for (; u + kDepth <= units; u += kDepth) {
@@ -415,15 +418,25 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             for (int d = 0; d < kDepth; d++) {
                 multiply(d);
                 request(d, c0, groups);
-                if (gr >= groups) end_of_step();
+                if (gr == groups) end_of_step();
             }
+            if (first < i) finish_steps();
         }
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
             if (u + d < units) {
                 multiply(d);
-                if (gr >= groups) end_of_step();
+                if (gr == groups) end_of_step();
             }
+        }
+        if (first < i) finish_steps();
+        int others = warp;
+        const bool cut = gr != 0 && units > 0, mine = i > run_step || begun;       // the run ends inside a step; which this warp began
+        if (cut) put(mine ? 0 : kDepth);
+        if (!handed) hand_over();
+        if (cut && mine) {
+            while (others + 1 < kWarps && run_of(others + 1, groups) < (i + 1) * groups) others++;
+            finish(i, 0, others);
         }
     }
 }

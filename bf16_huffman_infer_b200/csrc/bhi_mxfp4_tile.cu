@@ -1,5 +1,4 @@
 // The products of 4-bit microscaled weights in tiles: plans and launches.
-#include <cstdlib>
 #include "bhi_mxfp4_tile.cuh"
 
 namespace bhi {
@@ -25,19 +24,30 @@ EncodeTiledFn encode_tiled() {
 
 enum Kind { kPlain, kGatedPair, kGradient };
 
-// Rows of a tile (a multiple of 32): the fewest rounds of tiles over the pairs of SMs times what a tile costs, by its rows: measured (4096
-// columns, ns for 128 of them) 425 + 0.85 rows forward, twice (395 + 0.55 rows) for a gradient; an accumulator on its own (above 128 rows, forward)
-// keeps the products waiting while it is read.
-int rows_of_tile(int rows, int pairs_p, int groups, bool gradient) {
-    int best = 32;
+// Rows of a tile (a multiple of 32), and into how many parts c is cut (one, two or four pairs of SMs share a tile): the fewest rounds of tiles over
+// the pairs of SMs times what a tile costs, by its rows: measured (4096 columns, ns for 128 of them) 425 + 0.85 rows forward, twice (395 + 0.55
+// rows) for a gradient.  An accumulator on its own (above 128 rows, forward) keeps the products waiting while it is read; parts take
+// kJoin ns for their sums' way through shared memory, and run in one round only: of clusters of eight CTAs two fit on a GPC.
+struct TilePlan {
+    int nt = 32, splits = 1;
+};
+constexpr double kJoin = 2500;
+TilePlan tile_plan(int rows, int pairs_p, int groups, bool gradient) {
+    TilePlan best;
     double best_cost = 1e30;
+    const int pairs = sm_count() / 2;
     for (int nt = 32; nt <= kMtRows; nt += 32) {
-        const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p, pairs = sm_count() / 2;
-        const double tile = gradient ? groups * 2 * (395 + 0.55 * nt) : groups * (425 + 0.85 * nt) + (nt > kMtTwoRows ? 6.0 * nt : 0.0);
-        const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * tile + 1e-3 * nt;
-        if (cost < best_cost - 1e-9) {
-            best_cost = cost;
-            best = nt;
+        const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p;
+        const double group = gradient ? 2 * (395 + 0.55 * nt) : 425 + 0.85 * nt;
+        for (int s = 1; s <= 4; s *= 2) {
+            if (s > 1 && (tiles * s > (s == 4 ? pairs * 3 / 4 : pairs * 6 / 7) || groups < 2 * s)) break;
+            const double rounds = static_cast<double>((tiles + pairs - 1) / pairs);
+            const double tile = (groups + s - 1) / s * group + (s == 1 ? nt > kMtTwoRows && !gradient ? 6.0 * nt : 0.0 : kJoin);
+            if (rounds * tile + 1e-3 * nt < best_cost - 1e-9) {
+                best_cost = rounds * tile + 1e-3 * nt;
+                best.nt = nt;
+                best.splits = s;
+            }
         }
         if (nt >= rows) break;
     }
@@ -50,11 +60,15 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     if (!encode) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     const int per = kKind == kGatedPair ? 64 : 128;
     a.pairs_p = (a.outs + 2 * per - 1) / (2 * per);
-    a.nt = rows_of_tile(a.rows, a.pairs_p, static_cast<int>((b_cols + 127) / 128), kKind == kGradient);
-    if (getenv("MXN")) a.nt = atoi(getenv("MXN"));
+    const TilePlan plan = tile_plan(a.rows, a.pairs_p, static_cast<int>((b_cols + 127) / 128), kKind == kGradient);
+    a.nt = plan.nt;
+    a.splits = plan.splits;
     a.tiles_n = (a.rows + a.nt - 1) / a.nt;
     a.buffers = kKind == kGradient || a.nt <= kMtTwoRows ? 2 : 1;
     a.boxes_c = static_cast<int>((b_cols + kMtBox - 1) / kMtBox);
+    const int whole = kKind == kGradient ? 1 : 2, units = (a.boxes_c + whole - 1) / whole;      // a group forward
+    a.split_boxes = (units + a.splits - 1) / a.splits * whole;
+    if (a.split_boxes * (a.splits - 1) >= a.boxes_c) a.splits = 1, a.split_boxes = a.boxes_c;
     BHI_REQUIRE(static_cast<int64_t>(a.pairs_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
     const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 64u : static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;
     a.stages = static_cast<int>((kSmemTile - extra) / stage);
@@ -78,13 +92,13 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     const int tiles = a.pairs_p * a.tiles_n;
     cudaLaunchConfig_t cfg = {};
     const int pairs = sm_count() / 2;
-    cfg.gridDim = dim3(2 * (tiles < pairs ? tiles : pairs));
+    cfg.gridDim = dim3(2 * a.splits * (tiles < pairs ? tiles : pairs));
     cfg.blockDim = dim3(kMtThreads);
     cfg.dynamicSmemBytes = a.stages * stage + extra;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * a.splits;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
