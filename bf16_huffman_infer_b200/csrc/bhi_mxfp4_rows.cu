@@ -15,7 +15,7 @@ constexpr int kChunksMax = 8;
 
 template <class Form>
 int launch(MxRowsArgs a, cudaStream_t st) {
-    constexpr int per = Form::kGated ? 16 : 16 * Form::MT;
+    constexpr int per = Form::kGated ? 8 : 16 * Form::MT;
     a.steps = (a.outs + per - 1) / per;
     const int groups = a.W.groups, grid = std::min(a.steps, sm_count() * Form::kPerSm), most_steps = (a.steps + grid - 1) / grid;
     // as few chunks of K as shared memory takes
@@ -24,7 +24,7 @@ int launch(MxRowsArgs a, cudaStream_t st) {
         a.scale_off = static_cast<uint32_t>(a.rows) * Form::row_bytes(a.chunk_groups);
         a.part_off = a.scale_off + (Form::kHalf ? static_cast<uint32_t>(a.chunk_groups) * 8 * Form::NT * 4 : 0u);
         a.sum_off = a.part_off + Form::kWarps * Form::kPlaces * Form::kPart * 16u;
-        const uint64_t bytes = a.sum_off + (chunks > 1 ? static_cast<uint64_t>(most_steps) * Form::kSum * 16u : 0u);
+        const uint64_t bytes = a.sum_off + (chunks > 1 ? static_cast<uint64_t>(most_steps) * Form::kPart * 16u : 0u);
         if (bytes > (Form::kPerSm == 2 ? kSmemHalf : kSmemRows)) continue;
         auto kernel = mx_rows_kernel<Form>;
         if (int rc = staged_prepare(kernel, kSmemRows)) return rc;
@@ -51,8 +51,12 @@ int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, u
     if (rows > kMxRowsMost || static_cast<int64_t>((W.M + 15) / 16) * W.groups * (kMxTileCodes / 16) > UINT32_MAX) return kStagedDeclined;
     MxRowsArgs a{};
     a.W = W, a.X = X, a.bias = bias, a.Y = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
-    if (gated && a.outs % 16 == 0) return rows <= 8 ? launch<MxRowsForm<2, 1, 16, 1, 2, true>>(a, st) : launch<MxRowsForm<2, 2, 16, 1, 2, true>>(a, st);
-    if (gated) return rows <= 8 ? launch<MxRowsForm<3, 1, 16, 1, 1, true>>(a, st) : launch<MxRowsForm<3, 2, 16, 1, 1, true>>(a, st);      // ups lie across two tiles each
+    if (gated && rows > 8) return launch<MxRowsForm<1, 2, 16, 1, 4, true>>(a, st);
+    if (gated) {
+        // as below; from five rows on one CTA an SM, which brings and converts X once (18944 x 3584, 8 rows 20.2 against 22.5 us)
+        const int rc = rows <= 4 ? launch<MxRowsForm<1, 1, 8, 2, 3, true>>(a, st) : kStagedDeclined;
+        return rc != kStagedDeclined ? rc : launch<MxRowsForm<1, 1, 16, 1, 3, true>>(a, st);
+    }
     if (rows > 8) return launch<MxRowsForm<1, 2, 16, 1, 4, false>>(a, st);
     // Two CTAs an SM, so that the next kernel's are there as soon as one of them ends, where X leaves them room; two tiles a step share X's
     // fragments (151936 x 4096, 8 rows 65.7 against 72 us) where every CTA has four steps of them (37984 x 4096 either way 24).

@@ -1,7 +1,7 @@
 // Products of 4-bit microscaled weights with few rows of X.
 //
 // y[r][m] = sum over blocks b of 2^(s[m][b] - 127) * sum over the block's k of code[m][k] x[r][k], and with kGated the rows g and u of a
-// stacked weight at once, h = act(g) u.
+// stacked weight at once, h = act(g) u: the 16 rows of a product are then the gates and ups of eight outputs, so that a lane has both.
 //
 // Bound by the bytes of the weight.  A warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
 // They come straight from global memory into registers, kDepth units ahead, and are multiplied by m16n8k16 products.
@@ -35,7 +35,7 @@ struct MxRowsArgs {
     int outs;                                     // M, or inter of a gated pair
     int activation;
     // the launch's plan
-    int steps;                                    // plain: of MT tiles; gated: of 16 outputs
+    int steps;                                    // plain: of MT tiles; gated: of 8 outputs
     int chunk_groups;                             // groups whose X lies in shared memory at a time
     uint32_t scale_off, part_off, sum_off;
 };
@@ -70,7 +70,7 @@ struct MxRowsForm {
     static constexpr int kPlaces = kDepth_ + 1;                              // of a warp: the steps that end in a turn of kDepth units, and a part for another warp
     static_assert(kWarps <= kMxRowWarpsMax, "barriers");
     static constexpr int kPart = MT * NT * 32;                               // float4s of a warp's part of a step
-    static constexpr int kSum = (kGated ? 2 : MT) * NT * 32;                 // float4s of a step's sums
+    static_assert(!kGated || MT == 1, "a gated step is one tile");
     static __host__ __device__ uint32_t row_bytes(int chunk_groups) { return static_cast<uint32_t>(chunk_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
 };
 
@@ -78,11 +78,6 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
-}
-
-// byte j of a scale word as 2^(s - 127); the smallest scale, 2^-127, counts as zero here, 255 as infinity (its codes are zero)
-__device__ __forceinline__ float scale_of(uint32_t word, int j) {
-    return __uint_as_float((j < 3 ? word << (23 - 8 * j) : word >> 1) & 0x7F800000u);
 }
 
 template <class Form>
@@ -136,28 +131,37 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
     // ---- the warp's run of units of a chunk, (step, group) pairs, kDepth ahead of their use ------------------------------------------------
     uint4 qa[kDepth][MT], qb[kDepth][MT];
     uint32_t sa[kDepth][MT], sb[kDepth][MT];
-    // Tiles of the step that is being requested, at the next group: 16-byte units of codes, bytes of scales (a pair's scales lie at
-    // a sixteenth of its codes' offset; row b is eight rows on).
-    const uint8_t *codes = A.W.codes + t * kMxQuarter + g * 16, *scales = A.W.scales + g * 4;
-    uint32_t at[MT];
+    // Rows a and b (eight on, or an output's up) of the step that is being requested, at the next group: 16-byte units of the codes of their
+    // (tile, group) pairs, which are also bytes of the scales, and rows in their tiles.
+    const uint8_t *codes = A.W.codes + t * kMxQuarter, *scales = A.W.scales;
+    constexpr int kRows = kGated ? 2 : MT;                                   // different (tile, group) pairs of a unit
+    uint32_t at[kRows];
+    int ra = g, rb = g + 8;
     int ask_step, ask_group, asked, run, units;
     auto run_of = [&](int w, int groups) { return static_cast<int>(static_cast<int64_t>(my_steps) * groups * w / kWarps); };      // where warp w's begins
     auto tiles_of = [&](int c0) {
-        const int step = blockIdx.x + ask_step * gridDim.x, last = (A.W.M - 1) >> 4;
+        const int step = blockIdx.x + ask_step * gridDim.x;
+        if constexpr (kGated) {                                              // past the last output (of the padded weight all the same): nobody reads the results
+            const int ma = 8 * step + g, mb = A.outs + ma;
+            at[0] = (static_cast<uint32_t>(ma >> 4) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16);
+            at[1] = (static_cast<uint32_t>(mb >> 4) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16);
+            ra = ma & 15;
+            rb = mb & 15;
+        } else {                                                             // past the last tile: the last one
 #pragma unroll
-        for (int q = 0; q < MT; q++) {                                       // a tile past the end: the last one, nobody reads its results
-            const int tile = kGated ? (q == 0 ? step : (A.outs >> 4) + step + q - 1) : MT * step + q;
-            at[q] = (static_cast<uint32_t>(min(tile, last)) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16);
+            for (int q = 0; q < MT; q++)
+                at[q] = (static_cast<uint32_t>(min(MT * step + q, (A.W.M - 1) >> 4)) * A.W.groups + c0 + ask_group) * (kMxTileCodes / 16);
         }
     };
     auto request = [&](int slot, int c0, int groups) {                       // past the last unit: the last one again, without effect
 #pragma unroll
         for (int q = 0; q < MT; q++) {
-            const uint8_t *p = codes + static_cast<uint64_t>(at[q]) * 16, *s = scales + at[q];
-            qa[slot][q] = load_stream16(p);
-            qb[slot][q] = load_stream16(p + 128);
-            sa[slot][q] = load_stream4(s);
-            sb[slot][q] = load_stream4(s + 32);
+            const uint32_t pa = at[q], pb = at[kGated ? 1 : q];
+            const uint8_t *a = codes + static_cast<uint64_t>(pa) * 16 + ra * 16, *b = kGated ? codes + static_cast<uint64_t>(pb) * 16 + rb * 16 : a + 128;
+            qa[slot][q] = load_stream16(a);
+            qb[slot][q] = load_stream16(b);
+            sa[slot][q] = load_stream4(scales + pa + ra * 4);
+            sb[slot][q] = load_stream4(scales + pb + rb * 4);
         }
         if (++asked < units) {
             if (++ask_group == groups) {
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 tiles_of(c0);
             } else {
 #pragma unroll
-                for (int q = 0; q < MT; q++) at[q] += kMxTileCodes / 16;
+                for (int q = 0; q < kRows; q++) at[q] += kMxTileCodes / 16;
             }
         }
     };
@@ -262,6 +266,12 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
         int i = run_step, gr = run - i * groups, first = i;                  // step and group of the unit at hand; the first step not dealt with
         const bool begun = gr == 0;                                          // the run begins with its step
         auto multiply_f16 = [&](int d) {
+            uint32_t pa[MT][2], pb[MT][2];                                   // the blocks' scales in BF16
+#pragma unroll
+            for (int q = 0; q < MT; q++) {
+                mx_scales_bf16(sa[d][q], pa[q]);
+                mx_scales_bf16(sb[d][q], pb[q]);
+            }
             float cg[MT][NT][4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -274,7 +284,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                     uint32_t ha[4], hb[4];
                     mx_word_to_f16(j == 0 ? wa.x : j == 1 ? wa.y : j == 2 ? wa.z : wa.w, ha);
                     mx_word_to_f16(j == 0 ? wb.x : j == 1 ? wb.y : j == 2 ? wb.z : wb.w, hb);
-                    const float fa = scale_of(sa[d][q], j), fb = scale_of(sb[d][q], j);
+                    const float fa = j & 1 ? bf16hi_to_f32(pa[q][j >> 1]) : bf16lo_to_f32(pa[q][j >> 1]), fb = j & 1 ? bf16hi_to_f32(pb[q][j >> 1]) : bf16lo_to_f32(pb[q][j >> 1]);
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         float e[4];
@@ -354,48 +364,37 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             if (lane < others - warp) mx_wait(part_bar + 8 * (warp + 1 + lane), c & 1, &dead, 12);
             __syncwarp();
             const bool few = my_steps * groups < kWarps;                     // some runs are empty
-            constexpr int kItems = kGated ? NT : MT * NT, kUnroll = kItems == 1 && !kGated ? 4 : 1;       // (more code costs more than it hides)
+            constexpr int kItems = MT * NT, kUnroll = kItems == 1 ? 4 : 1;   // (more code costs more than it hides)
 #pragma unroll 1
             for (int item = 0; item < kItems; item++) {
                 const int at_v = item * 32 + lane, n = item % NT;
-                // up rows lie (outs mod 16) rows further on in their tiles
-                const int r0 = (A.outs & 15) + g, r1 = r0 + 8;
-                auto half = [&](int r) { return (((1 + (r >> 4)) * NT + n) * 32 + (r & 7) * 4 + t) * 2 + ((r >> 3) & 1); };
-                float4 v = own[at_v], u = make_float4(0.f, 0.f, 0.f, 0.f);
-                if constexpr (kGated) {
-                    const float2 p = reinterpret_cast<const float2 *>(own)[half(r0)], q = reinterpret_cast<const float2 *>(own)[half(r1)];
-                    u = make_float4(p.x, p.y, q.x, q.y);
-                }
+                float4 v = own[at_v];
 #pragma unroll(kUnroll)
                 for (int w = warp + 1; w <= others; w++) {
                     if (few && run_of(w, groups) == run_of(w + 1, groups)) continue;
-                    const float4 *src = places + (w * Form::kPlaces + kDepth) * Form::kPart;
-                    const float4 p = src[at_v];
+                    const float4 p = places[(w * Form::kPlaces + kDepth) * Form::kPart + at_v];
                     v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
-                    if constexpr (kGated) {
-                        const float2 a = reinterpret_cast<const float2 *>(src)[half(r0)], b = reinterpret_cast<const float2 *>(src)[half(r1)];
-                        u.x += a.x, u.y += a.y, u.z += b.x, u.w += b.y;
-                    }
                 }
-                float4 *keep = sums + local * Form::kSum + at_v;
+                float4 *keep = sums + local * Form::kPart + at_v;
                 if (c > 0) {
                     const float4 p = *keep;
                     v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
-                    if constexpr (kGated) {
-                        const float4 q = keep[NT * 32];
-                        u.x += q.x, u.y += q.y, u.z += q.z, u.w += q.w;
-                    }
                 }
                 if (c + 1 < chunks) {
                     *keep = v;
-                    if constexpr (kGated) keep[NT * 32] = u;
                     continue;
                 }
-                const int m = 16 * (kGated ? step : MT * step + item / NT) + g, col = 8 * n + 2 * t;
-                store(m, col, v.x, u.x);
-                store(m, col + 1, v.y, u.y);
-                store(m + 8, col, v.z, u.z);
-                store(m + 8, col + 1, v.w, u.w);
+                const int col = 8 * n + 2 * t;
+                if constexpr (kGated) {
+                    store(8 * step + g, col, v.x, v.z);
+                    store(8 * step + g, col + 1, v.y, v.w);
+                } else {
+                    const int m = 16 * (MT * step + item / NT) + g;
+                    store(m, col, v.x, 0.f);
+                    store(m, col + 1, v.y, 0.f);
+                    store(m + 8, col, v.z, 0.f);
+                    store(m + 8, col + 1, v.w, 0.f);
+                }
             }
             __syncwarp();                                                    // every lane has read the place
         };
