@@ -7,7 +7,7 @@ There is no CPU or non-CUDA code path: importing the package loads the native li
 fails if they have not been built (``python bf16_huffman_infer_b200/_build.py``).
 """
 from .functional import *  # noqa: F401,F403
-from .mxfp4 import GatedMXFP4, MXFP4Weight, gated_mxfp4, linear_mxfp4  # noqa: F401
+from .mxfp4 import GatedMLP, GatedMXFP4, MXFP4Weight, gated_mxfp4, linear_mxfp4  # noqa: F401
 from .functional import mv_ans, mv_huffman  # noqa: F401
 from .cudagraph_utils import get_graphed_model  # noqa: F401
 from .utils import get_model_size  # noqa: F401

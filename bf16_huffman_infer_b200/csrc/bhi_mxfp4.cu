@@ -213,7 +213,7 @@ int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, u
 int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *X, const uint16_t *bias, uint16_t *Y, int rows,
                      void *stream) {
     if (int rc = mx_check(codes, scales, M, K)) return rc;
-    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(rows >= 1 && rows <= BHI_MXFP4_MAX_ROWS, "bad number of rows");
     BHI_REQUIRE(X && Y && aligned(X, 16) && aligned(Y, 2) && aligned(bias, 2), "X must be 16-byte aligned");
     if (rows <= kMxRowsMost) {
         const int rc = mx_rows_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
@@ -224,7 +224,7 @@ int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, 
 
 int bhi_mxfp4_linear_grad(const uint8_t *codes, const uint8_t *scales, int M, int K, const uint16_t *dY, int ldy, uint16_t *dX, int rows, void *stream) {
     if (int rc = mx_check(codes, scales, M, K)) return rc;
-    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(rows >= 1 && rows <= BHI_MXFP4_MAX_ROWS, "bad number of rows");
     BHI_REQUIRE(ldy >= M && ldy % 8 == 0, "rows of dY must be a multiple of 8 values apart");
     BHI_REQUIRE(dY && dX && aligned(dY, 16) && aligned(dX, 16), "dY and dX must be 16-byte aligned");
     return mx_grad_launch(mx_weight(codes, scales, M, K), dY, ldy, dX, rows, static_cast<cudaStream_t>(stream));
@@ -234,7 +234,7 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
                     float *pre, int rows, void *stream) {
     BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2, "bad number of gated outputs");
     if (int rc = mx_check(codes, scales, 2 * inter, K)) return rc;
-    BHI_REQUIRE(rows >= 1, "no rows");
+    BHI_REQUIRE(rows >= 1 && rows <= BHI_MXFP4_MAX_ROWS, "bad number of rows");
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
     BHI_REQUIRE(X && H && aligned(X, 16) && aligned(H, 2) && aligned(bias, 2) && aligned(pre, 16), "X must be 16-byte aligned");
     const MxWeight W = mx_weight(codes, scales, 2 * inter, K);
@@ -246,7 +246,7 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
 }
 
 int bhi_mxfp4_gated_grad(const float *pre, const uint16_t *dH, int inter, int activation, uint16_t *dpre, int ldp, int rows, void *stream) {
-    BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2 && rows >= 1, "empty gradient");
+    BHI_REQUIRE(inter >= 1 && inter <= BHI_MXFP4_MAX_DIM / 2 && rows >= 1 && rows <= BHI_MXFP4_MAX_ROWS, "bad size of a gated gradient");
     BHI_REQUIRE(pre && dH && dpre && aligned(pre, 16) && aligned(dH, 2) && aligned(dpre, 16) && ldp >= 2 * inter && ldp % 4 == 0, "bad gradient buffers");
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -143,7 +143,10 @@ __device__ __forceinline__ void mx_word_to_f32(uint32_t w, float scale, float (&
 // act(g) = g s(g) and act'(g), in 32 bits.  s is a logistic function (silu: of g; gelu's tanh form: of 2 z, since
 // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)), which does not cancel for negative z) or half of erfc(-g / sqrt 2).  The fast exponential
 // and division are off by a few units of 2^-23 here: far below the one rounding to BF16 that follows.
-__device__ __forceinline__ float mx_logistic(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+__device__ __forceinline__ float mx_logistic(float v) {
+    const float e = __expf(-fabsf(v));                                       // at most 1, and the tail of negative v keeps its digits
+    return __fdividef(v < 0.f ? e : 1.f, 1.f + e);
+}
 
 __device__ __forceinline__ void mx_act_grad(int act, float g, float &a, float &da) {
     if (act == BHI_ACT_SILU) {
@@ -158,7 +161,7 @@ __device__ __forceinline__ void mx_act_grad(int act, float g, float &a, float &d
         const float g2 = g * g;
         const float s = mx_logistic(1.59576912160573071f * (g + 0.044715f * g2 * g));
         a = g * s;
-        da = s + a * (1.f - s) * 1.59576912160573071f * (1.f + 0.134145f * g2);
+        da = s + a * (1.f - s) * 1.59576912160573071f * (1.f + 0.134145f * fminf(g2, 1e4f));      // beyond, a (1 - s) is zero, or would be times infinity
     }
 }
 __device__ __forceinline__ float mx_act(int act, float g) {

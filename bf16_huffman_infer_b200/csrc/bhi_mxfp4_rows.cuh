@@ -9,7 +9,9 @@
 // Up to eight rows of X the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32
 // columns start at zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared
 // memory: each row's 128 values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to
-// 2^-32 of the largest in its 128; below, the error is under 2^-40 of that largest one, far less than a 32-bit sum with it loses.
+// 2^-31 of the largest in its 128; below, the error is at most 2^-39 of that largest one, far less than a 32-bit sum with it loses.  With X's
+// power of two, up to 2^23 in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are not
+// finite are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
 // With more rows that takes longer than it saves (0.7 us a row), and so do the scales of more sums: codes are expanded to BF16 with their
 // scales, X is read as it is, and the products add up through all of K.
 //
@@ -78,6 +80,22 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
+}
+
+// One output by itself: weight row m, row `col` of X, products in 32 bits.
+__device__ __forceinline__ float mx_one_output(const MxRowsArgs &A, int m, int col) {
+    const uint8_t *codes = A.W.codes + mx_code_row(m, A.W.groups), *scales = A.W.scales + mx_scale_row(m, A.W.groups);
+    const uint16_t *x = A.X + static_cast<int64_t>(col) * A.W.K;
+    float sum = 0.f;
+    for (int k = 0; k < A.W.K; k += 8) {
+        const int g = k >> 7, j = (k >> 5) & 3, t = (k >> 3) & 3;
+        float v[8];
+        mx_word_to_f32(*reinterpret_cast<const uint32_t *>(codes + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4),
+                       mx_scale(scales[static_cast<int64_t>(g) * kMxTileScales + j]), v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum = fmaf(v[i], __uint_as_float(static_cast<uint32_t>(load_written(x + k + i)) << 16), sum);
+    }
+    return sum;
 }
 
 template <class Form>
@@ -385,6 +403,21 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                     continue;
                 }
                 const int col = 8 * n + 2 * t;
+                if constexpr (Form::kHalf) {
+                    const bool even = !(isfinite(v.x) && isfinite(v.z)), odd = !(isfinite(v.y) && isfinite(v.w));
+                    if ((even && col < A.rows) || (odd && col + 1 < A.rows)) {
+                        const int ma = kGated ? 8 * step + g : 16 * (MT * step + item / NT) + g, mb = kGated ? A.outs + ma : ma + 8;
+#pragma unroll 1
+                        for (int k = 0; k < 4; k++) {
+                            if (!(k & 1 ? odd : even) || col + (k & 1) >= A.rows || (kGated ? ma : k < 2 ? ma : mb) >= A.outs) continue;
+                            const float one = mx_one_output(A, k < 2 ? ma : mb, col + (k & 1));
+                            if (k == 0) v.x = one;
+                            if (k == 1) v.y = one;
+                            if (k == 2) v.z = one;
+                            if (k == 3) v.w = one;
+                        }
+                    }
+                }
                 if constexpr (kGated) {
                     store(8 * step + g, col, v.x, v.z);
                     store(8 * step + g, col + 1, v.y, v.w);

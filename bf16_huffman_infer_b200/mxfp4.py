@@ -195,7 +195,7 @@ def _linear_backward(ctx, dy: Tensor):
     if ctx.needs_input_grad[0]:
         dx = _LinearGradient.apply(dy, ctx.held) if _recorded(dy, None) or _transformed() else _input_gradient(dy, ctx.held.weight)
     if ctx.needs_input_grad[2]:
-        db = dy.flatten(0, -2).sum(0, dtype=torch.float32).to(dy.dtype)
+        db = dy.sum(tuple(range(dy.dim() - 1)), dtype=torch.float32).to(dy.dtype) if dy.dim() > 1 else dy
     return dx, None, db
 
 

@@ -286,8 +286,10 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
  *                               nibble i (from the lowest) element 2 i, nibble 4 + i element 2 i + 1
  *   scales  u8 [T, G, 16, 4]      byte s of each block: 2^(s - 127); 255 is NaN (its codes must be zero)
  *
- * Padding must be zeros; bhi_mxfp4_quantize writes it.  Sums are 32-bit floats, each output is rounded to BF16 once. */
+ * Padding must be zeros; bhi_mxfp4_quantize writes it.  Sums are 32-bit floats, each output is rounded to BF16 once.  Up to
+ * BHI_MXFP4_MAX_ROWS rows of X, dY and the like. */
 #define BHI_MXFP4_MAX_DIM (1 << 24)
+#define BHI_MXFP4_MAX_ROWS (1 << 30)
 #define BHI_DTYPE_BF16 0
 #define BHI_DTYPE_FP16 1
 #define BHI_DTYPE_FP32 2
@@ -296,7 +298,8 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
 #define BHI_ACT_GELU_TANH 2    /* its approximation by tanh */
 
 /* W [M, K] of the named type, rows contiguous, to codes and scales: e = max(floor(log2 max|v|) - 2, -127), codes of v / 2^e
- * rounded to the nearest (ties to even), saturated at 6; a block with an infinity or NaN becomes NaN.  The products may follow on the same stream, launch overlap or not. */
+ * rounded to the nearest (ties to even), saturated at 6; a block with an infinity or NaN becomes NaN.  The products may
+ * follow on the same stream, with launch overlap or without. */
 int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
 
 /* Y bf16 [M, K]: the values (exact but for scales beyond BF16's range). */

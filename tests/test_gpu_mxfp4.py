@@ -4,11 +4,14 @@ Tolerances.  A BF16 output is the exact value rounded once: off by at most 2^-8 
 of the outputs' (the sums' own errors are far below that for the inputs here).  A single output may also be off by its 32-bit sum:
 K additions that lose at most 2^-23 each of the sum of the terms' magnitudes.  A gradient through the gated pair is
 rounded twice (the projections' gradients, which feed the product, and the result): 2^-7."""
+import ctypes
 import math
 
 import pytest
 import torch
 import torch.nn.functional as F
+
+from _util import Abi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -179,6 +182,50 @@ def test_infinities_and_nans_in_x(pkg, rows):
         assert torch.equal(y[2:], clean[2:])
 
 
+@pytest.mark.parametrize("byte", [0, 1, 30, 126, 127, 128, 200, 231, 232, 240, 251, 252])
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 33, 200])
+def test_scales_of_the_whole_range(pkg, rows, byte):
+    """One scale throughout, from the smallest to the largest whose values are finite, and X the other way: products near one."""
+    g = torch.Generator().manual_seed(rows + byte)
+    M, K = 150, 416
+    codes = torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, generator=g)
+    w = pkg.MXFP4Weight.from_packed(codes.to(DEV), torch.full((M, K // 32), byte, dtype=torch.uint8, device=DEV))
+    dense = w.get_weight().double()
+    grid = torch.cat([GRID, -GRID])
+    assert torch.equal(dense.cpu(), torch.ldexp(torch.stack([grid[(codes & 15).long()], grid[(codes >> 4).long()]], -1).view(M, K), torch.tensor(byte - 127)))
+    x = torch.ldexp(torch.randn(rows, K, generator=g).double(), torch.tensor(min(127 - byte, 120))).to(torch.bfloat16).to(DEV)
+    want, mag = x.double() @ dense.T, x.double().abs() @ dense.abs().T
+    # and half of BF16's and the products' smallest steps, for terms that are below
+    assert bool(((F.linear(x, w).double() - want).abs() <= want.abs() * 2.0 ** -8 + mag * (K * 2.0 ** -23) + K * 2.0 ** -134).all())
+    gate, up = want.chunk(2, -1)
+    gate_mag, up_mag = mag.chunk(2, -1)
+    # the sums' errors as above, through |act'| <= 1.1; the function's own error, a few units of 2^-23 of arguments up to 60 (where it is not small)
+    slack = 1.1 * gate_mag * K * 2.0 ** -23 * (up.abs() + up_mag * K * 2.0 ** -23) + act64(gate, "silu").abs() * up_mag * K * 2.0 ** -23
+    want = act64(gate, "silu") * up
+    assert bool(((pkg.gated_mxfp4(x, w).double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -14) + slack + 2.0 ** -100).all())
+
+
+@pytest.mark.parametrize("rows", [1, 8])
+def test_sums_that_overflow(pkg, rows):
+    """Few rows: outputs beyond the range are infinities of their sign, their neighbours (the other rows, the bias) are what they were."""
+    M, K = 40, 4096
+    g = torch.Generator().manual_seed(rows)
+    codes = torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, generator=g)
+    scales = torch.full((M, K // 32), 120, dtype=torch.uint8)
+    scales[::2, 40] = 250
+    codes[::2, 40 * 16:41 * 16] = 0x11                           # 0.5 2^123 throughout a block
+    w = pkg.MXFP4Weight.from_packed(codes.to(DEV), scales.to(DEV))
+    x = torch.randn(rows, K, generator=g).to(torch.bfloat16)
+    x[:, 40 * 32:41 * 32] = torch.tensor([2.0, -2.0] * rows).to(x.dtype)[:rows, None]      # 32 2^123 = 2^128
+    x = x.to(DEV)
+    y, bias = F.linear(x, w), normal(M, seed=3)
+    assert torch.equal(y[:, ::2], torch.where(x[:, 40 * 32, None] > 0, math.inf, -math.inf).to(y.dtype).expand(rows, M // 2))
+    dense = w.get_weight().double()[1::2]
+    mag = x.double().abs() @ dense.abs().T
+    assert bool(((y[:, 1::2].double() - x.double() @ dense.T).abs() <= (x.double() @ dense.T).abs() * 2.0 ** -8 + mag * (K * 2.0 ** -23)).all())
+    assert torch.equal(F.linear(x, w, bias)[:, ::2], y[:, ::2])
+
+
 def test_refused_calls(pkg):
     w, _ = made(pkg, 64, 128)
     x = normal(2, 128)
@@ -197,6 +244,15 @@ def test_refused_calls(pkg):
     odd, _ = made(pkg, 63, 128)
     with pytest.raises(RuntimeError):
         pkg.gated_mxfp4(x, odd)
+    ops, pre = pkg.ops, torch.empty(2, 64, device=DEV)
+    for bad in (lambda: ops.forward_mxfp4(x, w.codes[:3], w.scales, 64, None), lambda: ops.forward_mxfp4(x, w.codes, w.scales, 65, None),
+                lambda: ops.forward_mxfp4(x, w.codes, w.scales, 64, bias[1:]), lambda: ops.forward_mxfp4(x.T, w.codes, w.scales, 64, None),
+                lambda: ops.forward_mxfp4(x.view(-1)[1:129], w.codes, w.scales, 64, None), lambda: ops.mxfp4_quantize(x, w.codes, w.scales),
+                lambda: ops.mxfp4_linear_grad(x[:, :60].contiguous(), w.codes, w.scales, 64, 128), lambda: ops.dense_mxfp4(w.codes, w.scales, 64, 100),
+                lambda: ops.gated_mxfp4(x, w.codes, w.scales, 64, None, 3, None), lambda: ops.gated_mxfp4(x, w.codes, w.scales, 64, None, 0, pre[:1]),
+                lambda: ops.mxfp4_gated_grad(pre, x, 0), lambda: ops.mxfp4_gated_grad(pre, x[:, :32].contiguous(), -1)):
+        with pytest.raises(RuntimeError):
+            bad()
 
 
 # ---- its gradient --------------------------------------------------------------------------------------------------------
@@ -245,6 +301,21 @@ def test_gradients_of_views_and_broadcasts(pkg):
     e = x.new_empty(0, 256).requires_grad_()
     F.linear(e, w).sum().backward()
     assert e.grad.shape == (0, 256)
+
+
+def test_gradients_of_one_vector(pkg):
+    w, dense = made(pkg, 72, 256)
+    x, bias, dy = normal(256, seed=2), normal(72, seed=3), normal(72, seed=4)
+    leaf, b = x.clone().requires_grad_(), bias.clone().requires_grad_()
+    y = F.linear(leaf, w, b)
+    assert torch.equal(y.detach(), F.linear(x[None], w, bias)[0])
+    dx, db = torch.autograd.grad(y, (leaf, b), dy)
+    assert torch.equal(db, dy) and close(dx, dy.double() @ dense, dy.double().abs() @ dense.abs(), 72)
+    h = pkg.gated_mxfp4(leaf, w, b)
+    dx, db = torch.autograd.grad(h, (leaf, b), dy[:36])
+    many, bs = x[None].clone().requires_grad_(), bias.clone().requires_grad_()
+    want = torch.autograd.grad(pkg.gated_mxfp4(many, w, bs), (many, bs), dy[None, :36])
+    assert torch.equal(dx, want[0][0]) and torch.equal(db, want[1])
 
 
 def test_other_derivatives(pkg):
@@ -334,6 +405,50 @@ def test_gated_far_from_zero(pkg, rows, activation):
     assert bool(pkg.gated_mxfp4(far, w, bias, activation).isfinite().all())
 
 
+def plain_activation(g, name):
+    """act(g) and act'(g) in 64 bits, without cancellation for negative g."""
+    if name == "gelu":
+        s, ds = torch.special.erfc(-g / math.sqrt(2)) / 2, torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    else:
+        k = 2 * math.sqrt(2 / math.pi)
+        z, dz = (g, torch.ones_like(g)) if name == "silu" else (k * (g + 0.044715 * g ** 3), k * (1 + 3 * 0.044715 * g * g))
+        s = torch.sigmoid(z)
+        ds = s * torch.sigmoid(-z) * dz
+    return g * s, s + g * ds
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_tails_of_the_activations(pkg, activation):
+    """Where the exponential leaves the range of normal numbers, value by value."""
+    lo = {"silu": -102.0, "gelu": -13.0, "gelu_tanh": -9.9}[activation]
+    gates = torch.linspace(lo, 0, 97).to(torch.bfloat16)
+    K = 32
+    w = pkg.MXFP4Weight.from_packed(torch.tensor([[2] + [0] * 15, [32] + [0] * 15], dtype=torch.uint8, device=DEV),      # the first element, the second
+                                    torch.full((2, 1), 127, dtype=torch.uint8, device=DEV))
+    x = torch.zeros(97, K, dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = gates, 1
+    want = plain_activation(gates.double(), activation)[0].to(DEV)
+    few = torch.cat([pkg.gated_mxfp4(x[i:i + 8].to(DEV), w, None, activation) for i in range(0, 97, 8)])[:, 0].double()
+    many = pkg.gated_mxfp4(x.to(DEV), w, None, activation)[:, 0].double()
+    for got in (few, many):
+        # a rounding (half a step of 2^-133 for the smallest); arguments up to 102 with a few units of 2^-24 of their own; a 32-bit exponential in steps of
+        # 2^-149, times a gate up to 102
+        assert bool(((got - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -14) + 2.0 ** -134 + 2.0 ** -141).all()), (got, want)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("inter", [64, 65])
+def test_gradient_of_the_activations(pkg, inter, activation):
+    g = torch.cat([torch.linspace(-30, 30, 2 * inter - 6), torch.tensor([-1e30, -1e20, -1e5, 1e5, 1e20, 1e30])]).view(2, inter).to(DEV)
+    u, dh = normal(2, inter, seed=1, dtype=torch.float32), normal(2, inter, seed=2)
+    dpre = pkg.ops.mxfp4_gated_grad(torch.cat([g, u], 1), dh, {"silu": 0, "gelu": 1, "gelu_tanh": 2}[activation])[:, :2 * inter].double()
+    a, da = plain_activation(g.double(), activation)
+    da = torch.where(g.abs() > 1e4, (g > 0).double(), da)         # the formula's limits, where it leaves 64 bits
+    for got, want in ((dpre[:, :inter], dh.double() * u.double() * da), (dpre[:, inter:], dh.double() * a)):
+        # a rounding; act' in 32 bits: terms up to 1.6 (9, gelu_tanh's inner derivative times g (1 - s)) with a few units of 2^-23, arguments up to 30
+        assert bool(((got - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -14) + (dh.double() * u.double()).abs() * 2.0 ** -14 + 1e-30).all())
+
+
 def test_gated_layouts_and_empties(pkg):
     w, dense = made(pkg, 80, 256, std=0.1)
     x = normal(2, 3, 256)
@@ -396,6 +511,45 @@ def test_captured_and_on_two_streams(pkg):
         torch.cuda.synchronize()
         for _, x, y, _ in graphs:
             assert torch.equal(y, block(block(x)))
+
+
+def test_backward_in_a_graph(pkg):
+    """A whole training step of a block's products captured, on another stream, and replayed on new inputs."""
+    up, _ = made(pkg, 2 * 96, 256, seed=1, std=0.09)
+    down, _ = made(pkg, 256, 96, seed=2, std=0.1)
+
+    def step(x, dy):
+        leaf = x.detach().requires_grad_()
+        return torch.autograd.grad(F.linear(pkg.gated_mxfp4(leaf, up), down), leaf, dy)[0]
+
+    for rows in (3, 150):
+        x, dy = normal(rows, 256, seed=rows), normal(rows, 256, seed=rows + 1)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = step(x, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dx = step(x, dy)
+        graph.replay()
+        assert torch.equal(dx, eager)
+        x.copy_(normal(rows, 256, seed=7))
+        dy.copy_(normal(rows, 256, seed=8))
+        graph.replay()
+        assert torch.equal(dx, step(x, dy))
+
+
+def test_no_wait_ran_out(pkg):
+    """After products of every kind the kernels' status is clean."""
+    abi, status = Abi(), ctypes.c_int(-1)
+    abi.check(abi.lib.bhi_debug_status(ctypes.byref(status)))    # what earlier calls left
+    w, _ = made(pkg, 600, 2048)
+    for rows in (1, 8, 16, 17, 100, 400):
+        x = normal(rows, 2048).requires_grad_()
+        (F.linear(x, w).sum() + pkg.gated_mxfp4(x, w).sum()).backward()
+    abi.check(abi.lib.bhi_debug_status(ctypes.byref(status)))
+    assert status.value == 0
 
 
 def test_results_are_whole_for_the_next_kernel(pkg):

@@ -1,8 +1,11 @@
 """4-bit microscaled weights on the host: the order in memory and what is refused."""
+import ctypes
+
 import pytest
 import torch
 import torch.nn.functional as F
 
+from _util import LIB
 from bf16_huffman_infer_b200 import GatedMXFP4, MXFP4Weight, gated_mxfp4, linear_mxfp4, ops
 
 GRID = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6])
@@ -104,6 +107,37 @@ def test_operator_schemas():
         "mxfp4_gated_grad": "(Tensor pre, Tensor dH, int activation) -> Tensor",
     }.items():
         assert str(getattr(ns, name).default._schema) == f"bf16_huffman_infer::{name}{sig}"
+
+
+def test_refusals_of_the_library():
+    """The C entry points look at sizes, pointers and types before they touch a device."""
+    lib = ctypes.CDLL(LIB)
+    lib.bhi_last_error.restype = ctypes.c_char_p
+    p, odd, none, n = ctypes.c_void_p(256), ctypes.c_void_p(264), ctypes.c_void_p(0), ctypes.c_int
+    most, refused = (1 << 24) + 32, 1
+    weights = [(none, p, 16, 128), (p, none, 16, 128), (odd, p, 16, 128), (p, odd, 16, 128), (p, p, 0, 128), (p, p, 16, 0), (p, p, 16, 48), (p, p, most, 128), (p, p, 16, most)]
+    for c, s, M, K in weights:
+        assert lib.bhi_mxfp4_quantize(p, n(0), n(M), n(K), c, s, none) == refused
+        assert lib.bhi_mxfp4_dense(c, s, n(M), n(K), p, none) == refused
+        assert lib.bhi_mxfp4_linear(c, s, n(M), n(K), p, none, p, n(1), none) == refused
+        assert lib.bhi_mxfp4_linear_grad(c, s, n(M), n(K), p, n(max(M, 8) // 8 * 8), p, n(1), none) == refused
+        assert lib.bhi_mxfp4_gated(c, s, n(M // 2), n(K), p, none, n(0), p, none, n(1), none) == refused
+    assert lib.bhi_mxfp4_quantize(odd, n(0), n(16), n(128), p, p, none) == refused
+    assert lib.bhi_mxfp4_quantize(p, n(3), n(16), n(128), p, p, none) == refused
+    assert lib.bhi_mxfp4_dense(p, p, n(16), n(128), odd, none) == refused
+    for x, y, rows in [(none, p, 1), (odd, p, 1), (p, none, 1), (p, p, 0), (p, p, -1), (p, p, (1 << 30) + 1)]:
+        assert lib.bhi_mxfp4_linear(p, p, n(16), n(128), x, none, y, n(rows), none) == refused
+        assert lib.bhi_mxfp4_linear_grad(p, p, n(16), n(128), x, n(16), y, n(rows), none) == refused
+        assert lib.bhi_mxfp4_gated(p, p, n(8), n(128), x, none, n(0), y, none, n(rows), none) == refused
+    for ld in (8, 17, 20):
+        assert lib.bhi_mxfp4_linear_grad(p, p, n(16), n(128), p, n(ld), p, n(1), none) == refused
+    for act in (-1, 3):
+        assert lib.bhi_mxfp4_gated(p, p, n(8), n(128), p, none, n(act), p, none, n(1), none) == refused
+        assert lib.bhi_mxfp4_gated_grad(p, p, n(8), n(act), p, n(16), n(1), none) == refused
+    for pre, dh, out, inter, ld, rows in [(none, p, p, 8, 16, 1), (p, none, p, 8, 16, 1), (p, p, none, 8, 16, 1), (odd, p, p, 8, 16, 1), (p, p, p, 0, 16, 1),
+                                          (p, p, p, 8, 12, 1), (p, p, p, 8, 18, 1), (p, p, p, 8, 16, 0), (p, p, p, 8, 16, (1 << 30) + 1)]:
+        assert lib.bhi_mxfp4_gated_grad(pre, dh, n(inter), n(0), out, n(ld), n(rows), none) == refused
+    assert lib.bhi_last_error()
 
 
 def test_rows_of_a_weight():
