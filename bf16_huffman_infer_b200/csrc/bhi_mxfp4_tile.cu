@@ -70,10 +70,12 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     a.split_boxes = (units + a.splits - 1) / a.splits * whole;
     if (a.split_boxes * (a.splits - 1) >= a.boxes_c) a.splits = 1, a.split_boxes = a.boxes_c;
     BHI_REQUIRE(static_cast<int64_t>(a.pairs_p) * a.tiles_n <= INT32_MAX / 2, "too many tiles");
-    const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 64u : static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGatedPair ? kMtSwap : 0u;
+    const uint32_t stage = kKind == kGradient ? kMtABytes + static_cast<uint32_t>(a.nt) * 64u : static_cast<uint32_t>(a.nt) * 128u, extra = kKind == kGradient ? 0u : static_cast<uint32_t>(a.nt) * 512u;      // sums
     a.stages = static_cast<int>((kSmemTile - extra) / stage);
     if (a.stages > kMtStagesMax) a.stages = kMtStagesMax;
     if (kKind == kGradient) a.stages &= ~1;          // a slot is always the same team's
+    const int vec = kKind == kGatedPair ? 2 : 4;
+    a.wide = a.outs % vec == 0 && aligned(a.out, 2 * vec);
     alignas(64) CUtensorMap map;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(b_cols), static_cast<cuuint64_t>(a.rows)}, strides[1] = {static_cast<cuuint64_t>(ldb) * 2};
     const cuuint32_t box[2] = {kMtBox, static_cast<cuuint32_t>(a.nt / 2)}, estr[2] = {1, 1};

@@ -25,7 +25,6 @@ constexpr int kMtThreads = 32 * (kMtConverter + 2 * kMtTeam);
 constexpr int kMtBox = 64;                        // values of c a TMA box
 constexpr uint32_t kMtABytes = 128 * kMtBox * 2;
 constexpr int kMtStagesMax = 16;
-constexpr uint32_t kMtSwap = 2 * 16 * 64 * 4;         // bytes through which a gated block changes lanes
 constexpr int kMtRows = 256;                      // most rows of a tile
 constexpr int kMtTwoRows = 128;                   // forward: most rows of a tile with two accumulators
 
@@ -39,6 +38,7 @@ struct MxTileArgs {
     int nt, pairs_p, tiles_n, boxes_c;            // rows of a tile (a multiple of 32), pairs of tiles along p, tiles along n, boxes of 64 values of c
     int stages;                                   // of the ring
     int buffers;                                  // accumulators
+    bool wide;                                    // rows of out (and of pre) are whole aligned vectors of a lane's outputs
     int splits, split_boxes;                      // pairs of CTAs that share a tile's c, and the boxes of each
 };
 
@@ -64,12 +64,13 @@ __device__ __forceinline__ void mt_store8(uint32_t to, const uint4 &a, const uin
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"r"(to), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void mt_load(uint32_t from, float (&v)[N]) {
-    static_assert(N == 16, "one width");
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
-                   "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+__device__ __forceinline__ void mt_load(uint32_t from, float (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                   "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+                   "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                  : "r"(from));
 }
 // Whether a phase is over, without waiting: asked for the next stage before this one's products are issued, so that the answer costs no time.
@@ -129,137 +130,188 @@ __device__ __forceinline__ uint64_t mt_desc(uint32_t addr, uint32_t lbo) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lbo) << 16) | (static_cast<uint64_t>(64u) << 32) |
            (static_cast<uint64_t>(1u) << 46) | (static_cast<uint64_t>(2u) << 61);
 }
-// ---- sums to outputs: a thread's lane of the accumulator is value p, columns are rows of out --------------------------------------------
-// Two warps have the same lanes and take 16 columns in turn.  kGated: lanes 0 .. 63 are gates and 64 .. 127 the ups of the same outputs; of 16
-// columns the first eight become the gate lanes', the others the up lanes': each hands the other half over through shared memory.
-template <bool kGated>
-__device__ __forceinline__ void mt_store(const MxTileArgs &A, int64_t row, int m, float v, float u) {      // bias added; u: of a gated pair
-    A.out[row * A.outs + m] = f32_to_bf16_rn(kGated ? mx_act(A.activation, v) * u : v);
-}
-__device__ __forceinline__ float mt_bias(const MxTileArgs &A, int m, bool up, bool live) {
-    if (A.bias == nullptr || !live) return 0.f;
-    return __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m + (up ? A.outs : 0))) << 16);
+// ---- sums to outputs ----------------------------------------------------------------------------------------------------------------------
+// A thread's lane of the accumulator is value p, columns are rows of out.  Eight warps read it: two have the same lanes and take 32 columns in
+// turn.
+__device__ __forceinline__ void mt_free(const MtPart &P, uint32_t free_, int lane) {       // this warp's columns are read: the issuer may have them back
+    mt_fence_before();
+    __syncwarp();
+    if (lane == 0) mt_arrive(free_, P);
 }
 
-template <bool kGated, int kBuffer>
-__device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, const MtPart &P, uint32_t tmem, uint32_t done, uint32_t free_, float *swap, int *dead, int warp, int lane) {
-    const int quarter = warp & 3, half = (warp - kMtEpilogue) >> 2, lane_p = quarter * 32 + lane;
+// Gradient: straight from the accumulator, while the products go on in the other one.
+__device__ __forceinline__ void mt_epilogue(const MxTileArgs &A, const MtPart &P, uint32_t tmem, uint32_t done, uint32_t free_, int *dead, int warp, int lane) {
+    const int quarter = warp & 3, half = (warp - kMtEpilogue) >> 2;
     int buf = 0;
     uint32_t phase = 0u;
-    swap += half * (kMtSwap / 8);
-    auto read = [&]() {                                                      // this warp's columns are read: the issuer may have them back
-        mt_fence_before();
-        __syncwarp();
-        if (lane == 0) mt_arrive(free_ + 8 * buf, P);
-    };
-    pdl_wait();                                                              // outputs may be what the previous kernel reads, a bias what it writes
+    pdl_wait();                                                              // outputs may be what the previous kernel reads
     for (int tile = P.tile0; tile < P.tiles; tile += P.step) {
-        const int p = 2 * (tile % A.pairs_p) + P.half, n0 = tile / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0);
-        const int m = kGated ? 64 * p + (lane_p & 63) : 128 * p + lane_p;
-        const bool up = kGated && lane_p >= 64, live = m < A.outs;
-        const float bias = mt_bias(A, m, up, live);
+        const int n0 = tile / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0), m = 128 * (2 * (tile % A.pairs_p) + static_cast<int>(P.half)) + quarter * 32 + lane;
+        const bool live = m < A.outs;
         mx_wait(done + 8 * buf, phase, dead, 24);
         mt_fence_after();
-        const uint32_t from = tmem + buf * kBuffer + (static_cast<uint32_t>(quarter) << 21);
-        if (16 * half >= cols) read();
-        for (int c = 16 * half; c < cols; c += 32) {
-            float v[16];
+        const uint32_t from = tmem + buf * kMtRows + (static_cast<uint32_t>(quarter) << 21);
+        if (32 * half >= cols) mt_free(P, free_ + 8 * buf, lane);
+        for (int c = 32 * half; c < cols; c += 64) {
+            float v[32];
             mt_load(from + c, v);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (c + 32 >= cols) read();
+            if (c + 64 >= cols) mt_free(P, free_ + 8 * buf, lane);
+            if (!live) continue;
+            uint16_t *to = A.out + static_cast<int64_t>(n0 + c) * A.outs + m;
+            if (c + 32 <= cols) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] += bias;
-            if constexpr (!kGated) {
-                if (live) {
-                    uint16_t *to = A.out + static_cast<int64_t>(n0 + c) * A.outs + m;
-                    if (c + 16 <= cols) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++, to += A.outs) *to = f32_to_bf16_rn(v[i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i++, to += A.outs)
-                            if (c + i < cols) *to = f32_to_bf16_rn(v[i]);
-                    }
-                }
+                for (int i = 0; i < 32; i++, to += A.outs) *to = f32_to_bf16_rn(v[i]);
             } else {
-                if (A.pre != nullptr && live) {
-                    float *to = A.pre + static_cast<int64_t>(n0 + c) * 2 * A.outs + m + (up ? A.outs : 0);
 #pragma unroll
-                    for (int i = 0; i < 16; i++, to += 2 * static_cast<int64_t>(A.outs))
-                        if (c + i < cols) *to = v[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) swap[((up ? 0 : 8) + i) * 64 + (lane_p & 63)] = up ? v[i] : v[8 + i];
-                asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-                const int i0 = up ? 8 : 0;
-                if (live) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float other = swap[(i0 + i) * 64 + (lane_p & 63)];
-                        if (c + i0 + i < cols) mt_store<true>(A, n0 + c + i0 + i, m, up ? other : v[i], up ? v[8 + i] : other);
-                    }
-                }
-                asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+                for (int i = 0; i < 32; i++, to += A.outs)
+                    if (c + i < cols) *to = f32_to_bf16_rn(v[i]);
             }
         }
         if (++buf == A.buffers) buf = 0, phase ^= 1u;
     }
 }
 
-// Where several pairs share the tile's c (one tile a cluster): the sums go to shared memory as [column][lane], and after a barrier of the cluster each
-// pair puts every splits-th column together, in the pairs' order.
-__device__ __forceinline__ void mt_spill(const MxTileArgs &A, uint32_t tmem, uint32_t done, float *sums, int *dead, int warp, int lane) {
+// Forward, and where several pairs share the tile's c: the sums first go to shared memory as [column][lane], 128 KB for 256 rows in some 0.6 us, and the
+// products go on while outputs are made of them, whole vectors a lane.  (Read straight from a lone accumulator, the next tile's products waited
+// for all stores: gated 12288 x 4096, 2048 rows 310 against 257 us, with the projections kept 354 against 275.)
+__device__ __forceinline__ void mt_spill(const MxTileArgs &A, uint32_t from, int cols, float *sums, int warp, int lane) {
     const int quarter = warp & 3, half = (warp - kMtEpilogue) >> 2;
-    mx_wait(done, 0u, dead, 24);
-    mt_fence_after();
-    for (int c = 16 * half; c < A.nt; c += 32) {
-        float v[16];
-        mt_load(tmem + c + (static_cast<uint32_t>(quarter) << 21), v);
+    for (int c = 32 * half; c < cols; c += 64) {
+        float v[32];
+        mt_load(from + c + (static_cast<uint32_t>(quarter) << 21), v);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 16; i++) sums[(c + i) * 128 + quarter * 32 + lane] = v[i];
+        for (int i = 0; i < 32; i++) sums[(c + i) * 128 + quarter * 32 + lane] = v[i];
     }
 }
-template <bool kGated>
-__device__ __forceinline__ void mt_join(const MxTileArgs &A, const MtPart &P, const float *sums, int warp, int lane) {
-    const int w = warp - kMtEpilogue, p = 2 * (P.tile0 % A.pairs_p) + P.half, n0 = P.tile0 / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0);
-    constexpr int kBlocks = kGated ? 2 : 4, kAtOnce = 8;                     // blocks of 32 lanes with outputs; columns that are under way together
-    const int lane_p = w % kBlocks * 32 + lane, m = (kGated ? 64 : 128) * p + lane_p;
-    const bool live = m < A.outs;
-    const float bias = mt_bias(A, m, false, live), bias_up = kGated ? mt_bias(A, m, true, live) : 0.f;
-    const int first = (w / kBlocks) * A.splits + P.pair, stride = 8 / kBlocks * A.splits;
-    for (int c0 = first; c0 < cols; c0 += kAtOnce * stride) {
-        float v[kAtOnce] = {}, u[kAtOnce] = {};
-        for (int q = 0; q < A.splits; q++) {
-            const uint32_t from = mt_peer(smem_addr(sums) + lane_p * 4, 2u * q + P.half);
-            float x[kAtOnce], y[kAtOnce];
+
+__device__ __forceinline__ void mt_load_shared(const float *from, float (&v)[4]) {
+    const float4 q = *reinterpret_cast<const float4 *>(from);
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+}
+__device__ __forceinline__ void mt_load_shared(const float *from, float (&v)[2]) {
+    const float2 q = *reinterpret_cast<const float2 *>(from);
+    v[0] = q.x, v[1] = q.y;
+}
+__device__ __forceinline__ void mt_load_cluster(uint32_t from, float (&v)[4]) {
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from) : "memory");
+}
+__device__ __forceinline__ void mt_load_cluster(uint32_t from, float (&v)[2]) {
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(from) : "memory");
+}
+
+// Outputs from the sums in shared memory.  A warp takes a whole column, a lane four neighbours of it (gated: two gates, lanes 0 .. 63 of the
+// accumulator, and their ups, lanes 64 .. 127).  kJoin: every pair takes each splits-th column and adds up the pairs' sums, in their order.
+template <bool kGated, bool kJoin>
+__device__ __forceinline__ void mt_outputs(const MxTileArgs &A, const MtPart &P, int tile, const float *sums, int warp, int lane) {
+    constexpr int V = kGated ? 2 : 4, kAtOnce = 2;                           // columns that are under way together
+    const int p = 2 * (tile % A.pairs_p) + static_cast<int>(P.half), n0 = tile / A.pairs_p * A.nt, cols = min(A.nt, A.rows - n0);
+    const int m = (kGated ? 64 : 128) * p + V * lane, live = min(V, A.outs - m);
+    float bias[V] = {}, bias_up[V] = {};
+    if (A.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {                              // past the last column: some other one, not stored
-                const uint32_t at = from + min(c0 + i * stride, cols - 1) * 512;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[i]) : "r"(at) : "memory");
-                if constexpr (kGated) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[i]) : "r"(at + 256) : "memory");
-            }
-#pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                v[i] += x[i];
-                if constexpr (kGated) u[i] += y[i];
-            }
+        for (int i = 0; i < V; i++) {
+            if (i >= live) break;
+            bias[i] = __uint_as_float(static_cast<uint32_t>(load_written(A.bias + m + i)) << 16);
+            if (kGated) bias_up[i] = __uint_as_float(static_cast<uint32_t>(load_written(A.bias + A.outs + m + i)) << 16);
         }
-        if (!live) continue;
+    }
+    const int splits = kJoin ? A.splits : 1, stride = 8 * splits;
+    for (int c0 = (warp - kMtEpilogue) * splits + (kJoin ? static_cast<int>(P.pair) : 0); c0 < cols; c0 += kAtOnce * stride) {
+        float v[kAtOnce][V], u[kAtOnce][V];
+        const float *own = sums + V * lane;
+        for (int q = 0; q < splits; q++) {
+            float x[kAtOnce][V], y[kAtOnce][V];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {                              // past the last column: that one, not stored
+                const int at = min(c0 + i * stride, cols - 1) * 128;
+                if constexpr (kJoin) {
+                    const uint32_t from = mt_peer(smem_addr(own + at), 2u * q + P.half);
+                    mt_load_cluster(from, x[i]);
+                    if constexpr (kGated) mt_load_cluster(from + 256, y[i]);
+                } else {
+                    mt_load_shared(own + at, x[i]);
+                    if constexpr (kGated) mt_load_shared(own + at + 64, y[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    v[i][j] = q == 0 ? x[i][j] : v[i][j] + x[i][j];
+                    if constexpr (kGated) u[i][j] = q == 0 ? y[i][j] : u[i][j] + y[i][j];
+                }
+        }
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
             const int col = c0 + i * stride;
             if (col >= cols) break;
-            v[i] += bias;
-            u[i] += bias_up;
-            if (kGated && A.pre != nullptr) {
-                float *to = A.pre + static_cast<int64_t>(n0 + col) * 2 * A.outs + m;
-                to[0] = v[i];
-                to[A.outs] = u[i];
+            const int64_t row = n0 + col;
+            float h[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                v[i][j] += bias[j];
+                if constexpr (kGated) u[i][j] += bias_up[j];
+                h[j] = kGated ? mx_act(A.activation, v[i][j]) * u[i][j] : v[i][j];
             }
-            mt_store<kGated>(A, n0 + col, m, v[i], u[i]);
+            uint16_t *to = A.out + row * A.outs + m;
+            float *pre = kGated && A.pre != nullptr ? A.pre + row * 2 * A.outs + m : nullptr;
+            if (A.wide) {                                                    // whole vectors: all of it lives, or nothing
+                if (live <= 0) continue;
+                if constexpr (kGated) {
+                    *reinterpret_cast<uint32_t *>(to) = pack_bf16(h[0], h[1]);
+                    if (pre != nullptr) {
+                        *reinterpret_cast<float2 *>(pre) = make_float2(v[i][0], v[i][1]);
+                        *reinterpret_cast<float2 *>(pre + A.outs) = make_float2(u[i][0], u[i][1]);
+                    }
+                } else {
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    if (j >= live) break;
+                    to[j] = f32_to_bf16_rn(h[j]);
+                    if (pre != nullptr) pre[j] = v[i][j], pre[A.outs + j] = kGated ? u[i][j] : 0.f;
+                }
+            }
         }
     }
+}
+
+__device__ __forceinline__ void mt_epilogue_barrier() { asm volatile("bar.sync 2, 256;" ::: "memory"); }
+
+// Every tile of the pair, whose c is its own.
+template <bool kGated>
+__device__ __forceinline__ void mt_epilogue_staged(const MxTileArgs &A, const MtPart &P, uint32_t tmem, uint32_t done, uint32_t free_, float *sums, int *dead, int warp, int lane) {
+    int buf = 0;
+    uint32_t phase = 0u;
+    pdl_wait();                                                              // outputs may be what the previous kernel reads, a bias what it writes
+    for (int tile = P.tile0; tile < P.tiles; tile += P.step) {
+        mx_wait(done + 8 * buf, phase, dead, 24);
+        mt_fence_after();
+        mt_spill(A, tmem + buf * kMtTwoRows, min(A.nt, A.rows - tile / A.pairs_p * A.nt), sums, warp, lane);
+        mt_free(P, free_ + 8 * buf, lane);
+        mt_epilogue_barrier();
+        mt_outputs<kGated, false>(A, P, tile, sums, warp, lane);
+        mt_epilogue_barrier();
+        if (++buf == A.buffers) buf = 0, phase ^= 1u;
+    }
+}
+
+// The pairs that share a tile's c (one tile a cluster): each its sums, and after a barrier of the cluster its share of the outputs.
+__device__ __forceinline__ void mt_spill_part(const MxTileArgs &A, uint32_t tmem, uint32_t done, float *sums, int *dead, int warp, int lane) {
+    mx_wait(done, 0u, dead, 24);
+    mt_fence_after();
+    mt_spill(A, tmem, A.nt, sums, warp, lane);
+}
+template <bool kGated>
+__device__ __forceinline__ void mt_join(const MxTileArgs &A, const MtPart &P, const float *sums, int warp, int lane) {      // every warp
+    mt_cluster_sync();
+    if (warp < kMtEpilogue || warp >= kMtConverter) return;
+    pdl_wait();
+    mt_outputs<kGated, true>(A, P, P.tile0, sums, warp, lane);
 }
 
 // ---- B: a stage is kBoxes times 64 values of c of this CTA's half of a tile's rows ----------------------------------------------------------
@@ -437,16 +489,11 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
             if ((place += 2) >= kMtPlaces) place = team, phase ^= 1u;
         }
     } else if (warp >= kMtEpilogue) {
-        if (A.splits == 1) mt_epilogue<kGated, kMtTwoRows>(A, P, tmem, done, free_, reinterpret_cast<float *>(smem + A.stages * stage_bytes), &dead, warp, lane);
-        else mt_spill(A, tmem, done, reinterpret_cast<float *>(smem), &dead, warp, lane);
+        float *sums = reinterpret_cast<float *>(smem + A.stages * stage_bytes);
+        if (A.splits == 1) mt_epilogue_staged<kGated>(A, P, tmem, done, free_, sums, &dead, warp, lane);
+        else mt_spill_part(A, tmem, done, sums, &dead, warp, lane);
     }
-    if (A.splits > 1) {
-        mt_cluster_sync();
-        if (warp >= kMtEpilogue && warp < kMtConverter) {
-            pdl_wait();
-            mt_join<kGated>(A, P, reinterpret_cast<float *>(smem), warp, lane);
-        }
-    }
+    if (A.splits > 1) mt_join<kGated>(A, P, reinterpret_cast<float *>(smem + A.stages * stage_bytes), warp, lane);
     mt_end(tmem, &dead, warp);
 }
 
@@ -570,16 +617,10 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
             if ((slot += 2) >= A.stages) slot = team, phase ^= 1u;
         }
     } else if (warp >= kMtEpilogue) {
-        if (A.splits == 1) mt_epilogue<false, kMtRows>(A, P, tmem, done, free_, nullptr, &dead, warp, lane);
-        else mt_spill(A, tmem, done, reinterpret_cast<float *>(smem), &dead, warp, lane);
+        if (A.splits == 1) mt_epilogue(A, P, tmem, done, free_, &dead, warp, lane);
+        else mt_spill_part(A, tmem, done, reinterpret_cast<float *>(smem), &dead, warp, lane);      // the ring's time is over
     }
-    if (A.splits > 1) {
-        mt_cluster_sync();
-        if (warp >= kMtEpilogue && warp < kMtConverter) {
-            pdl_wait();
-            mt_join<false>(A, P, reinterpret_cast<float *>(smem), warp, lane);
-        }
-    }
+    if (A.splits > 1) mt_join<false>(A, P, reinterpret_cast<float *>(smem), warp, lane);
     mt_end(tmem, &dead, warp);
 }
 
