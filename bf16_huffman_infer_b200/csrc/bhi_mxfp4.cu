@@ -89,6 +89,35 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W
     }
 }
 
+// ---- from the plain order ----------------------------------------------------------------------------------------------
+// Two codes a byte along a row, the even element in the low half, and a scale byte a block, to the order of the kernels; threads as above.
+__global__ void __launch_bounds__(kMxQuantThreads) mx_layout_kernel(const uint8_t *packed, const uint8_t *packed_scales, int M, int K, int groups, uint8_t *codes, uint8_t *scales) {
+    const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
+    if (at >= groups * 16) return;
+    const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
+    const int tiles16 = (M + 15) / 16 * 16;
+    for (int m0 = blockIdx.y * kMxQuantRows; m0 < tiles16; m0 += gridDim.y * kMxQuantRows) {
+        uint32_t word[kMxQuantRows], byte[kMxQuantRows];
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) {
+            word[r] = byte[r] = 0u;
+            if (m0 + r < M && at * 8 < K) {
+                word[r] = __ldg(reinterpret_cast<const uint32_t *>(packed + static_cast<int64_t>(m0 + r) * (K / 2)) + at);
+                byte[r] = __ldg(packed_scales + static_cast<int64_t>(m0 + r) * (K / 32) + (at >> 2));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) {
+            uint32_t even = word[r] & 0x0F0F0F0Fu, odd = (word[r] >> 4) & 0x0F0F0F0Fu;      // a nibble a byte: side by side, in two steps
+            even = (even | even >> 4) & 0x00FF00FFu, odd = (odd | odd >> 4) & 0x00FF00FFu;
+            even = (even | even >> 8) & 0xFFFFu, odd = (odd | odd >> 8) & 0xFFFFu;
+            const int64_t row = mx_code_row(m0 + r, groups);
+            *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4) = byte[r] == 255u ? 0u : even | odd << 16;
+            if (t == 0) scales[mx_scale_row(m0 + r, groups) + static_cast<int64_t>(g) * kMxTileScales + j] = static_cast<uint8_t>(byte[r]);
+        }
+    }
+}
+
 // ---- the dense matrix ------------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, uint16_t *Y) {
     const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
@@ -151,7 +180,7 @@ __global__ void __launch_bounds__(kMxPairThreads) mx_gated_grad_kernel(const flo
     }
 }
 
-// Does nothing, after the quantisation: a kernel with launch overlap that follows may read the weight before it has waited for the kernel
+// Does nothing, after a kernel that writes a weight: a kernel with launch overlap that follows may read the weight before it has waited for the kernel
 // in front of it, which is then this one, and this one starts when the weight is complete.
 __global__ void mx_settle_kernel() {}
 
@@ -199,6 +228,18 @@ int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, u
     }
     mx_settle_kernel<<<1, 32, 0, st>>>();
     return mx_launched("quantisation launch");
+}
+
+int bhi_mxfp4_from_packed(const uint8_t *packed, const uint8_t *packed_scales, int M, int K, uint8_t *codes, uint8_t *scales, void *stream) {
+    if (int rc = mx_check(codes, scales, M, K)) return rc;
+    BHI_REQUIRE(packed && packed_scales && aligned(packed, 4), "packed codes must be 4-byte aligned");
+    const int groups = (K + kMxGroup - 1) / kMxGroup;
+    dim3 grid, block;
+    mx_matrix_grid(groups * 16, (M + 15) / 16 * 16, grid, block);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    mx_layout_kernel<<<grid, block, 0, st>>>(packed, packed_scales, M, K, groups, codes, scales);
+    mx_settle_kernel<<<1, 32, 0, st>>>();
+    return mx_launched("layout launch");
 }
 
 int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, uint16_t *Y, void *stream) {

@@ -716,6 +716,20 @@ void boxed_mxfp4_quantize(StableIValue *stack, uint64_t, uint64_t) {
     check(bhi_mxfp4_quantize(W.data_ptr(), dtype, v.M, v.K, ptr<uint8_t>(codes), ptr<uint8_t>(scales), stream_of(W)));
 }
 
+// mxfp4_from_packed(packed, packed_scales, codes(a!), scales(b!)) -> ()
+void boxed_mxfp4_from_packed(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor packed = arg(stack, 0), packed_scales = arg(stack, 1), codes = arg(stack, 2), scales = arg(stack, 3);
+    want(packed, ScalarType::Byte, "packed");
+    want(packed_scales, ScalarType::Byte, "packed_scales");
+    STD_TORCH_CHECK(packed.dim() == 2 && packed_scales.dim() == 2 && packed_scales.size(0) == packed.size(0) && packed.size(1) == 16 * packed_scales.size(1),
+                    "packed must be [M, K/2] and packed_scales [M, K/32]");
+    same_device(packed, packed_scales, "packed_scales");
+    same_device(packed, codes, "codes");
+    const MxView v = mx_of(codes, scales, packed.size(0), 2 * packed.size(1));
+    OnDevice on(packed);
+    check(bhi_mxfp4_from_packed(ptr<const uint8_t>(packed), ptr<const uint8_t>(packed_scales), v.M, v.K, ptr<uint8_t>(codes), ptr<uint8_t>(scales), stream_of(packed)));
+}
+
 // dense_mxfp4(codes, scales, M, K) -> W
 void boxed_dense_mxfp4(StableIValue *stack, uint64_t, uint64_t) {
     Tensor codes = arg(stack, 0), scales = arg(stack, 1);
@@ -838,6 +852,7 @@ STABLE_TORCH_LIBRARY(BHI_TORCH_NAMESPACE, m) {
     m.def("ans_emit_pass(Tensor W, int split_k, Tensor freq, Tensor cum, Tensor offsets, Tensor stream_words, Tensor(a!) rem, Tensor(b!) exp) -> ()");
     // 4-bit microscaled weights
     m.def("mxfp4_quantize(Tensor W, Tensor(a!) codes, Tensor(b!) scales) -> ()");
+    m.def("mxfp4_from_packed(Tensor packed, Tensor packed_scales, Tensor(a!) codes, Tensor(b!) scales) -> ()");
     m.def("dense_mxfp4(Tensor codes, Tensor scales, int M, int K) -> Tensor");
     m.def("forward_mxfp4(Tensor X, Tensor codes, Tensor scales, int M, Tensor? bias) -> Tensor");
     m.def("mxfp4_linear_grad(Tensor dY, Tensor codes, Tensor scales, int M, int K) -> Tensor");
@@ -877,6 +892,7 @@ STABLE_TORCH_LIBRARY_IMPL(BHI_TORCH_NAMESPACE, CUDA, m) {
     m.impl("ans_size_pass", &boxed_ans_size_pass);
     m.impl("ans_emit_pass", &boxed_ans_emit_pass);
     m.impl("mxfp4_quantize", &boxed_mxfp4_quantize);
+    m.impl("mxfp4_from_packed", &boxed_mxfp4_from_packed);
     m.impl("dense_mxfp4", &boxed_dense_mxfp4);
     m.impl("forward_mxfp4", &boxed_forward_mxfp4);
     m.impl("mxfp4_linear_grad", &boxed_mxfp4_linear_grad);

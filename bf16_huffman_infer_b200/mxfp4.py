@@ -86,8 +86,7 @@ class MXFP4Weight(nn.Module):
         if a.data_ptr() % 16:
             a = a.clone()
         tiles, groups = _padded(*a.shape)
-        codes = torch.empty(tiles, groups, 4, 16, 16, dtype=torch.uint8, device=a.device)
-        scales = torch.empty(tiles, groups, 16, 4, dtype=torch.uint8, device=a.device)
+        codes, scales = _empty(tiles, groups, a.device)
         ops.mxfp4_quantize(a, codes, scales)
         if to_cpu:
             codes, scales = transfer.download(codes), transfer.download(scales)
@@ -105,6 +104,11 @@ class MXFP4Weight(nn.Module):
                              f"{scales.dtype} {tuple(scales.shape)}")
         M, K = codes.size(0), 2 * codes.size(1)
         tiles, groups = _padded(M, K)
+        if codes.is_cuda:
+            c, s = _empty(tiles, groups, codes.device)
+            codes = codes.contiguous()
+            ops.mxfp4_from_packed(codes.clone() if codes.data_ptr() % 4 else codes, scales.contiguous(), c, s)
+            return cls(c, s, M, K)
         s = F.pad(scales, (0, groups * 4 - K // 32, 0, tiles * 16 - M))
         # a NaN block holds zero codes
         c = codes.view(M, -1, 16).masked_fill((scales == 255)[..., None], 0).view(M, -1)
@@ -112,10 +116,7 @@ class MXFP4Weight(nn.Module):
         low, high = c & 15, c >> 4
         byte = [low[..., 0] | low[..., 1] << 4, low[..., 2] | low[..., 3] << 4, high[..., 0] | high[..., 1] << 4, high[..., 2] | high[..., 3] << 4]
         c = torch.stack(byte, -1).permute(0, 2, 4, 1, 3, 5).reshape(tiles, groups, 4, 16, 16)
-        s = s.view(tiles, 16, groups, 4).transpose(1, 2).contiguous()
-        if c.is_cuda:
-            torch.cuda.current_stream(c.device).synchronize()          # complete in memory, as after compress
-        return cls(c, s, M, K)
+        return cls(c, s.view(tiles, 16, groups, 4).transpose(1, 2).contiguous(), M, K)
 
     def packed(self) -> Tuple[Tensor, Tensor]:
         """``(codes u8 [M, K/2], scales u8 [M, K/32])`` in the plain order; the inverse of :meth:`from_packed`."""
@@ -133,6 +134,11 @@ def _padded(M: int, K: int) -> Tuple[int, int]:
     if M < 1 or K < BLOCK or K % BLOCK:
         raise ValueError(f"an MXFP4 weight needs at least one row and a multiple of {BLOCK} columns, not {M} x {K}")
     return (M + 15) // 16, (K + 127) // 128
+
+
+def _empty(tiles: int, groups: int, device: torch.device) -> Tuple[Tensor, Tensor]:
+    return (torch.empty(tiles, groups, 4, 16, 16, dtype=torch.uint8, device=device),
+            torch.empty(tiles, groups, 16, 4, dtype=torch.uint8, device=device))
 
 
 _is_grad_enabled, _interpreter = torch.is_grad_enabled, torch._C._functorch.peek_interpreter_stack

@@ -159,6 +159,8 @@ def ans_emit_pass(W: Tensor, split_k: int, freq: Tensor, cum: Tensor, offsets: T
 # ---- 4-bit microscaled weights ----------------------------------------------------------------------
 # (W, codes, scales) -> (): W BF16, FP16 or FP32; codes and scales as in MXFP4Weight
 mxfp4_quantize = _ops.mxfp4_quantize.default
+# (packed [M, K/2], packed_scales [M, K/32], codes, scales) -> ()
+mxfp4_from_packed = _ops.mxfp4_from_packed.default
 # (codes, scales, M, K) -> W BF16
 dense_mxfp4 = _ops.dense_mxfp4.default
 # (X, codes, scales, M, bias or None) -> Y: any number of rows of X, any leading dimensions

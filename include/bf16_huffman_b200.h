@@ -302,6 +302,10 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
  * follow on the same stream, with launch overlap or without. */
 int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
 
+/* The same from the plain order: packed u8 [M, K / 2], the even element in the low half of a byte, and packed_scales u8 [M, K / 32].  The codes of
+ * blocks whose scale is NaN become zero. */
+int bhi_mxfp4_from_packed(const uint8_t *packed, const uint8_t *packed_scales, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
+
 /* Y bf16 [M, K]: the values (exact but for scales beyond BF16's range). */
 int bhi_mxfp4_dense(const uint8_t *codes, const uint8_t *scales, int M, int K, uint16_t *Y, void *stream);
 

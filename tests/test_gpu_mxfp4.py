@@ -108,6 +108,25 @@ def test_infinities_and_nans_make_their_block_nan(pkg):
         assert torch.equal(y.isnan().all(0), want.any(1)) and torch.equal(y.isnan().any(0), want.any(1))
 
 
+@pytest.mark.parametrize("M,K", SHAPES)
+def test_plain_order_as_on_the_host(pkg, M, K):
+    """Codes and scales of every value, NaN scales and padding among them; slices and odd addresses."""
+    g = torch.Generator().manual_seed(M)
+    codes = torch.randint(0, 256, (M + 2, K // 2), dtype=torch.uint8, generator=g)
+    scales = torch.randint(0, 256, (M + 2, K // 32), dtype=torch.uint8, generator=g)
+    scales[0, 0] = 255
+    on = codes.to(DEV), scales.to(DEV)
+    shifted = torch.empty(codes.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(codes.shape).copy_(codes)
+    for part in (slice(0, M), slice(1, M + 1), slice(2, M + 2)):
+        want = pkg.MXFP4Weight.from_packed(codes[part], scales[part])
+        for c, s in (on, (shifted, on[1]), (on[0].T.contiguous().T, on[1].T.contiguous().T), (on[0], on[1].view(torch.float8_e8m0fnu))):
+            got = pkg.MXFP4Weight.from_packed(c[part], s[part])
+            assert torch.equal(got.codes.cpu(), want.codes) and torch.equal(got.scales.cpu(), want.scales)
+    for c, s in ((on[0], scales), (codes, on[1])):
+        with pytest.raises(RuntimeError):
+            pkg.MXFP4Weight.from_packed(c, s)
+
+
 def test_quantisation_of_other_layouts(pkg):
     a = normal(64, 256, std=0.02)
     want = pkg.MXFP4Weight.compress(a, to_cpu=False).get_weight()

@@ -101,6 +101,7 @@ def test_operator_schemas():
     ns = torch.ops.bf16_huffman_infer
     for name, sig in {
         "mxfp4_quantize": "(Tensor W, Tensor(a!) codes, Tensor(b!) scales) -> ()",
+        "mxfp4_from_packed": "(Tensor packed, Tensor packed_scales, Tensor(a!) codes, Tensor(b!) scales) -> ()",
         "dense_mxfp4": "(Tensor codes, Tensor scales, int M, int K) -> Tensor",
         "forward_mxfp4": "(Tensor X, Tensor codes, Tensor scales, int M, Tensor? bias) -> Tensor",
         "mxfp4_linear_grad": "(Tensor dY, Tensor codes, Tensor scales, int M, int K) -> Tensor",
@@ -118,12 +119,15 @@ def test_refusals_of_the_library():
     weights = [(none, p, 16, 128), (p, none, 16, 128), (odd, p, 16, 128), (p, odd, 16, 128), (p, p, 0, 128), (p, p, 16, 0), (p, p, 16, 48), (p, p, most, 128), (p, p, 16, most)]
     for c, s, M, K in weights:
         assert lib.bhi_mxfp4_quantize(p, n(0), n(M), n(K), c, s, none) == refused
+        assert lib.bhi_mxfp4_from_packed(p, p, n(M), n(K), c, s, none) == refused
         assert lib.bhi_mxfp4_dense(c, s, n(M), n(K), p, none) == refused
         assert lib.bhi_mxfp4_linear(c, s, n(M), n(K), p, none, p, n(1), none) == refused
         assert lib.bhi_mxfp4_linear_grad(c, s, n(M), n(K), p, n(max(M, 8) // 8 * 8), p, n(1), none) == refused
         assert lib.bhi_mxfp4_gated(c, s, n(M // 2), n(K), p, none, n(0), p, none, n(1), none) == refused
     assert lib.bhi_mxfp4_quantize(odd, n(0), n(16), n(128), p, p, none) == refused
     assert lib.bhi_mxfp4_quantize(p, n(3), n(16), n(128), p, p, none) == refused
+    for codes, scales in [(none, p), (p, none), (ctypes.c_void_p(258), p)]:
+        assert lib.bhi_mxfp4_from_packed(codes, scales, n(16), n(128), p, p, none) == refused
     assert lib.bhi_mxfp4_dense(p, p, n(16), n(128), odd, none) == refused
     for x, y, rows in [(none, p, 1), (odd, p, 1), (p, none, 1), (p, p, 0), (p, p, -1), (p, p, (1 << 30) + 1)]:
         assert lib.bhi_mxfp4_linear(p, p, n(16), n(128), x, none, y, n(rows), none) == refused
