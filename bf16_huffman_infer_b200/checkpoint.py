@@ -118,7 +118,7 @@ def _empty_weight(meta: Dict) -> HuffmanWeight:
     if meta["algo"] == MXFP4Weight.algo:
         M, K = meta["shape"]
         tiles, groups = (M + 15) // 16, (K + 127) // 128
-        return MXFP4Weight(torch.empty(tiles, groups, 4, 16, 16, dtype=torch.uint8), torch.empty(tiles, groups, 16, 4, dtype=torch.uint8), M, K)
+        return MXFP4Weight(torch.empty(tiles, groups, 16, 4, 16, dtype=torch.uint8), torch.empty(tiles, groups, 16, 4, dtype=torch.uint8), M, K)
     rem = torch.empty(meta["rem"], dtype=torch.uint8)
     exp = torch.empty(meta["exp"], dtype=torch.int32)
     offsets = torch.empty(meta["offsets"], dtype=torch.int32)

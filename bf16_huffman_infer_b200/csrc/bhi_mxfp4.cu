@@ -9,7 +9,7 @@ namespace bhi {
 // hardware's conversion rounds and saturates so: every code is the format's own.  A block with an infinity or a NaN is NaN.
 //
 // A thread makes a word (8 values) of each of kMxQuantRows rows at once, the four threads of a block share its maximum; a warp reads
-// 256 values of a row in one piece and writes eight 16-byte pieces a row, four rows side by side.  Bound by memory: read once, written once.
+// 256 values of a row in one piece and writes them as two of 64 bytes, four rows side by side.  Bound by memory: read once, written once.
 template <class T>
 __device__ __forceinline__ void mx_load8(const T *p, uint32_t (&bits)[8]);
 template <>
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W
             }
             if (in_row) {
                 const int64_t row = mx_code_row(m0 + r, groups);
-                *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4) = word;
+                *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4) = word;
                 if (t == 0) scales[mx_scale_row(m0 + r, groups) + static_cast<int64_t>(g) * kMxTileScales + j] = static_cast<uint8_t>(byte);
             }
         }
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_layout_kernel(const uint8_
             even = (even | even >> 4) & 0x00FF00FFu, odd = (odd | odd >> 4) & 0x00FF00FFu;
             even = (even | even >> 8) & 0xFFFFu, odd = (odd | odd >> 8) & 0xFFFFu;
             const int64_t row = mx_code_row(m0 + r, groups);
-            *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4) = byte[r] == 255u ? 0u : even | odd << 16;
+            *reinterpret_cast<uint32_t *>(codes + row + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4) = byte[r] == 255u ? 0u : even | odd << 16;
             if (t == 0) scales[mx_scale_row(m0 + r, groups) + static_cast<int64_t>(g) * kMxTileScales + j] = static_cast<uint8_t>(byte[r]);
         }
     }
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, u
     const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
     if (at * 8 >= W.K) return;
     const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
-    const uint8_t *codes = W.codes + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4, *scales = W.scales + static_cast<int64_t>(g) * kMxTileScales + j;
+    const uint8_t *codes = W.codes + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4, *scales = W.scales + static_cast<int64_t>(g) * kMxTileScales + j;
     for (int m0 = blockIdx.y * kMxQuantRows; m0 < W.M; m0 += gridDim.y * kMxQuantRows) {
         uint32_t word[kMxQuantRows], scale[kMxQuantRows];
 #pragma unroll

@@ -5,9 +5,11 @@
 //
 // The rows are cut into tiles of 16 and the columns into groups of 128; both are padded with zeros.  One (tile, group) pair is
 // 1 KB of codes and 64 bytes of scales, so whatever walks along K reads whole lines.  A lane of an m16n8k16 product finds the four
-// words it needs of a row in one 16-byte load, and lanes that take a row each read 16 bytes side by side:
+// words it needs of a row in one 16-byte load, and the eight lanes that a load is served by at a time, two rows of four, read one line.  (With a
+// quarter's rows side by side they read four, and the first level's data path bounded the kernel: 151936 x 4096, 1 row 62.0 against 59.8 us;
+// readers that take a row a lane would have it so: 37984 x 4096, 64 rows 49.6 against 51.4.)
 //
-//   codes  [ceil(M / 16)][ceil(K / 128)][4 quarters t][16 rows][4 blocks j][4 bytes]   word (t, j): elements 8 t .. 8 t + 7 of block j
+//   codes  [ceil(M / 16)][ceil(K / 128)][16 rows][4 quarters t][4 blocks j][4 bytes]   word (t, j): elements 8 t .. 8 t + 7 of block j
 //   scales [ceil(M / 16)][ceil(K / 128)][16 rows][4 blocks j]
 //
 // Inside a word, nibble i is element 2 i and nibble 4 + i element 2 i + 1 (i = 0..3): a mask leaves the pair (2 i, 2 i + 1) in
@@ -27,17 +29,16 @@ constexpr int kMxRows = 16;                     // rows of a tile
 constexpr int kMxGroup = 128;                   // columns of a group
 constexpr int kMxTileCodes = 1024;              // bytes of a (tile, group) pair
 constexpr int kMxTileScales = 64;
+constexpr int kMxRowCodes = 64;                 // bytes of a row in it
 
 struct MxWeight {
     const uint8_t *codes, *scales;
     int M, K, groups;                           // groups = ceil(K / 128)
 };
 
-constexpr int kMxQuarter = 256;                 // bytes from a quarter of a row to the next
-
-// byte offsets of row m, group 0 (codes: quarter 0)
+// byte offsets of row m, group 0
 __host__ __device__ __forceinline__ int64_t mx_code_row(int m, int groups) {
-    return static_cast<int64_t>(m >> 4) * groups * kMxTileCodes + (m & 15) * 16;
+    return static_cast<int64_t>(m >> 4) * groups * kMxTileCodes + (m & 15) * kMxRowCodes;
 }
 __host__ __device__ __forceinline__ int64_t mx_scale_row(int m, int groups) {
     return static_cast<int64_t>(m >> 4) * groups * kMxTileScales + (m & 15) * 4;

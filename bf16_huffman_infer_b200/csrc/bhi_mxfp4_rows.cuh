@@ -90,7 +90,7 @@ __device__ __forceinline__ float mx_one_output(const MxRowsArgs &A, int m, int c
     for (int k = 0; k < A.W.K; k += 8) {
         const int g = k >> 7, j = (k >> 5) & 3, t = (k >> 3) & 3;
         float v[8];
-        mx_word_to_f32(*reinterpret_cast<const uint32_t *>(codes + static_cast<int64_t>(g) * kMxTileCodes + t * kMxQuarter + j * 4),
+        mx_word_to_f32(*reinterpret_cast<const uint32_t *>(codes + static_cast<int64_t>(g) * kMxTileCodes + t * 16 + j * 4),
                        mx_scale(scales[static_cast<int64_t>(g) * kMxTileScales + j]), v);
 #pragma unroll
         for (int i = 0; i < 8; i++) sum = fmaf(v[i], __uint_as_float(static_cast<uint32_t>(load_written(x + k + i)) << 16), sum);
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
     uint32_t sa[kDepth][MT], sb[kDepth][MT];
     // Rows a and b (eight on, or an output's up) of the step that is being requested, at the next group: 16-byte units of the codes of their
     // (tile, group) pairs, which are also bytes of the scales, and rows in their tiles.
-    const uint8_t *codes = A.W.codes + t * kMxQuarter, *scales = A.W.scales;
+    const uint8_t *codes = A.W.codes + t * 16, *scales = A.W.scales;
     constexpr int kRows = kGated ? 2 : MT;                                   // different (tile, group) pairs of a unit
     uint32_t at[kRows];
     int ra = g, rb = g + 8;
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
 #pragma unroll
         for (int q = 0; q < MT; q++) {
             const uint32_t pa = at[q], pb = at[kGated ? 1 : q];
-            const uint8_t *a = codes + static_cast<uint64_t>(pa) * 16 + ra * 16, *b = kGated ? codes + static_cast<uint64_t>(pb) * 16 + rb * 16 : a + 128;
+            const uint8_t *a = codes + static_cast<uint64_t>(pa) * 16 + ra * kMxRowCodes, *b = kGated ? codes + static_cast<uint64_t>(pb) * 16 + rb * kMxRowCodes : a + 8 * kMxRowCodes;
             qa[slot][q] = load_stream16(a);
             qb[slot][q] = load_stream16(b);
             sa[slot][q] = load_stream4(scales + pa + ra * 4);

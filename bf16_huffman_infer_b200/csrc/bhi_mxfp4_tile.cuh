@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         auto rows_of = [&]() {                                               // past the end: some other row, nobody reads the results
             const int p = 2 * (tile % A.pairs_p) + static_cast<int>(P.half);
             const int m = kGated ? min(64 * p + (row & 63), A.outs - 1) + (row >= 64 ? A.outs : 0) : min(128 * p + row, A.W.M - 1);
-            cp = A.W.codes + mx_code_row(m, A.W.groups) + half * 2 * kMxQuarter + static_cast<int64_t>(group0 + g) * kMxTileCodes;
+            cp = A.W.codes + mx_code_row(m, A.W.groups) + half * 32 + static_cast<int64_t>(group0 + g) * kMxTileCodes;
             sp = A.W.scales + mx_scale_row(m, A.W.groups) + static_cast<int64_t>(group0 + g) * kMxTileScales;
         };
         auto settle = [&]() {                                                // (tile, g) with g past the tile's groups: into the next tiles
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_tile_kernel(const MxTileArgs
         uint32_t s = 0u;
         auto load = [&]() {
             q0 = __ldg(reinterpret_cast<const uint4 *>(cp));
-            q1 = __ldg(reinterpret_cast<const uint4 *>(cp + kMxQuarter));
+            q1 = __ldg(reinterpret_cast<const uint4 *>(cp + 16));
             s = __ldg(reinterpret_cast<const uint32_t *>(sp));
         };
         settle();
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kMtThreads, 1) mx_grad_kernel(const MxTileArgs
         auto place = [&]() {                                                 // of stage ask_c of ask_tile; p past the end: nobody reads the results
             while (ask_c >= P.boxes && ask_tile < tiles) ask_c -= P.boxes, ask_tile += step;
             const int64_t at = static_cast<int64_t>(4 * (P.box0 + ask_c) + (row >> 4)) * A.W.groups + min(2 * (ask_tile % A.pairs_p) + static_cast<int>(P.half), A.W.groups - 1);
-            cp = A.W.codes + at * kMxTileCodes + t * kMxQuarter + (row & 15) * 16;
+            cp = A.W.codes + at * kMxTileCodes + t * 16 + (row & 15) * kMxRowCodes;
             sp = A.W.scales + at * kMxTileScales + (row & 15) * 4;
         };
         auto load = [&](uint4 &to_q, uint32_t &to_s) {

@@ -688,8 +688,8 @@ MxView mx_of(const Tensor &codes, const Tensor &scales, int64_t M, int64_t K) {
     same_device(codes, scales, "scales");
     STD_TORCH_CHECK(M >= 1 && K >= 32 && K % 32 == 0 && M <= BHI_MXFP4_MAX_DIM && K <= BHI_MXFP4_MAX_DIM, "a weight has rows and a multiple of 32 columns");
     const int64_t tiles = (M + 15) / 16, groups = (K + 127) / 128;
-    STD_TORCH_CHECK(codes.dim() == 5 && codes.size(0) == tiles && codes.size(1) == groups && codes.size(2) == 4 && codes.size(3) == 16 && codes.size(4) == 16,
-                    "codes must be [ceil(M/16), ceil(K/128), 4, 16, 16]");
+    STD_TORCH_CHECK(codes.dim() == 5 && codes.size(0) == tiles && codes.size(1) == groups && codes.size(2) == 16 && codes.size(3) == 4 && codes.size(4) == 16,
+                    "codes must be [ceil(M/16), ceil(K/128), 16, 4, 16]");
     STD_TORCH_CHECK(scales.dim() == 4 && scales.size(0) == tiles && scales.size(1) == groups && scales.size(2) == 16 && scales.size(3) == 4,
                     "scales must be [ceil(M/16), ceil(K/128), 16, 4]");
     return {ptr<const uint8_t>(codes), ptr<const uint8_t>(scales), static_cast<int>(M), static_cast<int>(K)};

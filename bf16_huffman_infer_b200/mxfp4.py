@@ -30,7 +30,7 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 class MXFP4Weight(nn.Module):
     """A ``[M, K]`` weight of 4-bit floats with a scale byte for every 32 (``K`` a multiple of 32).
 
-    Buffers, padded with zeros to tiles of 16 rows and groups of 128 columns: ``codes`` u8 ``[ceil(M/16), ceil(K/128), 4, 16, 16]`` and
+    Buffers, padded with zeros to tiles of 16 rows and groups of 128 columns: ``codes`` u8 ``[ceil(M/16), ceil(K/128), 16, 4, 16]`` and
     ``scales`` u8 ``[ceil(M/16), ceil(K/128), 16, 4]``, in the order that the kernels read (``include/bf16_huffman_b200.h``);
     :meth:`from_packed` and :meth:`packed` translate from and to the plain order that checkpoints have.
     """
@@ -40,7 +40,7 @@ class MXFP4Weight(nn.Module):
     def __init__(self, codes: Tensor, scales: Tensor, out_features: int, in_features: int):
         super().__init__()
         tiles, groups = _padded(out_features, in_features)
-        for name, t, shape in (("codes", codes, (tiles, groups, 4, 16, 16)), ("scales", scales, (tiles, groups, 16, 4))):
+        for name, t, shape in (("codes", codes, (tiles, groups, 16, 4, 16)), ("scales", scales, (tiles, groups, 16, 4))):
             if t.dtype != torch.uint8 or tuple(t.shape) != shape:
                 raise ValueError(f"{name} of a {out_features} x {in_features} weight must be u8 {shape}, not {t.dtype} {tuple(t.shape)}")
         # as register_buffer and nn.Module's attributes leave them, in a quarter of the time
@@ -115,14 +115,14 @@ class MXFP4Weight(nn.Module):
         c = F.pad(c, (0, groups * 64 - K // 2, 0, tiles * 16 - M)).view(tiles, 16, groups, 4, 4, 4)     # tile, row, group, block, quarter, byte
         low, high = c & 15, c >> 4
         byte = [low[..., 0] | low[..., 1] << 4, low[..., 2] | low[..., 3] << 4, high[..., 0] | high[..., 1] << 4, high[..., 2] | high[..., 3] << 4]
-        c = torch.stack(byte, -1).permute(0, 2, 4, 1, 3, 5).reshape(tiles, groups, 4, 16, 16)
+        c = torch.stack(byte, -1).permute(0, 2, 1, 4, 3, 5).reshape(tiles, groups, 16, 4, 16)
         return cls(c, s.view(tiles, 16, groups, 4).transpose(1, 2).contiguous(), M, K)
 
     def packed(self) -> Tuple[Tensor, Tensor]:
         """``(codes u8 [M, K/2], scales u8 [M, K/32])`` in the plain order; the inverse of :meth:`from_packed`."""
         M, K = self.shape
         tiles, groups = self.codes.shape[:2]
-        c = self.codes.view(tiles, groups, 4, 16, 4, 4).permute(0, 3, 1, 4, 2, 5).reshape(tiles * 16, groups * 16, 4)
+        c = self.codes.view(tiles, groups, 16, 4, 4, 4).permute(0, 2, 1, 4, 3, 5).reshape(tiles * 16, groups * 16, 4)
         low, high = c & 15, c >> 4
         byte = [low[..., 0] | low[..., 2] << 4, high[..., 0] | high[..., 2] << 4, low[..., 1] | low[..., 3] << 4, high[..., 1] | high[..., 3] << 4]
         c = torch.stack(byte, -1).view(tiles * 16, groups * 64)[:M, :K // 2].contiguous()
@@ -137,7 +137,7 @@ def _padded(M: int, K: int) -> Tuple[int, int]:
 
 
 def _empty(tiles: int, groups: int, device: torch.device) -> Tuple[Tensor, Tensor]:
-    return (torch.empty(tiles, groups, 4, 16, 16, dtype=torch.uint8, device=device),
+    return (torch.empty(tiles, groups, 16, 4, 16, dtype=torch.uint8, device=device),
             torch.empty(tiles, groups, 16, 4, dtype=torch.uint8, device=device))
 
 

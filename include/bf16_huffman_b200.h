@@ -282,7 +282,7 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
  * floats (E2M1).  M outputs, K columns (a multiple of 32), both up to BHI_MXFP4_MAX_DIM, padded to T = ceil(M / 16) tiles of
  * rows and G = ceil(K / 128) groups of columns:
  *
- *   codes   u8 [T, G, 4, 16, 16]  quarters t, rows of a tile, 16 bytes [4 blocks j][4 bytes]: elements 8 t .. 8 t + 7 of block j,
+ *   codes   u8 [T, G, 16, 4, 16]  rows of a tile, quarters t, 16 bytes [4 blocks j][4 bytes]: elements 8 t .. 8 t + 7 of block j,
  *                               nibble i (from the lowest) element 2 i, nibble 4 + i element 2 i + 1
  *   scales  u8 [T, G, 16, 4]      byte s of each block: 2^(s - 127); 255 is NaN (its codes must be zero)
  *

@@ -22,7 +22,7 @@ def packed_weight(M, K, seed=0):
 def test_packed_and_back(M, K):
     codes, scales = packed_weight(M, K)
     w = MXFP4Weight.from_packed(codes, scales)
-    assert w.shape == (M, K) and tuple(w.codes.shape) == ((M + 15) // 16, (K + 127) // 128, 4, 16, 16)
+    assert w.shape == (M, K) and tuple(w.codes.shape) == ((M + 15) // 16, (K + 127) // 128, 16, 4, 16)
     back = w.packed()
     assert torch.equal(back[0], codes) and torch.equal(back[1], scales)
 
@@ -35,8 +35,8 @@ def test_order_of_the_buffers():
         w = MXFP4Weight.from_packed(codes, torch.full((18, 8), 127, dtype=torch.uint8))
         group, j, t, e = k // 128, k % 128 // 32, k % 32 // 8, k % 8
         nibble = e // 2 + 4 * (e % 2)
-        want = torch.zeros(2, 2, 4, 16, 16, dtype=torch.uint8)
-        want[1, group, t, 1, 4 * j + nibble // 2] = 5 << (4 * (nibble % 2))
+        want = torch.zeros(2, 2, 16, 4, 16, dtype=torch.uint8)
+        want[1, group, 1, t, 4 * j + nibble // 2] = 5 << (4 * (nibble % 2))
         assert torch.equal(w.codes, want)
     scales = torch.arange(18 * 8, dtype=torch.uint8).view(18, 8)
     w = MXFP4Weight.from_packed(torch.zeros(18, 128, dtype=torch.uint8), scales)
