@@ -6,14 +6,14 @@
 // Bound by the bytes of the weight.  A warp takes one group of 128 columns of a step's MT tiles of 16 weight rows at a time.
 // They come straight from global memory into registers, kDepth units ahead, and are multiplied by m16n8k16 products.
 //
-// Up to eight rows of X the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32
-// columns start at zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared
-// memory: each row's 128 values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to
-// 2^-31 of the largest in its 128; below, the error is at most 2^-39 of that largest one, far less than a 32-bit sum with it loses.  With X's
-// power of two, up to 2^23 in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are not
-// finite are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
-// With more rows that takes longer than it saves (0.7 us a row), and so do the scales of more sums: codes are expanded to BF16 with their
-// scales, X is read as it is, and the products add up through all of K.
+// Mostly the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32 columns start at
+// zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared memory: each row's 128
+// values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-31 of the largest in
+// its 128; below, the error is at most 2^-39 of that largest one, far less than a 32-bit sum with it loses.  With X's power of two, up to 2^23
+// in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are not finite are computed once
+// more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
+// Where there are more than eight rows to bring to FP16 and few steps to use them in, that takes longer than it saves: codes are expanded to
+// BF16 with their scales, X is read as it is, and the products add up through all of K.
 //
 // The units of a CTA's steps, numbered through, are divided into one run for each warp: a step is one warp's but for those that the ends of
 // runs cut.  The warp with a cut step's beginning adds the parts of the warps after it, in order (they had them at the beginning of their runs)
@@ -62,12 +62,13 @@ __device__ __forceinline__ uint32_t load_stream4(const uint8_t *p) {
     return v;
 }
 
-// A form of the kernel: MT tiles of weight rows by NT blocks of eight rows of X, kWarps warps, kDepth units in flight a warp, kPerSm CTAs an SM.
-template <int MT_, int NT_, int kWarps_, int kPerSm_, int kDepth_, bool kGated_>
+// A form of the kernel: MT tiles of weight rows by NT blocks of eight rows of X, kWarps warps, kDepth units in flight a warp, kPerSm CTAs an SM,
+// FP16 or BF16 products.
+template <int MT_, int NT_, int kWarps_, int kPerSm_, int kDepth_, bool kGated_, bool kHalf_ = true>
 struct MxRowsForm {
     static constexpr int MT = MT_, NT = NT_, kWarps = kWarps_, kPerSm = kPerSm_, kDepth = kDepth_;
     static constexpr bool kGated = kGated_;
-    static constexpr bool kHalf = NT_ == 1;                                  // FP16 products
+    static constexpr bool kHalf = kHalf_;                                    // FP16 products
     static constexpr int kThreads = 32 * kWarps_;
     static constexpr int kPlaces = kDepth_ + 1;                              // of a warp: the steps that end in a turn of kDepth units, and a part for another warp
     static_assert(kWarps <= kMxRowWarpsMax, "barriers");
