@@ -24,10 +24,10 @@ EncodeTiledFn encode_tiled() {
 
 enum Kind { kPlain, kGatedPair, kGradient };
 
-// Rows of a tile (a multiple of 32), and into how many parts c is cut (one, two or four pairs of SMs share a tile): the fewest rounds of tiles over
+// Rows of a tile (a multiple of 32), and into how many parts c is cut (up to four pairs of SMs share a tile): the fewest rounds of tiles over
 // the pairs of SMs times what a tile costs, by its rows: measured (4096 columns, ns for 128 of them) 425 + 0.85 rows forward, twice (395 + 0.55
 // rows) for a gradient.  An accumulator on its own (above 128 rows, forward) keeps the products waiting while it is read; parts take
-// kJoin ns for their sums' way through shared memory, and run in one round only: of clusters of eight CTAs two fit on a GPC.
+// kJoin ns for their sums' way through shared memory, and run in one round only, of the clusters that fit: of 74 pairs 33 twos, 22 threes, 15 fours.
 struct TilePlan {
     int nt = 32, splits = 1;
 };
@@ -39,8 +39,8 @@ TilePlan tile_plan(int rows, int pairs_p, int groups, bool gradient) {
     for (int nt = 32; nt <= kMtRows; nt += 32) {
         const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p;
         const double group = gradient ? 2 * (395 + 0.55 * nt) : 425 + 0.85 * nt;
-        for (int s = 1; s <= 4; s *= 2) {
-            if (s > 1 && (tiles * s > (s == 4 ? pairs * 3 / 4 : pairs * 6 / 7) || groups < 2 * s)) break;
+        for (int s = 1; s <= 4; s++) {
+            if (s > 1 && (tiles * s > pairs * (s == 4 ? 4 : 6) / (s == 4 ? 5 : 7) || groups < 2 * s)) break;
             const double rounds = static_cast<double>((tiles + pairs - 1) / pairs);
             const double tile = (groups + s - 1) / s * group + (s == 1 ? nt > kMtTwoRows && !gradient ? 6.0 * nt : 0.0 : kJoin);
             if (rounds * tile + 1e-3 * nt < best_cost - 1e-9) {
