@@ -1,4 +1,6 @@
 // The products of 4-bit microscaled weights in tiles: plans and launches.
+#include <mutex>
+
 #include "bhi_mxfp4_tile.cuh"
 
 namespace bhi {
@@ -8,6 +10,7 @@ bool overlap_launches();
 namespace {
 
 constexpr uint32_t kSmemTile = kSmemMax - 1024;      // what the barriers leave
+constexpr int kSplitsMost = 4;                       // clusters of eight CTAs
 
 // The tensor-map encoder lives in the driver library, which this library does not link: it is looked up through the runtime once.
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -24,14 +27,41 @@ EncodeTiledFn encode_tiled() {
 
 enum Kind { kPlain, kGatedPair, kGradient };
 
+// How many clusters of `splits` pairs of CTAs are active at a time (of 74 pairs of SMs 33 twos, 22 threes, 15 fours: a cluster lies in one GPC).
+int clusters_that_fit(int splits) {
+    static std::mutex mu;
+    static int cached[64][kSplitsMost + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    int &n = cached[dev][splits];
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(sm_count() / (2 * splits) * (2 * splits));
+        cfg.blockDim = dim3(kMtThreads);
+        cfg.dynamicSmemBytes = kSmemTile;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2 * splits;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (staged_prepare(mx_grad_kernel, kSmemTile) != BHI_OK || cudaOccupancyMaxActiveClusters(&n, mx_grad_kernel, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = -1;                              // none
+        }
+    }
+    return n;
+}
+
 // Rows of a tile (a multiple of 32), and into how many parts c is cut (up to four pairs of SMs share a tile): the fewest rounds of tiles over
 // the pairs of SMs times what a tile costs, by its rows: measured (4096 columns, ns for 128 of them) 425 + 0.85 rows forward, twice (395 + 0.55
-// rows) for a gradient.  An accumulator on its own (above 128 rows, forward) keeps the products waiting while it is read; parts take
-// kJoin ns for their sums' way through shared memory, and run in one round only, of the clusters that fit: of 74 pairs 33 twos, 22 threes, 15 fours.
+// rows) for a gradient.  An accumulator on its own (above 128 rows, forward) keeps the products waiting while it is read; the
+// sums of parts take their way through shared memory (1000 + 16.5 rows), and parts run in one round only, of the clusters that fit.  (A last round's few tiles as a
+// launch of their own, in parts: 37984 x 4096, 64 rows, 149 tiles 48 against 51 us, but gated 12288 x 4096, 2048 rows, 768 tiles no faster.)
 struct TilePlan {
     int nt = 32, splits = 1;
 };
-constexpr double kJoin = 2500;
 TilePlan tile_plan(int rows, int pairs_p, int groups, bool gradient) {
     TilePlan best;
     double best_cost = 1e30;
@@ -39,10 +69,10 @@ TilePlan tile_plan(int rows, int pairs_p, int groups, bool gradient) {
     for (int nt = 32; nt <= kMtRows; nt += 32) {
         const int64_t tiles = static_cast<int64_t>((rows + nt - 1) / nt) * pairs_p;
         const double group = gradient ? 2 * (395 + 0.55 * nt) : 425 + 0.85 * nt;
-        for (int s = 1; s <= 4; s++) {
-            if (s > 1 && (tiles * s > pairs * (s == 4 ? 4 : 6) / (s == 4 ? 5 : 7) || groups < 2 * s)) break;
+        for (int s = 1; s <= kSplitsMost; s++) {
+            if (s > 1 && (tiles > clusters_that_fit(s) || groups < 2 * s)) break;
             const double rounds = static_cast<double>((tiles + pairs - 1) / pairs);
-            const double tile = (groups + s - 1) / s * group + (s == 1 ? nt > kMtTwoRows && !gradient ? 6.0 * nt : 0.0 : kJoin);
+            const double tile = (groups + s - 1) / s * group + (s == 1 ? nt > kMtTwoRows && !gradient ? 6.0 * nt : 0.0 : 1000 + 16.5 * nt);
             if (rounds * tile + 1e-3 * nt < best_cost - 1e-9) {
                 best_cost = rounds * tile + 1e-3 * nt;
                 best.nt = nt;
@@ -91,9 +121,8 @@ int launch(MxTileArgs a, const uint16_t *B, int64_t b_cols, int64_t ldb, cudaStr
     if (cr != CUDA_SUCCESS) return fail(BHI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(cr)));
     auto kernel = kKind == kGradient ? mx_grad_kernel : mx_tile_kernel<kKind == kGatedPair>;
     if (int rc = staged_prepare(kernel, kSmemTile)) return rc;
-    const int tiles = a.pairs_p * a.tiles_n;
+    const int tiles = a.pairs_p * a.tiles_n, pairs = sm_count() / 2;
     cudaLaunchConfig_t cfg = {};
-    const int pairs = sm_count() / 2;
     cfg.gridDim = dim3(2 * a.splits * (tiles < pairs ? tiles : pairs));
     cfg.blockDim = dim3(kMtThreads);
     cfg.dynamicSmemBytes = a.stages * stage + extra;

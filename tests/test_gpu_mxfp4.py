@@ -359,6 +359,23 @@ def test_other_derivatives(pkg):
     assert float((ddx.double() - want).norm()) <= 2.0 ** -6 * float(want.norm())                    # four roundings on the way
 
 
+@pytest.mark.parametrize("wide,other", [(75 * 256, 512), (76 * 256 - 90, 2080), (2 * 74 * 256 + 256 * 20, 800)])
+@pytest.mark.parametrize("rows", [30, 150])
+def test_tiles_of_a_last_round(pkg, wide, other, rows):
+    """A few tiles more than whole rounds over the pairs of SMs, forward (gated and not) and backward."""
+    w, dense = made(pkg, wide, other, std=1.5 / math.sqrt(other))
+    x = normal(rows, other, seed=rows)
+    mag = x.double().abs() @ dense.abs().T
+    want = x.double() @ dense.T
+    assert close(F.linear(x, w), want, mag, other)
+    g, u = want.chunk(2, -1)
+    want = act64(g, "silu") * u
+    assert float((pkg.gated_mxfp4(x, w).double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+    w, dense = made(pkg, other, wide // 32 * 32)
+    dy = normal(rows, other, seed=rows + 1)
+    assert close(pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, other, wide // 32 * 32), dy.double() @ dense, dy.double().abs() @ dense.abs(), other)
+
+
 # ---- the gated pair --------------------------------------------------------------------------------------------------------
 def act64(g, name):
     if name == "silu":
