@@ -195,6 +195,16 @@ static int mx_check(const void *codes, const void *scales, int M, int K) {
 }
 static MxWeight mx_weight(const uint8_t *codes, const uint8_t *scales, int M, int K) { return {codes, scales, M, K, (K + kMxGroup - 1) / kMxGroup}; }
 
+// Whether a product takes the kernel for few rows.  Its rate is the memory's where the weight is most of the traffic (32 rows of it would be slower: 4096 x
+// 12288 49 against 21 us, 37984 x 4096 51 either way; 16 rows: 12288 x 4096 14.0 against 19.3, 4096 x 4096 8.8 against 10.3).  From nine rows on the tiles are faster where the
+// weight is small (1024 x 1024, 9 rows 4.2 against 5.9 us, 2048 x 2048 5.8 against 6.5; 4096 x 2048 7.5 against 6.7) and where every SM would read a
+// large X for few outputs (2560 x 9728, 16 rows 14.0 against 20.1, 3584 x 18944, 9 rows 24.3 against 27.4; 2048 x 8192, 9 rows 11.9 against 9.9).
+static bool mx_few_rows(int rows, int M, int K) {
+    if (rows <= 8) return true;
+    if (rows > kMxRowsMost || static_cast<int64_t>(M) * K <= 1 << 22) return false;
+    return static_cast<int64_t>(rows) * K <= 125000 || M > 22 * 256;
+}
+
 static int mx_launched(const char *what) {
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? BHI_OK : cuda_fail(e, what);
@@ -256,7 +266,7 @@ int bhi_mxfp4_linear(const uint8_t *codes, const uint8_t *scales, int M, int K, 
     if (int rc = mx_check(codes, scales, M, K)) return rc;
     BHI_REQUIRE(rows >= 1 && rows <= BHI_MXFP4_MAX_ROWS, "bad number of rows");
     BHI_REQUIRE(X && Y && aligned(X, 16) && aligned(Y, 2) && aligned(bias, 2), "X must be 16-byte aligned");
-    if (rows <= kMxRowsMost) {
+    if (mx_few_rows(rows, M, K)) {
         const int rc = mx_rows_launch(mx_weight(codes, scales, M, K), X, bias, Y, false, 0, nullptr, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }
@@ -279,7 +289,7 @@ int bhi_mxfp4_gated(const uint8_t *codes, const uint8_t *scales, int inter, int 
     BHI_REQUIRE(activation >= BHI_ACT_SILU && activation <= BHI_ACT_GELU_TANH, "unknown activation");
     BHI_REQUIRE(X && H && aligned(X, 16) && aligned(H, 2) && aligned(bias, 2) && aligned(pre, 16), "X must be 16-byte aligned");
     const MxWeight W = mx_weight(codes, scales, 2 * inter, K);
-    if (rows <= kMxRowsMost) {
+    if (mx_few_rows(rows, W.M, K)) {
         const int rc = mx_rows_launch(W, X, bias, H, true, activation, pre, rows, static_cast<cudaStream_t>(stream));
         if (rc != kStagedDeclined) return rc;
     }

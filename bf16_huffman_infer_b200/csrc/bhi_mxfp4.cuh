@@ -171,8 +171,7 @@ __device__ __forceinline__ float mx_act(int act, float g) {
     return g * mx_logistic(1.59576912160573071f * (g + 0.044715f * g * g * g));
 }
 
-// Rows of X up to which a product takes the kernel that reads the weight straight into registers; beyond, the tiled one is faster (16 rows:
-// 4096 x 12288 22 against 26 us, 37984 x 4096 27 against 48; 32 rows: 49 against 27, 51 against 49).
+// Rows of X that the kernel which reads the weight straight into registers takes at most.
 constexpr int kMxRowsMost = 16;
 
 // The products' launchers, whose source files are compiled side by side.  Each returns kStagedDeclined for what it does not serve.

@@ -153,6 +153,36 @@ def test_product(pkg, M, K, rows):
     assert close(F.linear(x, w, bias), x.double() @ dense.T + bias.double(), mag + bias.double().abs(), K)
 
 
+@pytest.mark.parametrize("rows", [9, 13, 16])
+@pytest.mark.parametrize("M,K", [(2100, 2080), (2101, 6880), (24003, 416), (23700, 7840), (6000, 12288)])
+def test_nine_to_sixteen_rows(pkg, M, K, rows):
+    """Weights that are large enough for the kernel of few rows: a few steps an SM and many, X in one piece and in several."""
+    w, dense = made(pkg, M, K, seed=M + K, std=1.5 / math.sqrt(K))
+    x, bias = normal(rows, K, seed=rows), normal(M, seed=3)
+    mag = x.double().abs() @ dense.abs().T + bias.double().abs()
+    want = x.double() @ dense.T + bias.double()
+    assert close(F.linear(x, w, bias), want, mag, K)
+    if M % 2 == 0:
+        g, u = want.chunk(2, -1)
+        want = act64(g, "gelu") * u
+        pre = torch.empty(rows, M, device=DEV)
+        h = pkg.ops.gated_mxfp4(x, w.codes, w.scales, M, bias, 1, pre)
+        assert float((h.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+        assert bool(((pre.double() - torch.cat([g, u], -1)).abs() <= mag * (K * 2.0 ** -23)).all())
+
+
+@pytest.mark.parametrize("rows", [9, 16])
+@pytest.mark.parametrize("byte", [0, 60, 200, 240, 252])
+def test_scales_of_the_whole_range_in_many_steps(pkg, byte, rows):
+    g = torch.Generator().manual_seed(rows + byte)
+    M, K = 45000, 96
+    w = pkg.MXFP4Weight.from_packed(torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, generator=g).to(DEV), torch.full((M, K // 32), byte, dtype=torch.uint8, device=DEV))
+    dense = w.get_weight().double()
+    x = torch.ldexp(torch.randn(rows, K, generator=g).double(), torch.tensor(min(127 - byte, 120))).to(torch.bfloat16).to(DEV)
+    want, mag = x.double() @ dense.T, x.double().abs() @ dense.abs().T
+    assert bool(((F.linear(x, w).double() - want).abs() <= want.abs() * 2.0 ** -8 + mag * (K * 2.0 ** -23) + K * 2.0 ** -134).all())
+
+
 def test_product_of_other_layouts(pkg):
     w, dense = made(pkg, 130, 512)
     for rows in (3, 70):
