@@ -195,13 +195,16 @@ static int mx_check(const void *codes, const void *scales, int M, int K) {
 }
 static MxWeight mx_weight(const uint8_t *codes, const uint8_t *scales, int M, int K) { return {codes, scales, M, K, (K + kMxGroup - 1) / kMxGroup}; }
 
-// Whether a product takes the kernel for few rows.  Its rate is the memory's where the weight is most of the traffic (32 rows of it would be slower: 4096 x
-// 12288 49 against 21 us, 37984 x 4096 51 either way; 16 rows: 12288 x 4096 14.0 against 19.3, 4096 x 4096 8.8 against 10.3).  From nine rows on the tiles are faster where the
-// weight is small (1024 x 1024, 9 rows 4.2 against 5.9 us, 2048 x 2048 5.8 against 6.5; 4096 x 2048 7.5 against 6.7) and where every SM would read a
-// large X for few outputs (2560 x 9728, 16 rows 14.0 against 20.1, 3584 x 18944, 9 rows 24.3 against 27.4; 2048 x 8192, 9 rows 11.9 against 9.9).
+// Whether a product takes the kernel for few rows.  Its rate is the memory's where the weight is most of the traffic (16 rows: 12288 x 4096 14.0
+// against 19.3 us, 4096 x 4096 8.8 against 10.3).  From nine rows on the tiles are faster where the weight is small (1024 x 1024, 9 rows 4.2
+// against 5.9 us, 2048 x 2048 5.8 against 6.5; 4096 x 2048 7.5 against 6.7) and where every SM would read a large X for few outputs (2560 x
+// 9728, 16 rows 14.0 against 20.1, 3584 x 18944, 9 rows 24.3 against 27.4; 2048 x 8192, 9 rows 11.9 against 9.9).  From 17 rows on ten steps an SM have to
+// pay for X's conversion (24 rows: 24576 x 4096 31.4 against 34.2, 38000 x 12288 115 against 148, gated 18944 x 3584 35.6 against 36.3); with
+// 32 rows nothing does (24576 x 4096 48 against 34).
 static bool mx_few_rows(int rows, int M, int K) {
     if (rows <= 8) return true;
-    if (rows > kMxRowsMost || static_cast<int64_t>(M) * K <= 1 << 22) return false;
+    if (rows > 16) return rows <= kMxRowsMost && M >= 160 * sm_count();
+    if (static_cast<int64_t>(M) * K <= 1 << 22) return false;
     return static_cast<int64_t>(rows) * K <= 125000 || M > 22 * 256;
 }
 

@@ -172,7 +172,7 @@ __device__ __forceinline__ float mx_act(int act, float g) {
 }
 
 // Rows of X that the kernel which reads the weight straight into registers takes at most.
-constexpr int kMxRowsMost = 16;
+constexpr int kMxRowsMost = 24;
 
 // The products' launchers, whose source files are compiled side by side.  Each returns kStagedDeclined for what it does not serve.
 // `gated`: W.M = 2 * outputs; pre may be null.

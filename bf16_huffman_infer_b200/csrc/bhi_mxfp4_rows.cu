@@ -50,6 +50,7 @@ int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, u
     if (rows > kMxRowsMost || static_cast<int64_t>((W.M + 15) / 16) * W.groups * (kMxTileCodes / 16) > UINT32_MAX) return kStagedDeclined;
     MxRowsArgs a{};
     a.W = W, a.X = X, a.bias = bias, a.Y = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
+    if (rows > 16) return gated ? launch<MxRowsForm<1, 3, 16, 1, 2, true>>(a, st) : launch<MxRowsForm<1, 3, 16, 1, 2, false>>(a, st);
     if (rows > 8) {
         // FP16 where an SM has ten steps or more (16 rows: 151936 x 4096 87 against 108 us, 64 steps; gated 12288 x 4096 22.2 against 22.9, ten; 12288 x
         // 4096 15.1 against 14.0, five; gated 4096 x 2048 9.2 against 7.7, four)

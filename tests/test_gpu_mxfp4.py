@@ -171,7 +171,13 @@ def test_nine_to_sixteen_rows(pkg, M, K, rows):
         assert bool(((pre.double() - torch.cat([g, u], -1)).abs() <= mag * (K * 2.0 ** -23)).all())
 
 
-@pytest.mark.parametrize("rows", [9, 16])
+@pytest.mark.parametrize("rows", [17, 20, 24])
+@pytest.mark.parametrize("M,K", [(24003, 416), (23700, 7840), (24002, 96)])
+def test_seventeen_to_24_rows(pkg, M, K, rows):
+    test_nine_to_sixteen_rows(pkg, M, K, rows)
+
+
+@pytest.mark.parametrize("rows", [9, 16, 24])
 @pytest.mark.parametrize("byte", [0, 60, 200, 240, 252])
 def test_scales_of_the_whole_range_in_many_steps(pkg, byte, rows):
     g = torch.Generator().manual_seed(rows + byte)
