@@ -15,6 +15,8 @@ from __future__ import annotations
 
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
+import copy
+import math
 import os
 
 import numpy as np
@@ -872,45 +874,115 @@ def fuse_sibling_linears(model: nn.Module, groups=SIBLING_GROUPS, algo: str = "h
 
 
 def _activation_of(act_fn: nn.Module) -> Optional[str]:
-    """The name of the activation that ``act_fn`` computes, by what it does."""
-    v = torch.linspace(-6, 6, 97, device="cpu")
-    try:
-        with torch.no_grad():
-            y = act_fn(v)
-    except Exception:                            # an activation with parameters elsewhere, or of another signature
+    """The name of the activation that ``act_fn`` computes, by what it does in evaluation and in training: near zero, and so far out
+    that a limit anywhere shows."""
+    if any(True for _ in act_fn.parameters()) or any(True for _ in act_fn.buffers()):
         return None
+    far = torch.logspace(-8, 30, 153, device="cpu")
+    v = torch.cat([torch.linspace(-30, 30, 1921, device="cpu"), far, -far])
     known = {"silu": F.silu(v), "gelu": F.gelu(v), "gelu_tanh": F.gelu(v, approximate="tanh")}
     assert known.keys() == ACTIVATIONS.keys()
-    for name, want in known.items():
-        if torch.is_tensor(y) and y.shape == v.shape and torch.allclose(y, want, rtol=0, atol=1e-6):      # the two gelus are 5e-4 apart
-            return name
-    return None
+    names = set(known)
+    for training in (False, True):
+        try:
+            with torch.no_grad(), torch.random.fork_rng(devices=[]):
+                random = torch.get_rng_state()
+                y = copy.deepcopy(act_fn).train(training)(v.clone())
+                drew = not torch.equal(torch.get_rng_state(), random)
+        except Exception:                        # of another signature
+            return None
+        if drew or not torch.is_tensor(y) or y.shape != v.shape:
+            return None
+        # the two gelus are 5e-4 apart where they differ most
+        names = {name for name in names if torch.allclose(y, known[name], rtol=1e-5, atol=1e-6)}
+    return names.pop() if len(names) == 1 else None
 
 
-def _is_gated_mlp(parent: nn.Module) -> Optional[str]:
-    """The activation of a block that computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` and nothing else, found by its
-    parts and by running it on one row; None for any other module."""
+def _told(layer: nn.Linear, call) -> nn.Linear:
+    """``layer`` as a block sees it, with ``call`` in the place of its product."""
+    layer = copy.copy(layer)
+    layer.__dict__["forward"] = call
+    return layer
+
+
+def _computes_gated_pair(parent: nn.Module) -> bool:
+    """Whether ``parent`` computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` and nothing else, in evaluation and in training,
+    whatever its weights: its forward is run with projections that return chosen values, tiny to huge, infinite and NaN, and has to
+    hand on exactly what it is given.  A limit, a factor, a mask or dropout anywhere between shows, as does a draw of random numbers."""
+    hidden, inter, out = parent.gate_proj.in_features, parent.gate_proj.out_features, parent.down_proj.out_features
+    gen = torch.Generator().manual_seed(0)
+    rows = 24
+
+    def values(width):
+        v = torch.randn(rows, width, generator=gen, device="cpu") * torch.exp2(torch.randint(-20, 40, (rows, width), generator=gen, device="cpu").float())
+        v[1] = torch.randn(width, generator=gen, device="cpu")
+        v[2, 0], v[3, -1], v[4, 0] = float("inf"), -float("inf"), float("nan")
+        return v.to(torch.bfloat16)
+
+    x = values(hidden).nan_to_num(0, 1, 1)                    # the row's number, which is how a projection knows it, and whatever
+    x[:, 0] = torch.arange(rows, device="cpu")
+    gates, ups, weight = values(inter), values(inter), torch.randn(out, generator=gen, device="cpu").to(torch.bfloat16)
+    column = torch.arange(out, device="cpu") % inter
+
+    def projection(table):
+        def call(v):
+            row = v[..., 0].long()
+            if not torch.equal(v, x[row]):
+                raise ValueError("a projection reads something else than the block's input")
+            return table[row]
+        return call
+
+    def bits(v):
+        return v.contiguous().view(torch.int16)
+
+    def down(h):
+        return h[..., column] * weight
+
+    def same(training, shape):
+        act_fn = copy.deepcopy(parent.act_fn).train(training)
+        probe = copy.copy(parent)
+        probe.__dict__["_modules"] = {**parent._modules, "act_fn": act_fn, "down_proj": _told(parent.down_proj, down),
+                                      "gate_proj": _told(parent.gate_proj, projection(gates)), "up_proj": _told(parent.up_proj, projection(ups))}
+        probe.training = training
+        v = x[:math.prod(shape[:-1])].view(shape)
+        row, random = v[..., 0].long(), torch.get_rng_state()
+        y = probe(v.clone())
+        drew = not torch.equal(torch.get_rng_state(), random)
+        want = down(act_fn(gates[row]) * ups[row])
+        return type(y) is Tensor and y.dtype == want.dtype and not drew and torch.equal(bits(y), bits(want))
+
+    try:
+        with torch.no_grad(), torch.random.fork_rng(devices=[]):
+            return all(same(training, shape) for training in (False, True) for shape in ((rows, hidden), (2, rows // 2, hidden), (1, hidden), (1, 1, hidden)))
+    except Exception:                            # takes, asks for or returns something else
+        return False
+
+
+def _gated_activation(parent: nn.Module) -> Optional[str]:
+    """The activation of a block that computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` and nothing else, by its parts and by
+    what its forward does with them, whatever type its weights have and wherever they are; None for any other module."""
     parts = dict(parent.named_children())
     if parts.keys() != {"gate_proj", "up_proj", "down_proj", "act_fn"} or any(True for _ in parent.parameters(recurse=False)):
         return None
     gate, up, down = (parts[n] for n in ("gate_proj", "up_proj", "down_proj"))
     if not all(type(m) is nn.Linear for m in (gate, up, down)) or gate.weight.shape != up.weight.shape or gate.in_features % 32:
         return None
-    if (gate.bias is None) != (up.bias is None) or gate.weight.dtype != torch.bfloat16 or gate.weight.device != up.weight.device:
+    if down.in_features != gate.out_features or (gate.bias is None) != (up.bias is None):
         return None
     if any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in parent.modules()):
         return None
+    if any("forward" in m.__dict__ for m in parent.modules()):                   # somebody's own, in front of the class's
+        return None
     name = _activation_of(parts["act_fn"])
-    if name is None:
+    return name if name is not None and _computes_gated_pair(parent) else None
+
+
+def _is_gated_mlp(parent: nn.Module) -> Optional[str]:
+    """:func:`_gated_activation` of a block whose weights can be rounded as they are: BF16, on one device."""
+    name = _gated_activation(parent)
+    if name is None or parent.gate_proj.weight.dtype != torch.bfloat16 or parent.gate_proj.weight.device != parent.up_proj.weight.device:
         return None
-    x = torch.linspace(-2, 2, gate.in_features, device=gate.weight.device).to(torch.bfloat16)[None]
-    try:
-        with torch.no_grad():
-            # by their bits: a model that is still to be loaded may hold NaNs
-            same = torch.equal(parent(x).view(torch.int16), down(parts["act_fn"](gate(x)) * up(x)).view(torch.int16))
-    except Exception:                            # takes or returns something else
-        return None
-    return name if same else None
+    return name
 
 
 def fuse_gated_mlps(model: nn.Module, algo: str = "mxfp4", progress: bool = False) -> int:
