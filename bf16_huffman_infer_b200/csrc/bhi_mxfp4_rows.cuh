@@ -9,9 +9,12 @@
 // Mostly the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32 columns start at
 // zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared memory: each row's 128
 // values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-31 of the largest in
-// its 128; below, the error is at most 2^-39 of that largest one, far less than a 32-bit sum with it loses.  With X's power of two, up to 2^23
-// in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are not finite are computed once
-// more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
+// its 128.  Where one lies below (it may be all that counts: the weights of the large ones can be zero), X is brought once more and multiplied as
+// it is, by the BF16 products of the next paragraph in a walk of its own.  (Looking for such
+// values costs most where X is most of the work: 1024 x 4096, 1 row 4.65 against 4.52 us, 151936 x 4096, 8 rows 62 against 61, 38000 x 12288, 24 rows
+// 118 against 115, gated 12288 x 4096, 16 rows 22.9 against 22.1.  A branch in every unit instead of the walk: 8 rows 66 us.)
+// With X's power of two, up to 2^23 in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are
+// not finite are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
 // Where there are more than eight rows to bring to FP16 and few steps to use them in, that takes longer than it saves: codes are expanded to
 // BF16 with their scales, X is read as it is, and the products add up through all of K.
 //
@@ -77,10 +80,32 @@ struct MxRowsForm {
     static __host__ __device__ uint32_t row_bytes(int chunk_groups) { return static_cast<uint32_t>(chunk_groups) * 256u + 64u; }     // rows 64 bytes apart in banks
 };
 
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+// The larger and the smaller magnitude of each half; signs are left over (and a NaN is the larger).
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
+}
+__device__ __forceinline__ uint32_t min_abs_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// Of eight BF16 values the largest magnitude (low half) and 65535 less the smallest (high half), as bits: both are found by maxima from here on.
+__device__ __forceinline__ uint32_t mx_ends(const uint4 &v) {
+    const uint32_t top = max_abs_bf16x2(max_abs_bf16x2(v.x, v.y), max_abs_bf16x2(v.z, v.w)) & 0x7FFF7FFFu;
+    const uint32_t low = ~min_abs_bf16x2(min_abs_bf16x2(v.x, v.y), min_abs_bf16x2(v.z, v.w)) | 0x80008000u;
+    return max_u16x2(__byte_perm(top, low, 0x5410), __byte_perm(top, low, 0x7632));
+}
+// Whether one of two BF16 values is neither zero nor as large as `from` (magnitudes as bits).
+__device__ __forceinline__ bool mx_below(uint32_t pair, uint32_t from) {
+    const uint32_t lo = pair & 0x7FFFu, hi = (pair >> 16) & 0x7FFFu;
+    return (lo != 0u && lo < from) || (hi != 0u && hi < from);
 }
 
 // One output by itself: weight row m, row `col` of X, products in 32 bits.
@@ -105,6 +130,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
     constexpr bool kGated = Form::kGated;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kMxRowWarpsMax + 1];
+    __shared__ int not_fp16;                                                 // the last chunk (its number and one) with a value of X that FP16 does not hold
     __shared__ int dead;                                                     // a wait has run out: no other one waits any more
     constexpr int kWarps = Form::kWarps, threads = Form::kThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -120,6 +146,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
         mbar_init(x_bar, 1);
         mbar_fence_init();
         dead = 0;
+        not_fp16 = 0;
     }
     __syncthreads();
 
@@ -206,6 +233,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
         }
     };
     begin_chunk(0, min(A.chunk_groups, A.W.groups));
+    uint32_t x_phase = 0u;
     for (int c = 0; c < chunks; c++) {
         const int c0 = c * A.chunk_groups, groups = min(A.chunk_groups, A.W.groups - c0);
 
@@ -217,13 +245,22 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             begin_chunk(c0, groups);
             __syncthreads();                                                      // nobody reads the last chunk's X any more
         }
-        if (warp == 0) {
-            if (c == 0) pdl_wait();
-            if (lane == 0) mbar_expect_tx(x_bar, static_cast<uint32_t>(x_bytes * A.rows));
-            __syncwarp();
-            if (lane < A.rows) bulk_copy_g2s(base + lane * row_bytes, A.X + static_cast<int64_t>(lane) * A.W.K + c0 * kMxGroup, x_bytes, x_bar);
-        }
-        mx_wait(x_bar, c & 1, &dead, 10);
+        auto bring_x = [&]() {
+            if (warp == 0) {
+                if (lane == 0) mbar_expect_tx(x_bar, static_cast<uint32_t>(x_bytes * A.rows));
+                __syncwarp();
+                if (lane < A.rows) bulk_copy_g2s(base + lane * row_bytes, A.X + static_cast<int64_t>(lane) * A.W.K + c0 * kMxGroup, x_bytes, x_bar);
+            }
+            mx_wait(x_bar, x_phase, &dead, 10);
+            x_phase ^= 1u;
+        };
+        auto pad_x = [&]() {                                                 // past the last column: zeros
+            const int pad = groups * 256 - x_bytes;
+            for (int i = tid * 16; i < A.rows * pad; i += threads * 16) *reinterpret_cast<uint4 *>(smem + i / pad * row_bytes + x_bytes + i % pad) = make_uint4(0u, 0u, 0u, 0u);
+        };
+        if (c == 0 && warp == 0) pdl_wait();
+        bring_x();
+        bool fp16 = Form::kHalf;                                             // FP16 products, here and now
         if constexpr (Form::kHalf) {
             // to FP16 in place: chunk (group, block, quarter) is eight values, in the order of a word's nibbles; half a warp takes a group of a
             // row, four of them at once
@@ -231,8 +268,9 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
             const int teams = threads / 16, ch = lane & 15, jobs = groups * A.rows, on = teams / A.rows, more = teams - on * A.rows;
             const uint32_t half = 0xFFFFu << (lane & 16);
             int xg = (tid >> 4) / A.rows, xr = (tid >> 4) - xg * A.rows;
+            bool far = false;                                                // a value that FP16 does not hold
             for (int job0 = tid >> 4; job0 < jobs; job0 += teams * kAtOnce) {
-                uint32_t w[kAtOnce][4], top[kAtOnce], at_x[kAtOnce], at_s[kAtOnce];
+                uint32_t w[kAtOnce][4], ends[kAtOnce], at_x[kAtOnce], at_s[kAtOnce];
 #pragma unroll
                 for (int q = 0; q < kAtOnce; q++) {
                     at_x[q] = xr * row_bytes + xg * 256 + ch * 16;
@@ -240,9 +278,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                     uint4 v = make_uint4(0u, 0u, 0u, 0u);
                     if (job0 + q * teams < jobs && xg * 256 + ch * 16 < x_bytes) v = *reinterpret_cast<const uint4 *>(smem + at_x[q]);
                     w[q][0] = v.x, w[q][1] = v.y, w[q][2] = v.z, w[q][3] = v.w;
-                    // magnitudes as bits; an infinity or NaN makes the whole row one, whatever becomes of its other values
-                    const uint32_t m = max_bf16x2(max_bf16x2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), max_bf16x2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-                    top[q] = max(m & 0xFFFFu, m >> 16);
+                    ends[q] = mx_ends(v);                                    // (an infinity or NaN makes the whole row one, whatever becomes of its other values)
                     xg += on;
                     xr += more;
                     if (xr >= A.rows) xr -= A.rows, xg++;
@@ -250,11 +286,15 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1)
 #pragma unroll
-                    for (int q = 0; q < kAtOnce; q++) top[q] = max(top[q], __shfl_xor_sync(half, top[q], o));
+                    for (int q = 0; q < kAtOnce; q++) ends[q] = max_u16x2(ends[q], __shfl_xor_sync(half, ends[q], o));
 #pragma unroll
                 for (int q = 0; q < kAtOnce; q++) {
                     if (job0 + q * teams >= jobs) break;
-                    const uint32_t up = min(268u - (top[q] >> 7), 253u);     // exponent field of 2^(14 - floor(log2 top))
+                    const uint32_t top = ends[q] & 0xFF80u;                  // without its mantissa
+                    const uint32_t up = min(268u - (top >> 7), 253u);        // exponent field of 2^(14 - floor(log2 top))
+                    // the smallest is less than 2^-31 of it: a zero, or (next to an infinity or NaN that does not matter) a value that FP16 does not hold
+                    if ((ends[q] >> 16) + top > 0xFFFFu + (31u << 7) && top < 0x7F80u)
+                        for (int i = 0; i < 4; i++) far |= mx_below(w[q][i], top - (31u << 7));
                     const float scale = __uint_as_float(up << 23);
                     uint32_t h[4];
 #pragma unroll
@@ -268,11 +308,20 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                     if (ch == 0) xscale[at_s[q]] = __uint_as_float((254u - up) << 23);
                 }
             }
+            if (far) not_fp16 = c + 1;
+            __syncthreads();
+            fp16 = not_fp16 != c + 1;
+            if (!fp16) {                                                     // X as it is
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncthreads();
+                bring_x();
+                pad_x();
+                __syncthreads();
+            }
         } else {
-            const int pad = groups * 256 - x_bytes;                          // past the last column: zeros
-            for (int i = tid * 16; i < A.rows * pad; i += threads * 16) *reinterpret_cast<uint4 *>(smem + i / pad * row_bytes + x_bytes + i % pad) = make_uint4(0u, 0u, 0u, 0u);
+            pad_x();
+            __syncthreads();
         }
-        __syncthreads();
 
         float acc[MT][NT][4];
 #pragma unroll
@@ -347,14 +396,14 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 }
             }
         };
-        auto multiply = [&](int d) {
-            if constexpr (Form::kHalf) {
+        auto multiply = [&](int d, auto as_half) {
+            if constexpr (decltype(as_half)::value) {
                 multiply_f16(d);
             } else {
                 uint32_t any = 0u;
 #pragma unroll
                 for (int q = 0; q < MT; q++) any |= sa[d][q] | sb[d][q];
-                if (__any_sync(0xFFFFFFFFu, (any & 0x80808080u) != 0u)) multiply_bf16(d, std::true_type{});
+                if (Form::kHalf || __any_sync(0xFFFFFFFFu, (any & 0x80808080u) != 0u)) multiply_bf16(d, std::true_type{});
                 else multiply_bf16(d, std::false_type{});
             }
             gr++;
@@ -445,24 +494,32 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 else finish(first, place, warp);
             }
         };
-        int u = 0;
-        for (; u + kDepth <= units; u += kDepth) {
+        auto walk = [&](auto as_half) {
+            int u = 0;
+            for (; u + kDepth <= units; u += kDepth) {
+#pragma unroll
+                for (int d = 0; d < kDepth; d++) {
+                    multiply(d, as_half);
+                    request(d, c0, groups);
+                    if (gr == groups) end_of_step();
+                }
+                if (first < i) finish_steps();
+            }
 #pragma unroll
             for (int d = 0; d < kDepth; d++) {
-                multiply(d);
-                request(d, c0, groups);
-                if (gr == groups) end_of_step();
+                if (u + d < units) {
+                    multiply(d, as_half);
+                    if (gr == groups) end_of_step();
+                }
             }
             if (first < i) finish_steps();
+        };
+        if constexpr (Form::kHalf) {
+            if (fp16) walk(std::true_type{});
+            else walk(std::false_type{});
+        } else {
+            walk(std::false_type{});
         }
-#pragma unroll
-        for (int d = 0; d < kDepth; d++) {
-            if (u + d < units) {
-                multiply(d);
-                if (gr == groups) end_of_step();
-            }
-        }
-        if (first < i) finish_steps();
         int others = warp;
         const bool cut = gr != 0 && units > 0, mine = i > run_step || begun;       // the run ends inside a step; which this warp began
         if (cut) put(mine ? 0 : kDepth);

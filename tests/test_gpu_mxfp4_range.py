@@ -1,0 +1,80 @@
+"""Products of 4-bit weights where few rows of X meet the ends of the number range, against plain computations in 64 bits.
+
+Tolerances.  An output is its 32-bit sum rounded to BF16 once: off by at most 2^-8 of itself and, for the sum, by K additions that lose at
+most 2^-23 each of the sum of the terms' magnitudes; K halves of BF16's smallest step, 2^-134, for what lies below the normal numbers."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+# rows of X and the weight's shape: every form of the kernel for few rows (two tiles of the weight a step from 256 rows an SM on)
+FORMS = [(1, 40, 512), (3, 40, 2080), (8, 40, 2080), (1, 40000, 128), (8, 40000, 160), (8, 40000, 1056), (5, 3000, 4128), (9, 24003, 416), (16, 24000, 416), (16, 2100, 2080),
+         (17, 24002, 160), (24, 24002, 416), (24, 23700, 2080), (40, 130, 416)]
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    import bf16_huffman_infer_b200
+    return bf16_huffman_infer_b200
+
+
+def weight(pkg, M, K, seed, lo=120, hi=128):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, generator=g, device=DEV)
+    return codes, torch.randint(lo, hi, (M, K // 32), dtype=torch.uint8, generator=g, device=DEV)
+
+
+def within(y, want, mag, K):
+    err = (y.double() - want).abs()
+    bound = want.abs() * 2.0 ** -8 + mag * (K * 2.0 ** -23) + K * 2.0 ** -134
+    assert bool((err <= bound).all()), (float((err / bound.clamp(min=1e-300)).max()), int((err > bound).sum()))
+
+
+def gated64(z, mag, K):
+    """silu(g) u of projections in 64 bits, and how far the sums' errors may move it (|silu'| <= 1.1)"""
+    (g, u), (mg, mu) = z.chunk(2, -1), mag.chunk(2, -1)
+    a = g * torch.sigmoid(g)
+    slack = 1.1 * mg * K * 2.0 ** -23 * (u.abs() + mu * K * 2.0 ** -23) + a.abs() * mu * K * 2.0 ** -23
+    return a * u, slack + (a * u).abs() * 2.0 ** -14              # the function's own error, some units of 2^-23 of arguments
+
+
+@pytest.mark.parametrize("rows,M,K", FORMS)
+@pytest.mark.parametrize("spread", [30, 34, 45, 90])
+def test_x_far_apart_inside_a_group(pkg, rows, M, K, spread):
+    """Neighbouring values of X up to 2^spread apart, and weights that are zero wherever X is large: what is left is all that counts."""
+    codes, scales = weight(pkg, M, K, spread)
+    g = torch.Generator(device=DEV).manual_seed(rows + spread)
+    x = torch.randn(rows, K, generator=g, device=DEV)
+    small = torch.rand(K, generator=g, device=DEV) < 0.7
+    small[:2] = torch.tensor([False, True], device=DEV)
+    x = torch.where(small, x * 2.0 ** -spread, x)
+    x[:, 0] = 1.0
+    x = x.to(torch.bfloat16)
+    keep = torch.where(small[0::2], 0x0F, 0) + torch.where(small[1::2], 0xF0, 0)
+    codes[: M // 2 * 2: 2] &= keep.to(torch.uint8)               # every other row
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dense = w.get_weight().double()
+    want, mag = x.double() @ dense.T, x.double().abs() @ dense.abs().T
+    within(F.linear(x, w), want, mag, K)
+    if M % 2 == 0:
+        h, slack = gated64(want, mag, K)
+        err = (pkg.gated_mxfp4(x, w).double() - h).abs()
+        assert bool((err <= h.abs() * 2.0 ** -8 + slack + 2.0 ** -134).all())
+
+
+@pytest.mark.parametrize("rows", [1, 8, 16])
+def test_one_row_far_apart_leaves_the_others(pkg, rows):
+    """A chunk of K whose X is far apart in one row is multiplied in another way; every row keeps its tolerance, chunk by chunk."""
+    M, K = 24000, 16384                                          # X in several chunks from eight rows on
+    codes, scales = weight(pkg, M, K, 1)
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dense = w.get_weight()
+    for at in (5, K - 3):
+        x = torch.randn(rows, K, generator=torch.Generator(device=DEV).manual_seed(at), device=DEV)
+        x[rows // 2, at] = 2.0 ** -50
+        x = x.to(torch.bfloat16)
+        want = torch.cat([x.double() @ part.double().T for part in dense.split(4000)], 1)
+        mag = torch.cat([x.double().abs() @ part.double().abs().T for part in dense.split(4000)], 1)
+        within(F.linear(x, w), want, mag, K)
