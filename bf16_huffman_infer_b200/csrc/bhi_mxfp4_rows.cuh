@@ -13,8 +13,9 @@
 // it is, by the BF16 products of the next paragraph in a walk of its own.  (Looking for such
 // values costs most where X is most of the work: 1024 x 4096, 1 row 4.65 against 4.52 us, 151936 x 4096, 8 rows 62 against 61, 38000 x 12288, 24 rows
 // 118 against 115, gated 12288 x 4096, 16 rows 22.9 against 22.1.  A branch in every unit instead of the walk: 8 rows 66 us.)
-// With X's power of two, up to 2^23 in all, a block's sum can overflow under a scale of 2^105 or more where the output does not: outputs that are
-// not finite are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1 row 64 against 62 us.)
+// With X's power of two, up to 2^25 in four blocks, sums can overflow under a scale of 2^103 or more where the output does not: outputs that are
+// not finite, of weight rows with large scales, are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1
+// row 64 against 62 us.  Looking at the scales first: 151936 x 4096, 8 rows with a NaN in one 94 us, not 1255; 17 rows without 116 us, not 112.)
 // Where there are more than eight rows to bring to FP16 and few steps to use them in, that takes longer than it saves: codes are expanded to
 // BF16 with their scales, X is read as it is, and the products add up through all of K.
 //
@@ -108,8 +109,20 @@ __device__ __forceinline__ bool mx_below(uint32_t pair, uint32_t from) {
     return (lo != 0u && lo < from) || (hi != 0u && hi < from);
 }
 
-// One output by itself: weight row m, row `col` of X, products in 32 bits.
-__device__ __forceinline__ float mx_one_output(const MxRowsArgs &A, int m, int col) {
+// Whether weight row m has a scale of 2^65 or more (NaN scales aside): without one, a sum that is not finite is the output.
+__device__ __forceinline__ bool mx_row_of_large_scales(const MxRowsArgs &A, int m) {
+    const uint8_t *scales = A.W.scales + mx_scale_row(m, A.W.groups);
+    uint32_t found = 0u;
+    for (int g = 0; g < A.W.groups; g++) {
+        const uint32_t s = load_stream4(scales + static_cast<int64_t>(g) * kMxTileScales);
+        found |= s & (s << 1) & ~__vcmpeq4(s, 0xFFFFFFFFu);
+    }
+    return (found & 0x80808080u) != 0u;
+}
+
+// One output by itself: weight row m, row `col` of X, products in 32 bits.  Only if the weight row has large scales; otherwise what it `was`.
+__device__ __forceinline__ float mx_one_output(const MxRowsArgs &A, int m, int col, float was) {
+    if (!mx_row_of_large_scales(A, m)) return was;
     const uint8_t *codes = A.W.codes + mx_code_row(m, A.W.groups), *scales = A.W.scales + mx_scale_row(m, A.W.groups);
     const uint16_t *x = A.X + static_cast<int64_t>(col) * A.W.K;
     float sum = 0.f;
@@ -459,8 +472,9 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                         const int ma = kGated ? 8 * step + g : 16 * (MT * step + item / NT) + g, mb = kGated ? A.outs + ma : ma + 8;
 #pragma unroll 1
                         for (int k = 0; k < 4; k++) {
-                            if (!(k & 1 ? odd : even) || col + (k & 1) >= A.rows || (kGated ? ma : k < 2 ? ma : mb) >= A.outs) continue;
-                            const float one = mx_one_output(A, k < 2 ? ma : mb, col + (k & 1));
+                            const int m = k < 2 ? ma : mb;
+                            if (!(k & 1 ? odd : even) || col + (k & 1) >= A.rows || (kGated ? ma : m) >= A.outs) continue;
+                            const float one = mx_one_output(A, m, col + (k & 1), k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w);
                             if (k == 0) v.x = one;
                             if (k == 1) v.y = one;
                             if (k == 2) v.z = one;

@@ -2,6 +2,7 @@
 
 Tolerances.  An output is its 32-bit sum rounded to BF16 once: off by at most 2^-8 of itself and, for the sum, by K additions that lose at
 most 2^-23 each of the sum of the terms' magnitudes; K halves of BF16's smallest step, 2^-134, for what lies below the normal numbers."""
+import math
 
 import pytest
 import torch
@@ -78,3 +79,61 @@ def test_one_row_far_apart_leaves_the_others(pkg, rows):
         want = torch.cat([x.double() @ part.double().T for part in dense.split(4000)], 1)
         mag = torch.cat([x.double().abs() @ part.double().abs().T for part in dense.split(4000)], 1)
         within(F.linear(x, w), want, mag, K)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 16, 24])
+def test_sums_of_infinities_and_nans_in_x(pkg, rows):
+    """A row with infinities of one sign, of both, or a NaN, next to rows without: classes of results term by term."""
+    M, K = 24002, 416
+    codes, scales = weight(pkg, M, K, 7)
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dense = w.get_weight().double()
+    x = torch.randn(rows, K, generator=torch.Generator(device=DEV).manual_seed(rows), device=DEV).to(torch.bfloat16)
+    clean = F.linear(x, w)
+    for values in ([(3, math.inf)], [(3, math.inf), (200, math.inf)], [(3, math.inf), (5, -math.inf)], [(415, math.nan)], [(0, 3e38), (1, -math.inf)]):
+        v = x.clone()
+        for at, value in values:
+            v[0, at] = value
+        special = ~v[0].isfinite()
+        terms = v[0, special].double() * dense[:, special]
+        y = F.linear(v, w)
+        want = terms.sum(1)
+        assert torch.equal(y[0].isnan(), want.isnan()) and torch.equal(y[0][~want.isnan()].double(), want[~want.isnan()])
+        assert torch.equal(y[1:], clean[1:])
+
+
+def test_a_row_with_a_nan_takes_little_time_of_its_own(pkg):
+    """Its outputs are NaNs by the products as they are: nothing is computed once more (which took eighteen times as long)."""
+    M, K, rows = 40000, 4096, 8
+    w = pkg.MXFP4Weight.from_packed(*weight(pkg, M, K, 3))
+    x = torch.randn(rows, K, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    nan = x.clone()
+    nan[0, 5] = math.nan
+
+    def time(v):
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            for _ in range(20):
+                F.linear(v, w)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    time(x)
+    assert time(nan) < 5 * time(x)
+
+
+def test_overflow_inside_is_not_the_outputs(pkg):
+    """Scales near 2^104, under which the FP16 sums of four blocks overflow while the outputs, X being small, do not."""
+    for rows in (1, 8, 16):
+        for byte in (229, 231, 233, 250):
+            M, K = (24000, 512) if rows > 8 else (40, 512)
+            codes = torch.full((M, K // 2), 0x77, dtype=torch.uint8, device=DEV)
+            w = pkg.MXFP4Weight.from_packed(codes, torch.full((M, K // 32), byte, dtype=torch.uint8, device=DEV))
+            x = torch.full((rows, K), 2.0 ** -70 * 1.9921875, device=DEV, dtype=torch.bfloat16)
+            want = x.double().sum(1, keepdim=True) * 6 * 2.0 ** (byte - 127)
+            assert torch.equal(F.linear(x, w).double(), want.to(torch.bfloat16).double().expand(rows, M))
