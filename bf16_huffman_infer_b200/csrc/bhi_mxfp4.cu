@@ -91,9 +91,25 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_quantize_kernel(const T *W
 
 // ---- from the plain order ----------------------------------------------------------------------------------------------
 // Two codes a byte along a row, the even element in the low half, and a scale byte a block, to the order of the kernels; threads as above.
+// Scales of 2^126 and 2^127, under which some codes leave the range of BF16 and of 32-bit floats, are not stored, so that whatever multiplies by
+// codes and scales apart agrees with whatever multiplies by values: a block without such codes is the same values under 2^125, one with any
+// has infinities and is NaN, as in quantisation.
+
+// The codes of a word of a block under 2^(125 + up) as those under 2^125; those that have none make `beyond` true.
+__device__ __forceinline__ uint32_t mx_codes_under_125(uint32_t word, uint32_t up, bool &beyond) {
+    // of 0, 0.5, 1, 1.5, 2, 3, 4, 6 the codes of twice and four times the value
+    const uint32_t codes = up == 1u ? 0x00765420u : 0x00007640u, most = up == 1u ? 5u : 3u;
+    uint32_t out = word & 0x88888888u;
+    for (int i = 0; i < 32; i += 4) {
+        const uint32_t magnitude = (word >> i) & 7u;
+        beyond |= magnitude > most;
+        out |= ((codes >> (4 * magnitude)) & 7u) << i;
+    }
+    return out;
+}
 __global__ void __launch_bounds__(kMxQuantThreads) mx_layout_kernel(const uint8_t *packed, const uint8_t *packed_scales, int M, int K, int groups, uint8_t *codes, uint8_t *scales) {
     const int at = blockIdx.x * blockDim.x + threadIdx.x;                // word of a row
-    if (at >= groups * 16) return;
+    const bool in_row = at < groups * 16;
     const int g = at >> 4, j = (at >> 2) & 3, t = at & 3;
     const int tiles16 = (M + 15) / 16 * 16;
     for (int m0 = blockIdx.y * kMxQuantRows; m0 < tiles16; m0 += gridDim.y * kMxQuantRows) {
@@ -106,6 +122,21 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_layout_kernel(const uint8_
                 byte[r] = __ldg(packed_scales + static_cast<int64_t>(m0 + r) * (K / 32) + (at >> 2));
             }
         }
+        bool high = false;
+#pragma unroll
+        for (int r = 0; r < kMxQuantRows; r++) high |= byte[r] == 253u || byte[r] == 254u;
+        if (__any_sync(0xFFFFFFFFu, high)) {
+#pragma unroll
+            for (int r = 0; r < kMxQuantRows; r++) {
+                bool beyond = false;
+                if (byte[r] == 253u || byte[r] == 254u) word[r] = mx_codes_under_125(word[r], byte[r] - 252u, beyond), byte[r] = 252u;
+                uint32_t nan = beyond ? 1u : 0u;                             // anywhere in the block: its four threads
+                nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 1);
+                nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 2);
+                if (nan) byte[r] = 255u;
+            }
+        }
+        if (!in_row) continue;
 #pragma unroll
         for (int r = 0; r < kMxQuantRows; r++) {
             uint32_t even = word[r] & 0x0F0F0F0Fu, odd = (word[r] >> 4) & 0x0F0F0F0Fu;      // a nibble a byte: side by side, in two steps

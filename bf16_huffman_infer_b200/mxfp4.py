@@ -95,7 +95,9 @@ class MXFP4Weight(nn.Module):
     @classmethod
     def from_packed(cls, codes: Tensor, scales: Tensor) -> "MXFP4Weight":
         """From the plain order: ``codes`` u8 ``[M, K/2]`` (the even element in the low half of a byte) and ``scales`` u8 ``[M, K/32]``
-        (E8M0; also as ``torch.float8_e8m0fnu``), on their device."""
+        (E8M0; also as ``torch.float8_e8m0fnu``), on their device.  A block with values beyond BF16's range (scale bytes 253 and 254:
+        4 or 6 times 2^126, 2 and more times 2^127) becomes NaN, as one with an infinity does in :meth:`compress`; without them it is kept
+        under the scale byte 252."""
         if scales.dtype == torch.float8_e8m0fnu:
             scales = scales.view(torch.uint8)
         if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.size(1) % 16 \
@@ -109,9 +111,10 @@ class MXFP4Weight(nn.Module):
             codes = codes.contiguous()
             ops.mxfp4_from_packed(codes.clone() if codes.data_ptr() % 4 else codes, scales.contiguous(), c, s)
             return cls(c, s, M, K)
+        codes, scales = _within_range(codes.view(M, -1, 16), scales)
         s = F.pad(scales, (0, groups * 4 - K // 32, 0, tiles * 16 - M))
         # a NaN block holds zero codes
-        c = codes.view(M, -1, 16).masked_fill((scales == 255)[..., None], 0).view(M, -1)
+        c = codes.masked_fill((scales == 255)[..., None], 0).view(M, -1)
         c = F.pad(c, (0, groups * 64 - K // 2, 0, tiles * 16 - M)).view(tiles, 16, groups, 4, 4, 4)     # tile, row, group, block, quarter, byte
         low, high = c & 15, c >> 4
         byte = [low[..., 0] | low[..., 1] << 4, low[..., 2] | low[..., 3] << 4, high[..., 0] | high[..., 1] << 4, high[..., 2] | high[..., 3] << 4]
@@ -119,7 +122,7 @@ class MXFP4Weight(nn.Module):
         return cls(c, s.view(tiles, 16, groups, 4).transpose(1, 2).contiguous(), M, K)
 
     def packed(self) -> Tuple[Tensor, Tensor]:
-        """``(codes u8 [M, K/2], scales u8 [M, K/32])`` in the plain order; the inverse of :meth:`from_packed`."""
+        """``(codes u8 [M, K/2], scales u8 [M, K/32])`` in the plain order; the inverse of :meth:`from_packed` (scale bytes 253 and 254 aside)."""
         M, K = self.shape
         tiles, groups = self.codes.shape[:2]
         c = self.codes.view(tiles, groups, 16, 4, 4, 4).permute(0, 2, 1, 4, 3, 5).reshape(tiles * 16, groups * 16, 4)
@@ -127,6 +130,19 @@ class MXFP4Weight(nn.Module):
         byte = [low[..., 0] | low[..., 2] << 4, high[..., 0] | high[..., 2] << 4, low[..., 1] | low[..., 3] << 4, high[..., 1] | high[..., 3] << 4]
         c = torch.stack(byte, -1).view(tiles * 16, groups * 64)[:M, :K // 2].contiguous()
         return c, self.scales.transpose(1, 2).reshape(tiles * 16, groups * 4)[:M, :K // 32].contiguous()
+
+
+def _within_range(codes: Tensor, scales: Tensor) -> Tuple[Tensor, Tensor]:
+    """Blocks ``[M, blocks, 16]`` without the scale bytes 253 and 254: the same values under 252, or NaN where there is none."""
+    up = torch.where((scales == 253) | (scales == 254), scales.int() - 252, 0)[..., None]
+    if not bool(up.any()):
+        return codes, scales
+    # of 0, 0.5, 1, 1.5, 2, 3, 4, 6 the codes of once, twice and four times the value; 8: beyond the range
+    table = torch.tensor([[0, 1, 2, 3, 4, 5, 6, 7], [0, 2, 4, 5, 6, 7, 8, 8], [0, 4, 6, 7, 8, 8, 8, 8]], dtype=torch.uint8, device=codes.device)
+    low, high = table[up, (codes & 7).int()], table[up, (codes >> 4 & 7).int()]
+    beyond = ((low | high) & 8 != 0).any(-1)
+    scales = torch.where(up[..., 0] > 0, 252, scales).masked_fill(beyond, 255)
+    return codes & 0x88 | low & 7 | (high & 7) << 4, scales.to(torch.uint8)
 
 
 def _padded(M: int, K: int) -> Tuple[int, int]:

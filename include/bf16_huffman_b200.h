@@ -284,7 +284,8 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
  *
  *   codes   u8 [T, G, 16, 4, 16]  rows of a tile, quarters t, 16 bytes [4 blocks j][4 bytes]: elements 8 t .. 8 t + 7 of block j,
  *                               nibble i (from the lowest) element 2 i, nibble 4 + i element 2 i + 1
- *   scales  u8 [T, G, 16, 4]      byte s of each block: 2^(s - 127); 255 is NaN (its codes must be zero)
+ *   scales  u8 [T, G, 16, 4]      byte s of each block: 2^(s - 127), at most 252 (under 253 and 254 some codes leave BF16's range); or 255,
+ *                               NaN (its codes must be zero)
  *
  * Padding must be zeros; bhi_mxfp4_quantize writes it.  Sums are 32-bit floats, each output is rounded to BF16 once.  Up to
  * BHI_MXFP4_MAX_ROWS rows of X, dY and the like. */
@@ -303,7 +304,8 @@ int bhi_ans_emit_pass(const uint16_t *W, int M, int K, int split_k, const uint32
 int bhi_mxfp4_quantize(const void *W, int dtype, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
 
 /* The same from the plain order: packed u8 [M, K / 2], the even element in the low half of a byte, and packed_scales u8 [M, K / 32].  The codes of
- * blocks whose scale is NaN become zero. */
+ * blocks whose scale is NaN become zero.  Blocks with scale byte 253 or 254 become the same values under 252, or NaN if any of their
+ * values is beyond BF16's range. */
 int bhi_mxfp4_from_packed(const uint8_t *packed, const uint8_t *packed_scales, int M, int K, uint8_t *codes, uint8_t *scales, void *stream);
 
 /* Y bf16 [M, K]: the values (exact but for scales beyond BF16's range). */

@@ -137,3 +137,57 @@ def test_overflow_inside_is_not_the_outputs(pkg):
             x = torch.full((rows, K), 2.0 ** -70 * 1.9921875, device=DEV, dtype=torch.bfloat16)
             want = x.double().sum(1, keepdim=True) * 6 * 2.0 ** (byte - 127)
             assert torch.equal(F.linear(x, w).double(), want.to(torch.bfloat16).double().expand(rows, M))
+
+
+@pytest.mark.parametrize("rows,M,K", FORMS)
+@pytest.mark.parametrize("byte", [191, 192, 231, 252, 253, 254, 255])
+def test_large_scales_in_some_rows(pkg, rows, M, K, byte):
+    """Scales from 2^64 on in a few blocks, those among them under which codes leave the range: every form agrees with the dense matrix, zeros in X
+    included, and the other rows of the weight keep their tolerance."""
+    codes, scales = weight(pkg, M, K, byte)
+    g = torch.Generator(device=DEV).manual_seed(rows + byte)
+    at = torch.randint(0, M, (5,), generator=g, device=DEV)
+    scales[at, torch.randint(0, K // 32, (5,), generator=g, device=DEV)] = byte
+    x = torch.randn(rows, K, generator=g, device=DEV) * 2.0 ** -30
+    x[:, torch.rand(K, generator=g, device=DEV) < 0.3] = 0.0
+    x[0] = 0.0
+    x = x.to(torch.bfloat16)
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dense = w.get_weight()
+    assert bool(dense.isnan().any()) == (byte > 252) and not bool(dense.isinf().any())
+    wide = dense.double()
+    clean = torch.where(wide.isfinite(), wide, 0)
+    bad = torch.nonzero(~wide.isfinite().all(1))[:, 0]
+    want, mag = x.double() @ clean.T, x.double().abs() @ clean.abs().T
+    for m in bad.tolist():                                       # NaNs term by term
+        want[:, m] = (x.double() * wide[m]).sum(1)
+    y = F.linear(x, w)
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf()) and torch.equal(y[y.isinf()].double(), want[y.isinf()])
+    fine = want.isfinite()
+    within(y[fine], want[fine], mag[fine], K)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 16, 40])
+@pytest.mark.parametrize("code,byte", [(7, 253), (6, 253), (5, 253), (4, 254), (3, 254), (15, 254), (11, 254), (1, 254)])
+def test_codes_beyond_the_range(pkg, rows, code, byte):
+    """Values that BF16 just has and just has not, few rows and many alike."""
+    M = 24000 if rows == 16 else 32                              # FP16 products and BF16 ones of few rows
+    w = pkg.MXFP4Weight.from_packed(torch.full((M, 64), code * 17, dtype=torch.uint8, device=DEV), torch.full((M, 4), byte, dtype=torch.uint8, device=DEV))
+    dense = w.get_weight().double()
+    value = [0, 0.5, 1, 1.5, 2, 3, 4, 6][code & 7] * 2.0 ** (byte - 127) * (-1 if code & 8 else 1)
+    fits = abs(value) < 2.0 ** 128
+    assert bool((dense == value).all() if fits else dense.isnan().all())
+    for x in (torch.full((rows, 128), 2.0 ** -100, device=DEV), torch.eye(128, device=DEV)[:rows] * 2.0 ** -60, torch.zeros(rows, 128, device=DEV)):
+        x = x.to(torch.bfloat16)
+        y = F.linear(x, w).double()
+        want = x.double().sum(1, keepdim=True).expand(rows, M) * value
+        assert torch.equal(y, want) if fits else bool(y.isnan().all())
+
+
+def test_plain_order_beyond_the_range_as_on_the_host(pkg):
+    from test_mxfp4_range import every_code_under
+    for byte in range(250, 256):
+        codes, scales = every_code_under(byte)
+        codes, scales = codes[:528].view(-1, 3 * 16), scales[:528].view(-1, 3)      # blocks side by side
+        want, got = pkg.MXFP4Weight.from_packed(codes, scales), pkg.MXFP4Weight.from_packed(codes.to(DEV), scales.to(DEV))
+        assert torch.equal(got.codes.cpu(), want.codes) and torch.equal(got.scales.cpu(), want.scales)
