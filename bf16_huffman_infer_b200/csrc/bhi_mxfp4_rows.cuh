@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                 __syncwarp();
                 if (lane < A.rows) bulk_copy_g2s(base + lane * row_bytes, A.X + static_cast<int64_t>(lane) * A.W.K + c0 * kMxGroup, x_bytes, x_bar);
             }
-            mx_wait(x_bar, x_phase, &dead, 10);
+            mx_wait(x_bar, x_phase, &dead, 11);
             x_phase ^= 1u;
         };
         auto pad_x = [&]() {                                                 // past the last column: zeros

@@ -68,7 +68,10 @@ int bhi_set_launch_overlap(int on);
 /* Reads and clears the device-side status word of the current device.  0 = no incident; otherwise
  * the last bounded wait that ran out inside a kernel: 1 a record's bulk copy (the record was
  * skipped), 2 the prepared-table copy, 3-7 the tensor-core path's stage / accumulator barriers,
- * 8 peers not ready and 9 peers not done in an exchange kernel; or 10, no wait: shared memory does
+ * 8 peers not ready and 9 peers not done in an exchange kernel, 11 X and 12 another warp's part of a
+ * sum in a 4-bit product of few rows, 20-25 a 4-bit product in tiles or its gradient (20 a place of
+ * the ring, 21 an accumulator, 22 X or dY, 23 a place of the expanded weight, 24 the sums, 25 the
+ * expanded weight): the outputs of that launch are invalid.  Or 10, no wait: shared memory does
  * not start where the fused kernel's tables are read, and all records were decoded from global
  * memory, rightly but several times as slowly.  The kernels always run to their end.  Synchronises the device; meant for tests and post-mortems, not for the launch path. */
 int bhi_debug_status(int *status_out);
