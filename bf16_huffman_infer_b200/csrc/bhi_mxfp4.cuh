@@ -44,15 +44,16 @@ __host__ __device__ __forceinline__ int64_t mx_scale_row(int m, int groups) {
     return static_cast<int64_t>(m >> 4) * groups * kMxTileScales + (m & 15) * 4;
 }
 
-// A wait of at most about a second; when one runs out, the kernel's status word is set and no other wait of the CTA goes on: the CTA
-// runs to its end with whatever it has.
+// A wait of at most about a second, counted from the end of the kernel before (which has its own limits, more than one of them: for a peer's
+// signals, say) where this one runs ahead of it.  When one runs out, the kernel's status word is set and no other wait of the CTA goes on: the
+// CTA runs to its end with whatever it has.
 __device__ __forceinline__ void mx_wait(uint32_t bar, uint32_t parity, int *dead, int status) {
     uint64_t t0 = 0;
     for (uint32_t i = 1; !mbar_try_wait(bar, parity); i++) {
         if ((i & 1023u) != 0u) continue;
         if (*static_cast<volatile int *>(dead)) return;
+        if (t0 == 0) pdl_wait(), t0 = global_ns();
         const uint64_t now = global_ns();
-        if (t0 == 0) t0 = now;
         if (now - t0 > 1000000000ull) {
             atomicExch(dead, 1);
             atomicExch(&g_staged_status, status);
