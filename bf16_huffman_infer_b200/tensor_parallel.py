@@ -118,7 +118,7 @@ class PeerArena:
     output ``[8, out_features]``.
 
     Usage: ``slot = arena.add(out_features)`` for every layer (same order on every rank), then
-    ``arena.commit()`` once (a collective call), then ``arena.output(slot)`` / ``arena.peers(slot)``.
+    ``arena.commit()`` once (a collective call; without layers it does nothing), then ``arena.output(slot)`` / ``arena.peers(slot)``.
     A single-rank arena (``group=None`` without an initialised process group, or ``world == 1``) uses
     plain device memory, so the same kernels run on one GPU.
     """
@@ -149,7 +149,10 @@ class PeerArena:
         return len(self._sizes) - 1
 
     def commit(self) -> None:
-        assert self.buffer is None and self._total > 0
+        assert self.buffer is None, "the arena is already committed"
+        if self._total == 0:                  # no layer exchanges (4-bit weights, say): nothing to map, on any rank
+            self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
+            return
         if self.world > 1:
             import torch.distributed._symmetric_memory as symm_mem
             self.buffer = symm_mem.empty(self._total, dtype=torch.uint8, device=self.device)
