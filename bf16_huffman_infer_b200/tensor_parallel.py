@@ -19,6 +19,7 @@ from typing import List, Optional, Tuple
 import torch
 import torch.distributed as dist
 from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .functional import FUSED_MAX_ROWS, ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight
@@ -75,12 +76,56 @@ def shard_rows(weight: HuffmanWeight, rank: int, world: int) -> HuffmanWeight:
                          code_lengths=weight.code_lengths, **kwargs)
 
 
+def _gather(y: Tensor, world: int, group: Optional[dist.ProcessGroup]) -> Tensor:
+    """The ranks' slices ``[..., features / world]`` side by side."""
+    flat = y.reshape(-1, y.shape[-1]).contiguous()
+    gathered = torch.empty(world, *flat.shape, dtype=flat.dtype, device=flat.device)
+    if flat.is_cuda:
+        dist.all_gather_into_tensor(gathered, flat, group=group)
+    else:                                   # CPU process groups (tests): list form
+        dist.all_gather(list(gathered.unbind(0)), flat, group=group)
+    return gathered.permute(1, 0, 2).reshape(*y.shape[:-1], world * y.shape[-1])
+
+
+class _Gathered(torch.autograd.Function):
+    """:func:`_gather`; its gradient, which every rank has whole, is this rank's slice of it."""
+
+    @staticmethod
+    def forward(ctx, y, world, group):
+        ctx.rows = row_range(world * y.shape[-1], dist.get_rank(group), world)
+        return _gather(y, world, group)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        lo, hi = ctx.rows
+        return dy[..., lo:hi], None, None
+
+
+class _Shared(torch.autograd.Function):
+    """An input that every rank multiplies by rows of its own: the gradient is the sum of theirs, in 32 bits."""
+
+    @staticmethod
+    def forward(ctx, x, group):
+        ctx.group = group
+        return x.view_as(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx):
+        total = dx.to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+        dist.all_reduce(total, group=ctx.group)
+        return total.to(dx.dtype), None
+
+
 class RowShardedLinear(nn.Module):
     """A :class:`CompressedLinear` holding only this rank's output rows; ``forward`` returns the full output.
 
     The local slice is computed by the fused kernel (or decode + GEMM above 8 rows) and the slices
     of all ranks are gathered along the feature dimension.  Row counts must be equal across ranks
-    (``out_features % world == 0``) so that a single ``all_gather_into_tensor`` suffices.
+    (``out_features % world == 0``) so that a single ``all_gather_into_tensor`` suffices.  The output of a 4-bit layer is
+    differentiable with respect to the input (once): the ranks take their slices of its gradient, which each has whole, and add up what
+    they make of them, so a backward pass is a collective too.
     """
 
     def __init__(self, local: CompressedLinear, out_features: int, group: Optional[dist.ProcessGroup] = None):
@@ -98,18 +143,12 @@ class RowShardedLinear(nn.Module):
         return cls(CompressedLinear(shard_rows(full.weight, rank, world), bias), M, group)
 
     def forward(self, input: Tensor) -> Tensor:
-        y = self.local(input)
         world = dist.get_world_size(self.group) if dist.is_initialized() else 1
         if world == 1:
-            return y
-        lead = y.shape[:-1]
-        flat = y.reshape(-1, y.shape[-1]).contiguous()
-        gathered = torch.empty(world, *flat.shape, dtype=flat.dtype, device=flat.device)
-        if flat.is_cuda:
-            dist.all_gather_into_tensor(gathered, flat, group=self.group)
-        else:                                   # CPU process groups (tests): list form
-            dist.all_gather(list(gathered.unbind(0)), flat, group=self.group)
-        return gathered.permute(1, 0, 2).reshape(*lead, self.out_features)
+            return self.local(input)
+        if input.requires_grad and torch.is_grad_enabled() and isinstance(getattr(self.local, "weight", None), MXFP4Weight):
+            return _Gathered.apply(self.local(_Shared.apply(input, self.group)), world, self.group)
+        return _gather(self.local(input), world, self.group)
 
 
 class PeerArena:
