@@ -21,7 +21,7 @@ from safetensors import safe_open
 from safetensors.torch import save_file
 from torch import nn
 
-from .functional import (ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight, _FusedSlice, _is_gated_mlp)
+from .functional import (ANSWeight, CompressedLinear, FusedCompressedLinear, HuffmanWeight, _FusedSlice, _gated_activation)
 from .mxfp4 import GatedMLP, GatedMXFP4, MXFP4Weight
 
 __all__ = ["save_compressed", "load_compressed", "compressed_manifest"]
@@ -106,7 +106,7 @@ def _validate(model: nn.Module, manifest: Dict) -> None:
             check_shape(name, meta, splits[-1][1], olds[0].in_features)
         elif meta.get("kind") == "gated":
             old = names.get(name)
-            act = None if old is None else _is_gated_mlp(old)
+            act = None if old is None else _gated_activation(old)       # of any type, on any device: its weights are not looked at
             if act is None or act != meta.get("activation") or meta.get("algo") != MXFP4Weight.algo:
                 raise ValueError(f"checkpoint names {name!r}, which is not a feed-forward block with the activation {meta.get('activation')!r}")
             check_shape(name, meta, 2 * old.gate_proj.out_features, old.gate_proj.in_features)
@@ -144,14 +144,19 @@ def load_compressed(model: nn.Module, path: str, strict: bool = True) -> nn.Modu
     for name, meta in manifest["modules"].items():             # blocks before the projections inside them
         if meta["kind"] == "gated":
             bias = nn.Parameter(torch.empty(meta["shape"][0], dtype=state[name + ".gate_up.bias"].dtype), requires_grad=False) if meta["bias"] else None
-            model.set_submodule(name, GatedMLP(GatedMXFP4(_empty_weight(meta), bias, meta["activation"]), model.get_submodule(name).down_proj))
+            old = model.get_submodule(name)
+            model.set_submodule(name, GatedMLP(GatedMXFP4(_empty_weight(meta), bias, meta["activation"]), old.down_proj).train(old.training))
     for name, meta in manifest["modules"].items():
         if meta["kind"] == "gated":
             continue
         weight = _empty_weight(meta)
         if meta["kind"] == "linear":
             old = model.get_submodule(name)
-            bias = nn.Parameter(torch.empty_like(old.bias), requires_grad=False) if meta["bias"] else None
+            bias = None
+            if meta["bias"] and meta["algo"] == MXFP4Weight.algo:      # its products take biases of the saved type only
+                bias = nn.Parameter(torch.empty(old.out_features, dtype=state[name + ".bias"].dtype), requires_grad=False)
+            elif meta["bias"]:
+                bias = nn.Parameter(torch.empty_like(old.bias), requires_grad=False)
             model.set_submodule(name, CompressedLinear(weight, bias))
         else:
             rows = meta["splits"][-1][1]
