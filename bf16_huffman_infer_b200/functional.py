@@ -731,7 +731,8 @@ _CODERS = {"huffman": (HuffmanWeight,), "ans": (ANSWeight,), "smallest": (Huffma
 def _compress_for(a: Tensor, algo: str) -> HuffmanWeight:
     """``a`` compressed as ``algo`` says, on the device it is on."""
     if algo == MXFP4Weight.algo:
-        assert a.dtype == torch.bfloat16, a.dtype          # its products take activations of this type
+        if a.dtype != torch.bfloat16:                      # its products take activations of this type
+            raise AssertionError(f"layers to be rounded to 4 bits have BF16 weights, not {a.dtype}")
         return MXFP4Weight.compress(a, to_cpu=not a.is_cuda)
     assert algo in _CODERS
     return _compress(a, get_block_size_n(a)[0], _CODERS[algo], to_cpu=not a.is_cuda)

@@ -68,7 +68,8 @@ class MXFP4Weight(nn.Module):
     def get_weight(self) -> Tensor:
         """Dense BF16 ``[M, K]``: exactly the values that the products use."""
         b = self.__dict__["_buffers"]
-        assert b["codes"].is_cuda
+        if not b["codes"].is_cuda:
+            raise AssertionError("the dense matrix of a 4-bit weight is made on a CUDA device")
         return ops.dense_mxfp4(b["codes"], b["scales"], self.out_features, self.in_features)
 
     # -- making one ---------------------------------------------------------------------------
@@ -76,7 +77,8 @@ class MXFP4Weight(nn.Module):
     def compress(cls, a: Tensor, to_cpu: bool = True) -> "MXFP4Weight":
         """``a`` (BF16, FP16 or FP32) rounded to the format: the scale of a block is ``2^(floor(log2 max|v|) - 2)``, values go to
         the nearest code (ties to even) and saturate at 6 scales.  A block with an infinity or a NaN becomes NaN."""
-        assert a.dim() == 2 and a.dtype in _TYPES, (a.shape, a.dtype)
+        if a.dim() != 2 or a.dtype not in _TYPES:
+            raise ValueError(f"want a matrix of BF16, FP16 or FP32, got {a.dtype} {tuple(a.shape)}")
         a = a.detach()
         if not a.is_cuda and not torch.cuda.is_available():
             raise RuntimeError("bf16_huffman_infer_b200 needs a CUDA device: there is no CPU implementation")
@@ -177,9 +179,17 @@ def _plain(x: Tensor) -> Tensor:
     return x.clone() if x.data_ptr() % 16 else x
 
 
+def _under_autocast(input: Tensor, bias: Optional[Tensor]) -> Tuple[Tensor, Optional[Tensor]]:
+    """Input and bias as ``torch.autocast`` to BF16 hands them to ``F.linear``; as they are without it."""
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") is torch.bfloat16:
+        input, bias = (t.to(torch.bfloat16) if t is not None and t.is_cuda and t.dtype in _TYPES else t for t in (input, bias))
+    return input, bias
+
+
 def _check(input: Tensor, weight: "MXFP4Weight", bias: Optional[Tensor]) -> None:
     """What the operators do not see for themselves."""
-    assert input.is_cuda and input.dtype is torch.bfloat16, (input.device, input.dtype)
+    if not input.is_cuda or input.dtype is not torch.bfloat16:
+        raise AssertionError(f"products on 4-bit weights take BF16 tensors on a CUDA device, not {input.dtype} on {input.device}")
     if input.dim() < 1 or input.size(-1) != weight.in_features:
         raise RuntimeError(f"input of shape {tuple(input.shape)} does not fit a weight of {weight.in_features} columns")
     if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (weight.out_features,) or bias.device != input.device):
@@ -298,7 +308,11 @@ def _batched(info, in_dims, x: Tensor, bias: Optional[Tensor], call: Callable) -
 
 def linear_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = None) -> Tensor:
     """``F.linear`` on a 4-bit weight: ``input`` BF16 ``[..., K]``, any number of rows; the bias (BF16, a value for each output) is part
-    of the 32-bit sum.  Differentiable with respect to the input and the bias."""
+    of the 32-bit sum.  Differentiable with respect to the input and the bias, also by forward-mode derivatives and under the
+    transformations of ``torch.func``.  Under ``torch.autocast`` to BF16, FP32 and FP16 inputs and biases are cast; other types are
+    refused."""
+    if input.dtype is not torch.bfloat16 or (bias is not None and bias.dtype is not torch.bfloat16):
+        input, bias = _under_autocast(input, bias)
     _check(input, weight, bias)
     if _transformed():
         return _LinearTransformed.apply(input, _Held(weight), bias)
@@ -343,12 +357,15 @@ def _gated(x: Tensor, weight: MXFP4Weight, bias: Optional[Tensor], activation: i
 def gated_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = None, activation: str = "silu") -> Tensor:
     """``act(x G^T + b_g) * (x U^T + b_u)`` for the stacked weight ``[G; U]`` (gate rows first) and bias ``[b_g; b_u]``: BF16 ``[..., M/2]``
     from BF16 ``[..., K]`` in one kernel, the projections kept in 32 bits.  ``activation``: ``"silu"``, ``"gelu"`` or
-    ``"gelu_tanh"``.  Differentiable once with respect to the input and the bias; a call that may be differentiated keeps
-    the projections (8 bytes a gated value) for the backward pass."""
+    ``"gelu_tanh"``.  Differentiable once with respect to the input and the bias, by backward passes alone (forward-mode derivatives
+    and the transformations of ``torch.func`` are refused); a call that may be differentiated keeps the projections (8 bytes a
+    gated value) for the backward pass.  ``torch.autocast`` as in :func:`linear_mxfp4`."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
     if weight.out_features % 2:
         raise RuntimeError(f"a stacked weight has an even number of rows, not {weight.out_features}")
+    if input.dtype is not torch.bfloat16 or (bias is not None and bias.dtype is not torch.bfloat16):
+        input, bias = _under_autocast(input, bias)
     _check(input, weight, bias)
     if _recorded(input, bias) or _transformed():
         return _Gated.apply(input, _Held(weight), bias, ACTIVATIONS[activation])
