@@ -174,7 +174,10 @@ __global__ void __launch_bounds__(kMxQuantThreads) mx_dense_kernel(MxWeight W, u
 }
 
 // ---- the gated pair's gradient: dg = dh u act'(g), du = dh act(g) --------------------------------------------------------
-// Bound by memory: 8 bytes of projections and 2 of dh in, 4 out.  A thread takes kVec neighbours of a row.
+// Bound by memory: 8 bytes of projections and 2 of dh in, 4 out.  A thread takes kVec neighbours of a row.  Everything up to the store is 32 bits
+// wide; dg and du are rounded to BF16 because they are the operand of a BF16 product, of which no other type is exact on the expanded weight
+// and as fast.  With the rounding of dx after it that makes the error of dx 0.0023 of its norm where one rounding makes 0.0017 (12288 x 4096, 2048 rows);
+// two BF16 parts a value would take the product's time twice.
 constexpr int kMxPairThreads = 256;
 
 template <int kVec>
@@ -227,11 +230,11 @@ static int mx_check(const void *codes, const void *scales, int M, int K) {
 static MxWeight mx_weight(const uint8_t *codes, const uint8_t *scales, int M, int K) { return {codes, scales, M, K, (K + kMxGroup - 1) / kMxGroup}; }
 
 // Whether a product takes the kernel for few rows.  Its rate is the memory's where the weight is most of the traffic (16 rows: 12288 x 4096 14.0
-// against 19.3 us, 4096 x 4096 8.8 against 10.3).  From nine rows on the tiles are faster where the weight is small (1024 x 1024, 9 rows 4.2
-// against 5.9 us, 2048 x 2048 5.8 against 6.5; 4096 x 2048 7.5 against 6.7) and where every SM would read a large X for few outputs (2560 x
-// 9728, 16 rows 14.0 against 20.1, 3584 x 18944, 9 rows 24.3 against 27.4; 2048 x 8192, 9 rows 11.9 against 9.9).  From 17 rows on ten steps an SM have to
-// pay for X's conversion (24 rows: 24576 x 4096 31.4 against 34.2, 38000 x 12288 115 against 148, gated 18944 x 3584 35.6 against 36.3); with
-// 32 rows nothing does (24576 x 4096 48 against 34).
+// against 19.3 us, 4096 x 4096 8.9 against 10.3).  From nine rows on the tiles are faster where the weight is small (1024 x 1024, 9 rows 4.1
+// against 5.9 us, 2048 x 2048 5.8 against 6.5; 4096 x 2048 7.4 against 6.7) and where every SM would read a large X for few outputs (2560 x
+// 9728, 16 rows 14.0 against 20.3, 3584 x 18944, 9 rows 24.3 against 27.6; 2048 x 8192, 9 rows 11.8 against 10.1).  From 17 rows on ten steps an SM have to
+// pay for X's conversion (24 rows: 24576 x 4096 33.6 against 34.3, 38000 x 12288 123 against 148, gated 18944 x 3584 36.8 against 36.2, at 20 rows 33.3
+// against 36.1); with 32 rows nothing does (24576 x 4096 48 against 34).
 static bool mx_few_rows(int rows, int M, int K) {
     if (rows <= 8) return true;
     if (rows > 16) return rows <= kMxRowsMost && M >= 160 * sm_count();

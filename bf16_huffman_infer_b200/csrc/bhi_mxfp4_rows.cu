@@ -52,16 +52,17 @@ int mx_rows_launch(const MxWeight &W, const uint16_t *X, const uint16_t *bias, u
     a.W = W, a.X = X, a.bias = bias, a.Y = Y, a.pre = pre, a.rows = rows, a.outs = gated ? W.M / 2 : W.M, a.activation = activation;
     if (rows > 16) return gated ? launch<MxRowsForm<1, 3, 16, 1, 2, true>>(a, st) : launch<MxRowsForm<1, 3, 16, 1, 2, false>>(a, st);
     if (rows > 8) {
-        // FP16 where an SM has ten steps or more (16 rows: 151936 x 4096 87 against 108 us, 64 steps; gated 12288 x 4096 22.2 against 22.9, ten; 12288 x
-        // 4096 15.1 against 14.0, five; gated 4096 x 2048 9.2 against 7.7, four)
+        // FP16 where an SM has ten steps or more (16 rows: 151936 x 4096 85 against 108 us, 64 steps; 32000 x 4096 25.3 against 26.9, 13; gated 12288 x
+        // 4096 23.1 both, ten; 12288 x 4096 16.2 against 14.0, five; gated 4096 x 2048 9.3 against 7.6, three)
         const bool half = (a.outs + (gated ? 7 : 15)) / (gated ? 8 : 16) >= 10 * sm_count();
         if (gated) return half ? launch<MxRowsForm<1, 2, 16, 1, 3, true>>(a, st) : launch<MxRowsForm<1, 2, 16, 1, 4, true, false>>(a, st);
         return half ? launch<MxRowsForm<1, 2, 16, 1, 3, false>>(a, st) : launch<MxRowsForm<1, 2, 16, 1, 4, false, false>>(a, st);
     }
     if (gated) return launch<MxRowsForm<1, 1, 16, 1, 3, true>>(a, st);
-    // Two tiles a step share X's fragments (151936 x 4096, 8 rows 64 against 70 us) where every SM has eight steps of them.  Where X is small, two CTAs
-    // an SM: the next kernel's are there as soon as one of them ends (1 row: 4096 x 4096 5.9 against 6.5 us, 37984 x 4096 18.9 against 20.6); else
-    // one, which brings and converts X once (4096 x 12288, 1 row 10.1 against 11.1; 12288 x 4096, 8 rows 10.6 against 12.8; gated, 4 rows 15.2 against 16.4).
+    // Two tiles a step share X's fragments (151936 x 4096, 8 rows 62 against 65 us; fewer steps: 37984 x 4096, 8 rows 21.7 against 20.9) where every SM
+    // has eight steps of them.  Where X is small, two CTAs an SM: the next kernel's are there as soon as one of them ends (1 row: 4096 x 4096 6.1 against
+    // 6.7 us, 37984 x 4096 19.5 against 20.0); else one, which brings and converts X once (4096 x 12288, 1 row 10.8 against 11.4; 12288 x 4096, 8 rows
+    // 11.4 against 14.2).
     const bool many = W.M >= 256 * sm_count();
     if (static_cast<int64_t>(rows) * W.K <= 8192) return many ? launch<MxRowsForm<2, 1, 8, 2, 2, false>>(a, st) : launch<MxRowsForm<1, 1, 8, 2, 4, false>>(a, st);
     return many ? launch<MxRowsForm<2, 1, 16, 1, 2, false>>(a, st) : launch<MxRowsForm<1, 1, 16, 1, 4, false>>(a, st);

@@ -359,7 +359,9 @@ def gated_mxfp4(input: Tensor, weight: MXFP4Weight, bias: Optional[Tensor] = Non
     from BF16 ``[..., K]`` in one kernel, the projections kept in 32 bits.  ``activation``: ``"silu"``, ``"gelu"`` or
     ``"gelu_tanh"``.  Differentiable once with respect to the input and the bias, by backward passes alone (forward-mode derivatives
     and the transformations of ``torch.func`` are refused); a call that may be differentiated keeps the projections (8 bytes a
-    gated value) for the backward pass.  ``torch.autocast`` as in :func:`linear_mxfp4`."""
+    gated value) for the backward pass.  There the projections' gradients are rounded to BF16, the operand of the product that makes the
+    input's, and that one once more: its error is 1.4 times that of one rounding (0.0023 against 0.0017 of its norm).  ``torch.autocast``
+    as in :func:`linear_mxfp4`."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
     if weight.out_features % 2:
