@@ -963,7 +963,9 @@ def _gated_activation(parent: nn.Module) -> Optional[str]:
     """The activation of a block that computes ``down_proj(act_fn(gate_proj(x)) * up_proj(x))`` and nothing else, by its parts and by
     what its forward does with them, whatever type its weights have and wherever they are; None for any other module."""
     parts = dict(parent.named_children())
-    if parts.keys() != {"gate_proj", "up_proj", "down_proj", "act_fn"} or any(True for _ in parent.parameters(recurse=False)):
+    if parts.keys() != {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+        return None
+    if any(True for _ in (*parent.parameters(recurse=False), *parent.buffers(recurse=False))):       # a factor, say, which a checkpoint may still change
         return None
     gate, up, down = (parts[n] for n in ("gate_proj", "up_proj", "down_proj"))
     if not all(type(m) is nn.Linear for m in (gate, up, down)) or gate.weight.shape != up.weight.shape or gate.in_features % 32:

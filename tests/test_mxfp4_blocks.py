@@ -64,6 +64,17 @@ class Swapped(Block):
         return self.down_proj(self.act_fn(self.up_proj(x)) * self.gate_proj(x))
 
 
+class Factor(Block):
+    """A factor in a buffer, one as it is made and whatever a checkpoint brings."""
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.register_buffer("factor", torch.ones((), dtype=torch.bfloat16))
+
+    def forward(self, x):
+        return super().forward(x) * self.factor
+
+
 class OneRowDiffers(Block):
     def forward(self, x):
         return super().forward(x) if x.numel() == x.size(-1) else super().forward(x).neg()
@@ -120,7 +131,7 @@ def filled(block, value):
     return block
 
 
-@pytest.mark.parametrize("kind", [Clamped, FarClamped, ClampedOutput, Dropped, TrainingOnly, Doubled, Residual, Scaled, Swapped, OneRowDiffers, NanToNum, Around, Pair])
+@pytest.mark.parametrize("kind", [Clamped, FarClamped, ClampedOutput, Dropped, TrainingOnly, Doubled, Residual, Scaled, Swapped, Factor, OneRowDiffers, NanToNum, Around, Pair])
 @pytest.mark.parametrize("weights", [None, 0.0, float("nan")])
 @pytest.mark.parametrize("training", [False, True])
 def test_blocks_that_do_something_else(kind, weights, training):
