@@ -9,7 +9,7 @@
 // Mostly the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32 columns start at
 // zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared memory: each row's 128
 // values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-31 of the largest in
-// its 128.  Where one lies below (it may be all that counts: the weights of the large ones can be zero), X is brought once more and multiplied as
+// its 128, and down to 2^-28 the sums of blocks are multiples of 2^-22, whose products with any scale are whole steps of 2^-149.  Where one lies below (it may be all that counts: the weights of the large ones can be zero), X is brought once more and multiplied as
 // it is, by the BF16 products of the next paragraph in a walk of its own.  (Looking for such
 // values costs most where X is most of the work: 1024 x 4096, 1 row 4.65 against 4.52 us, 151936 x 4096, 8 rows 62 against 61, 38000 x 12288, 24 rows
 // 118 against 115, gated 12288 x 4096, 16 rows 22.9 against 22.1.  A branch in every unit instead of the walk: 8 rows 66 us.)
@@ -31,6 +31,7 @@
 namespace bhi {
 
 constexpr int kMxRowWarpsMax = 16;
+constexpr uint32_t kMxRowsBelow = 28;             // powers of two between a group's largest value and the least that FP16 products serve
 
 struct MxRowsArgs {
     MxWeight W;
@@ -305,9 +306,9 @@ __global__ void __launch_bounds__(Form::kThreads, Form::kPerSm) mx_rows_kernel(c
                     if (job0 + q * teams >= jobs) break;
                     const uint32_t top = ends[q] & 0xFF80u;                  // without its mantissa
                     const uint32_t up = min(268u - (top >> 7), 253u);        // exponent field of 2^(14 - floor(log2 top))
-                    // the smallest is less than 2^-31 of it: a zero, or (next to an infinity or NaN that does not matter) a value that FP16 does not hold
-                    if ((ends[q] >> 16) + top > 0xFFFFu + (31u << 7) && top < 0x7F80u)
-                        for (int i = 0; i < 4; i++) far |= mx_below(w[q][i], top - (31u << 7));
+                    // the smallest is too far below: a zero, or (next to an infinity or NaN that does not matter) a value that FP16 products do not serve
+                    if ((ends[q] >> 16) + top > 0xFFFFu + (kMxRowsBelow << 7) && top < 0x7F80u)
+                        for (int i = 0; i < 4; i++) far |= mx_below(w[q][i], top - (kMxRowsBelow << 7));
                     const float scale = __uint_as_float(up << 23);
                     uint32_t h[4];
 #pragma unroll

@@ -65,6 +65,24 @@ def test_x_far_apart_inside_a_group(pkg, rows, M, K, spread):
         assert bool((err <= h.abs() * 2.0 ** -8 + slack + 2.0 ** -134).all())
 
 
+@pytest.mark.parametrize("rows,M,K", FORMS)
+@pytest.mark.parametrize("byte", [0, 1, 2, 3])
+@pytest.mark.parametrize("spread", [26, 29, 31])
+def test_x_far_apart_under_the_smallest_scales(pkg, rows, M, K, byte, spread):
+    """The same with X up to 2^100 and scales of 2^-127 and little more: what is left are ordinary numbers."""
+    codes, scales = weight(pkg, M, K, spread, byte, byte + 1)
+    g = torch.Generator(device=DEV).manual_seed(rows + spread)
+    x = (1 + torch.rand(rows, K, generator=g, device=DEV)) * 2.0 ** (100 - spread)
+    x[:, ::128] = 2.0 ** 100
+    x = x.to(torch.bfloat16)
+    codes[:, ::64] &= 0xF0                                       # zero codes where X is large
+    codes[:, 1:] &= 0x11                                         # and others up to 0.5
+    codes[:, 4:] = 0                                             # few of them: a sum of one group
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dense = w.get_weight().double()
+    within(F.linear(x, w), x.double() @ dense.T, x.double().abs() @ dense.abs().T, K)
+
+
 @pytest.mark.parametrize("rows", [1, 8, 16])
 def test_one_row_far_apart_leaves_the_others(pkg, rows):
     """A chunk of K whose X is far apart in one row is multiplied in another way; every row keeps its tolerance, chunk by chunk."""
