@@ -209,3 +209,33 @@ def test_plain_order_beyond_the_range_as_on_the_host(pkg):
         codes, scales = codes[:528].view(-1, 3 * 16), scales[:528].view(-1, 3)      # blocks side by side
         want, got = pkg.MXFP4Weight.from_packed(codes, scales), pkg.MXFP4Weight.from_packed(codes.to(DEV), scales.to(DEV))
         assert torch.equal(got.codes.cpu(), want.codes) and torch.equal(got.scales.cpu(), want.scales)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("byte", [0, 1, 60, 127, 128, 200, 251, 252])
+def test_input_gradient_under_scales_of_the_whole_range(pkg, rows, byte):
+    M, K = 150, 416
+    w = pkg.MXFP4Weight.from_packed(*weight(pkg, M, K, byte, byte, byte + 1))
+    dense = w.get_weight().double()
+    g = torch.Generator(device=DEV).manual_seed(rows + byte)
+    dy = torch.ldexp(torch.randn(rows, 152, generator=g, device=DEV).double(), torch.tensor(min(127 - byte, 120), device=DEV)).to(torch.bfloat16)
+    dx = pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, M, K)  # two columns more than the weight has rows: not read
+    dy = dy[:, :M].double()
+    within(dx, dy @ dense, dy.abs() @ dense.abs(), M)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_input_gradient_of_nan_blocks_and_of_nans(pkg, rows):
+    """A NaN block makes its 32 columns NaN, a NaN in dy its row; nothing else."""
+    M, K = 150, 416
+    codes, scales = weight(pkg, M, K, 5)
+    scales[149, 2], scales[3, 12] = 255, 255
+    w = pkg.MXFP4Weight.from_packed(codes, scales)
+    dy = torch.randn(rows, 152, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    dy[:, 150:] = math.nan                                       # past the weight's rows
+    want = torch.zeros(rows, K, dtype=torch.bool, device=DEV)
+    want[:, 64:96] = want[:, 384:416] = True
+    assert torch.equal(pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, M, K).isnan(), want)
+    dy[rows // 2, 7] = math.nan
+    want[rows // 2] = True
+    assert torch.equal(pkg.ops.mxfp4_linear_grad(dy, w.codes, w.scales, M, K).isnan(), want)
