@@ -9,10 +9,11 @@
 // Mostly the products are FP16 ones: the hardware's conversion makes two values of a code byte.  The sums of a block of 32 columns start at
 // zero and its scale applies to them, in 32 bits, so codes need no scaling of their own.  X is brought to FP16 in shared memory: each row's 128
 // values of a group to [2^14, 2^15) by a power of two that the sum gives back.  That is exact for every value down to 2^-31 of the largest in
-// its 128, and down to 2^-28 the sums of blocks are multiples of 2^-22, whose products with any scale are whole steps of 2^-149.  Where one lies below (it may be all that counts: the weights of the large ones can be zero), X is brought once more and multiplied as
-// it is, by the BF16 products of the next paragraph in a walk of its own.  (Looking for such
-// values costs most where X is most of the work: 1024 x 4096, 1 row 4.65 against 4.52 us, 151936 x 4096, 8 rows 62 against 61, 38000 x 12288, 24 rows
-// 118 against 115, gated 12288 x 4096, 16 rows 22.9 against 22.1.  A branch in every unit instead of the walk: 8 rows 66 us.)
+// its 128, and down to 2^-28 the sums of blocks are multiples of 2^-22, whose products with any scale are whole steps of 2^-149.  Where one lies
+// below (it may be all that counts: the weights of the large ones can be zero), X is brought once more and multiplied as it is, by the BF16 products
+// of the next paragraph in a walk of its own.  (Looking for such values costs most where X is most of the work: 1024 x 4096, 1 row 4.65 against
+// 4.52 us, 151936 x 4096, 8 rows 62 against 61, 38000 x 12288, 24 rows 118 against 115, gated 12288 x 4096, 16 rows 22.9 against 22.1; where there
+// are some, 8 rows take 100 us.  A branch in every unit instead of the walk: 8 rows 66 us without any.)
 // With X's power of two, up to 2^25 in four blocks, sums can overflow under a scale of 2^103 or more where the output does not: outputs that are
 // not finite, of weight rows with large scales, are computed once more, one by one.  (Asking every unit for large scales took longer: 151936 x 4096, 1
 // row 64 against 62 us.  Looking at the scales first: 151936 x 4096, 8 rows with a NaN in one 94 us, not 1255; 17 rows without 116 us, not 112.)
